@@ -405,6 +405,70 @@ EG_API eg_status eg_op_topk(const float* logits, int n, int k, uint32_t* ids, fl
 EG_API eg_status eg_op_sample_topk(const uint32_t* ids, const float* vals, int k, float temp,
                                    float r, uint32_t* out, void* stream);
 
+/* ---------------- paged serving ops ----------------------------------------
+ * Operators over the paged cache of eg_seq_init_paged's kind: pools
+ * [n_pages][16][nkv][128] (f16 when kv_f16 else f32), row t of a sequence at
+ * row t % 16 of page pages[t / 16].  Positions, slots, page ids and lengths
+ * are read on the device, so a captured graph serves every step.  err: one
+ * device int (may be NULL), zero before the call, set to 1 when a value read
+ * on the device is out of range (what then happens is said at each call).
+ * They allocate nothing and keep nothing between calls; device pointers and
+ * stream belong to the current device. */
+/* ROPE_T + WRITE_KV_PAGE of T ragged token rows (kernels.js:588-618,
+ * :1657-1911): row t of qkv ([q | k | v], nh + 2 nkv heads of 128, ld floats
+ * from row to row) is the token at position pos[t] of slot slot[t].  k turned
+ * by its position and v go to row pos[t] - prefix_len of the slot's pages
+ * (pages [n_slots][max_pages]; a slot that continues a shared prefix holds
+ * only what follows it), each rounded once to the cache's type; q turned goes
+ * to q_out (rows ldq floats apart; NULL: q is not wanted; not qkv itself).
+ * The rotation is f32 in both cache types.  cos_t / sin_t: [table_len][128].
+ * pos[t] < 0: a padding row, nothing of it is read on or written.  A position
+ * outside the table or the slot's pages, a slot outside n_slots or a page
+ * outside the pool: err, and nothing is written for that row.  Two rows with
+ * the same slot and position in one call: either's values may stay.  qkv,
+ * q_out, caches and tables 16-byte aligned, ld and ldq multiples of 4. */
+EG_API eg_status eg_op_kv_append_paged(const float* qkv, int64_t ld, int T, const int* pos, const int* slot,
+                                       const uint32_t* pages, int n_slots, int max_pages, int n_pages,
+                                       int prefix_len, void* k_cache, void* v_cache, const float* cos_t,
+                                       const float* sin_t, int table_len, int nh, int nkv, int kv_f16,
+                                       float* q_out, int64_t ldq, int* err, void* stream);
+/* One decode token of each of nseq sequences that share a prefix
+ * (ATTN_PARTIAL_PAGED + ATTN_COMBINE, kernels.js:1657-1911, with the prefix
+ * computed once for all): q row b (turned, nh heads of 128, ldq floats from
+ * row to row) attends over the prefix_len rows of prefix_pages and then over
+ * the first lens[b] rows of the sequence's own pages (pages [nseq][max_pages]),
+ * scores scaled by 1/sqrt(128); out rows ldo floats apart.  f32 results for
+ * either cache type; |q|/8 and an f32 cache's values must lie in the f16 range.
+ * lens[b] = 0: the prefix alone; no key at all: zeros; lens[b] < 0: a padding
+ * sequence, its out row is left as it was.  lens[b] > max_len: err, max_len
+ * rows are used; a page outside the pool: err, its rows are left out.
+ * ws: eg_op_attn_shared_prefix_bytes bytes of device memory (16-byte aligned,
+ * no initial contents needed); calls that may overlap need one each. */
+EG_API eg_status eg_op_attn_shared_prefix_bytes(int nseq, int nh, int nkv, int prefix_len, int max_len,
+                                                uint64_t* bytes);
+EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq, const void* k_cache,
+                                          const void* v_cache, int n_pages, const uint32_t* prefix_pages,
+                                          int prefix_len, const uint32_t* pages, int max_pages, const int* lens,
+                                          int max_len, int nh, int nkv, int kv_f16, float* out, int64_t ldo,
+                                          void* ws, uint64_t ws_bytes, int* err, void* stream);
+/* A token per row of logits [rows][n] (ld floats from row to row) by given
+ * random numbers r[rows] (clamped to [0, 1], as eg_sample does): temperature,
+ * then top-k, top-p and min-p over the whole vocabulary, each a device array
+ * of one value per row or NULL (temperature 1, filter off).  Order and masked
+ * values are TOPK_SELECT's (kernels.js:785-813: value falling, ties to the
+ * lower id; NaN and values below -1e30 never taken); w = exp((x - max) / temp),
+ * temp <= 0 reads as 1 as in SAMPLE_TOPK (kernels.js:814-883; greedy is
+ * top_k = 1).  top_k <= 0, top_p >= 1 and min_p <= 0 are off; top_p keeps the
+ * shortest leading part with top_p of the mass that top-k left, min_p the
+ * tokens with w >= min_p; the best token always stays.  ids[row] = the first
+ * token whose running mass reaches r times the mass kept, probs[row] (NULL:
+ * not wanted) its share of that mass.  A row with nothing to take: id
+ * 0xffffffff, share 0.  Masses are sums of integers: the same inputs give the
+ * same bits. */
+EG_API eg_status eg_op_sample_filtered(const float* logits, int64_t ld, int rows, int n, const float* temp,
+                                       const int* top_k, const float* top_p, const float* min_p, const float* r,
+                                       uint32_t* ids, float* probs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,6 +119,12 @@ _SIGS = {
     "eg_op_argmax": (i32, [vp, i32, vp, vp]),
     "eg_op_topk": (i32, [vp, i32, i32, vp, vp, vp]),
     "eg_op_sample_topk": (i32, [vp, vp, i32, f32, f32, vp, vp]),
+    "eg_op_kv_append_paged": (i32, [vp, i64, i32, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, i32,
+                                    i32, vp, i64, vp, vp]),
+    "eg_op_attn_shared_prefix_bytes": (i32, [i32, i32, i32, i32, i32, C.POINTER(u64)]),
+    "eg_op_attn_shared_prefix": (i32, [vp, i64, i32, vp, vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, vp, i64,
+                                       vp, u64, vp, vp]),
+    "eg_op_sample_filtered": (i32, [vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "eg_synth_normal": (None, [vp, i64, u64, f64, i64]),
     "eg_synth_stream_at": (u64, [u64, u64]),
 }

@@ -1,0 +1,579 @@
+// eg_paged.cu -- operators on a paged K/V cache: the rotated append of ragged
+// token rows, and decode attention for a batch that shares a prefix.
+//
+// The cache is the paged slots' (WRITE_KV_PAGE / ATTN_PARTIAL_PAGED,
+// kernels.js:1657-1911): pools [n_pages][16][nkv][128] of f16 or f32, row t of
+// a sequence at physical row pages[t / 16] * 16 + t % 16.  Page ids and
+// lengths live on the device, so a captured graph serves every step.
+#include <math.h>
+#include <algorithm>
+#include <type_traits>
+
+#include "eg_common.cuh"
+#include "eg_device.cuh"
+#include "eg_host.h"
+#include "emberglass.h"
+
+namespace eg {
+namespace {
+
+constexpr int kPage = 16;  // rows of a page
+
+// ======================================================================
+// Append: RoPE(k) and v of T token rows into the pool, RoPE(q) beside it
+// ======================================================================
+struct AppendArgs {
+  const float* qkv;
+  long long ld;
+  int T;
+  const int* pos;
+  const int* slot;
+  const uint32_t* pages;
+  int n_slots, max_pages, n_pages, prefix_len;
+  void* kc;
+  void* vc;
+  const float* cosT;
+  const float* sinT;
+  int table_len, nh, nkv;
+  float* q_out;
+  long long ldq;
+  int* err;
+};
+
+// A head of a token is 16 lanes: lane l holds dims 4l..4l+3 and their RoPE
+// partners 64 + 4l.., so a pair is turned in one thread (rope_pair, f32:
+// two rounded products and one sum) and rounded once, to the cache's type.
+template <typename KVT>
+__device__ __forceinline__ void store4(KVT* d, float4 v);
+template <>
+__device__ __forceinline__ void store4<float>(float* d, float4 v) {
+  *reinterpret_cast<float4*>(d) = v;
+}
+template <>
+__device__ __forceinline__ void store4<__half>(__half* d, float4 v) {
+  *reinterpret_cast<uint2*>(d) =
+      make_uint2(h2_bits(__floats2half2_rn(v.x, v.y)), h2_bits(__floats2half2_rn(v.z, v.w)));
+}
+
+template <typename KVT>
+__global__ void __launch_bounds__(256) kv_append_paged_kernel(AppendArgs a) {
+  const int H = a.nh + 2 * a.nkv, l = threadIdx.x & 15;
+  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
+  if (item >= (long long)a.T * H) return;
+  const int t = (int)(item / H), h = (int)(item - (long long)t * H);
+  if (h < a.nh && !a.q_out) return;
+  const float* src = a.qkv + t * a.ld + h * kHeadDim + 4 * l;
+  float4 lo = __ldcs(reinterpret_cast<const float4*>(src));
+  float4 hi = __ldcs(reinterpret_cast<const float4*>(src + kHeadDim / 2));
+  const int pos = __ldg(a.pos + t), s = __ldg(a.slot + t);
+  if (pos < 0) return;  // a padding row
+  const int row = pos - a.prefix_len;
+  bool ok = pos < a.table_len && row >= 0 && s >= 0 && s < a.n_slots && row / kPage < a.max_pages;
+  uint32_t page = 0;
+  if (ok) {
+    page = __ldg(a.pages + (size_t)s * a.max_pages + row / kPage);
+    ok = page < (uint32_t)a.n_pages;
+  }
+  if (!ok) {
+    if (a.err && l == 0) *a.err = 1;
+    return;
+  }
+  if (h < a.nh + a.nkv) {
+    const float4 c = __ldg(reinterpret_cast<const float4*>(a.cosT + (size_t)pos * kHeadDim + 4 * l));
+    const float4 n = __ldg(reinterpret_cast<const float4*>(a.sinT + (size_t)pos * kHeadDim + 4 * l));
+    rope_pair(lo.x, hi.x, c.x, n.x, 0);
+    rope_pair(lo.y, hi.y, c.y, n.y, 0);
+    rope_pair(lo.z, hi.z, c.z, n.z, 0);
+    rope_pair(lo.w, hi.w, c.w, n.w, 0);
+  }
+  if (h < a.nh) {
+    float* d = a.q_out + t * a.ldq + h * kHeadDim + 4 * l;
+    store4(d, lo);
+    store4(d + kHeadDim / 2, hi);
+    return;
+  }
+  const int kvh = h < a.nh + a.nkv ? h - a.nh : h - a.nh - a.nkv;
+  KVT* d = static_cast<KVT*>(h < a.nh + a.nkv ? a.kc : a.vc) +
+           (((size_t)page * kPage + row % kPage) * a.nkv + kvh) * kHeadDim + 4 * l;
+  store4(d, lo);
+  store4(d + kHeadDim / 2, hi);
+}
+
+// ======================================================================
+// Decode attention over a shared prefix
+// ======================================================================
+// Row r = b * G + g of a KV head is query head kvh * G + g of sequence b
+// (G = nh / nkv).  o = softmax(q k^T / sqrt(128)) v over the prefix's keys and
+// the sequence's own.  The keys are cut into splits; each split of a row
+// gives (m, l, o) with m the running maximum of s2 = q.k * log2(e)/sqrt(128),
+// l = sum p, o = sum p v, p = 2^(s2 - m + kPBits), and the combine weighs the
+// splits by 2^(m - max m).  kPBits lifts p to (0, 2^14]: its f16 hi + lo parts
+// then keep an absolute error of 2^-39 of the largest weight, so many small
+// weights beside one large one are not lost below the f16 range.
+constexpr float kPBits = 14.f;
+constexpr int kWarps = 4;       // warps of a CTA, each with its own 16-key tiles
+constexpr int kSms = 148;       // plans are made for the B200's SM count
+
+struct SharedPlan {
+  int G, gch;          // query heads per KV head; chunks of 8 of them
+  int rows;            // nseq * G rows per KV head
+  int pref_keys, n_pref, row_groups;  // keys per prefix split, splits, groups of 8 rows
+  int suf_keys, n_suf;                // keys per suffix split, most splits of a sequence
+};
+
+struct SharedArgs {
+  const float* q;
+  long long ldq;
+  int nseq, nh, nkv;
+  const void* kc;
+  const void* vc;
+  uint32_t n_pages;
+  const uint32_t* prefix_pages;
+  int prefix_len;
+  const uint32_t* pages;
+  int max_pages;
+  const int* lens;
+  int max_len;
+  float* out;
+  long long ldo;
+  float *pm, *pl, *po;  // [split][nseq * nh] and [...][128]
+  int* err;
+  SharedPlan p;
+};
+
+int round_up(int x, int m) { return (x + m - 1) / m * m; }
+
+SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len) {
+  SharedPlan p;
+  p.G = nh / nkv;
+  p.gch = (p.G + 7) / 8;
+  p.rows = nseq * p.G;
+  p.row_groups = (p.rows + 7) / 8;
+  // about four CTAs an SM, never under 128 keys a split
+  const long long units = (long long)p.row_groups * nkv;
+  const long long want = std::max(1LL, 4LL * kSms / units);
+  p.pref_keys = std::max(128, round_up((int)((prefix_len + want - 1) / want), 64));
+  p.n_pref = (prefix_len + p.pref_keys - 1) / p.pref_keys;
+  p.suf_keys = 128;
+  p.n_suf = (max_len + p.suf_keys - 1) / p.suf_keys;
+  return p;
+}
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+
+// One warp's walk over the 16-key tiles of a key range, 8 rows at a time.
+// S^T = K q^T and O^T = V^T p^T as mma.sync m16n8k16 (16 keys or dims x 8
+// rows), so the 8 query heads of a group fill the n side exactly.  q and p are
+// f16 hi + lo pairs (two products); with an f32 cache K and V are split too
+// (three products, the lo.lo one left out: 2^-22 of the product).
+template <typename KVT>
+struct WarpTile {
+  static constexpr int kRow = kHeadDim * (int)sizeof(KVT);  // bytes of a staged row
+  static constexpr int kBytes = 2 * kPage * kRow;           // K and V of one tile
+  static constexpr int kStages = 2;
+  static constexpr int kChunks = kRow / 16;
+};
+
+// 16-byte chunk c of staged row r, XOR-swizzled: 8 rows' chunks of one column
+// lie in different banks.
+template <typename KVT>
+__device__ __forceinline__ int tile_off(int r, int c) {
+  return r * WarpTile<KVT>::kRow + ((c ^ (r & 7)) << 4);
+}
+
+template <typename KVT>
+__device__ __forceinline__ void tile_load(unsigned char* st, const SharedArgs& a, int kvh, uint32_t page, int nv) {
+  using W = WarpTile<KVT>;
+  const int lane = threadIdx.x & 31;
+  const size_t base = ((size_t)page * kPage * a.nkv + kvh) * kHeadDim * sizeof(KVT);
+  const char* k = static_cast<const char*>(a.kc) + base;
+  const char* v = static_cast<const char*>(a.vc) + base;
+  const size_t rs = (size_t)a.nkv * kHeadDim * sizeof(KVT);
+#pragma unroll
+  for (int i = lane; i < kPage * W::kChunks; i += 32) {
+    const int r = i / W::kChunks, c = i % W::kChunks;
+    const size_t off = r < nv ? r * rs + c * 16 : 0;  // rows past the end are filled with zeros
+    cp_async16(st + tile_off<KVT>(r, c), k + off, r < nv ? 16 : 0);
+    cp_async16(st + kPage * W::kRow + tile_off<KVT>(r, c), v + off, r < nv ? 16 : 0);
+  }
+}
+
+// (16 keys x 16 dims at dim 16 ks) as A fragments, hi and (f32 cache) lo
+__device__ __forceinline__ void k_frag(const unsigned char* st, int ks, uint32_t (&h)[4], uint32_t (&)[4], __half) {
+  const int lane = threadIdx.x & 31, i = lane >> 3, r = (lane & 7) + 8 * (i & 1);
+  ldsm_x4(smem_addr(st + tile_off<__half>(r, 2 * ks + (i >> 1))), h[0], h[1], h[2], h[3]);
+}
+__device__ __forceinline__ void k_frag(const unsigned char* st, int ks, uint32_t (&h)[4], uint32_t (&l)[4], float) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = g + 8 * (i & 1), d = 16 * ks + 8 * (i >> 1) + 2 * tq;
+    const float2 x = *reinterpret_cast<const float2*>(st + tile_off<float>(r, d >> 2) + (d & 3) * 4);
+    split2(x.x, x.y, h[i], l[i]);
+  }
+}
+// (16 dims at 16 dt x 16 keys) of V^T as A fragments
+__device__ __forceinline__ void v_frag(const unsigned char* st, int dt, uint32_t (&h)[4], uint32_t (&)[4], __half) {
+  const int lane = threadIdx.x & 31, i = lane >> 3, r = (lane & 7) + 8 * (i >> 1);
+  ldsm_x4_t(smem_addr(st + tile_off<__half>(r, 2 * dt + (i & 1))), h[0], h[1], h[2], h[3]);
+}
+__device__ __forceinline__ void v_frag(const unsigned char* st, int dt, uint32_t (&h)[4], uint32_t (&l)[4], float) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int d = 16 * dt + g + 8 * (i & 1), r = 8 * (i >> 1) + 2 * tq;
+    const float x = *reinterpret_cast<const float*>(st + tile_off<float>(r, d >> 2) + (d & 3) * 4);
+    const float y = *reinterpret_cast<const float*>(st + tile_off<float>(r + 1, d >> 2) + (d & 3) * 4);
+    split2(x, y, h[i], l[i]);
+  }
+}
+
+// CTA = one split of the keys for up to 8 rows of one KV head.  Blocks
+// [0, prefix blocks) take the prefix, the others the suffixes.
+template <typename KVT>
+__global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_constant__ SharedArgs a) {
+  using W = WarpTile<KVT>;
+  constexpr bool F32 = std::is_same<KVT, float>::value;
+  extern __shared__ __align__(128) unsigned char sm[];
+  __shared__ float sm_m[kWarps][8], sm_l[kWarps][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const SharedPlan& p = a.p;
+  const int G = p.G;
+
+  // the CTA's rows [row0, row0 + nrow) of KV head kvh and its keys [k0, k1)
+  int kvh, row0, nrow, k0, k1, split;
+  const uint32_t* table;
+  int blk = blockIdx.x;
+  const int pref_blocks = p.n_pref * p.row_groups * a.nkv;
+  if (blk < pref_blocks) {
+    const int rg = blk % p.row_groups;
+    blk /= p.row_groups;
+    kvh = blk % a.nkv;
+    split = blk / a.nkv;
+    row0 = 8 * rg;
+    nrow = min(8, p.rows - row0);
+    table = a.prefix_pages;
+    k0 = split * p.pref_keys;
+    k1 = min(a.prefix_len, k0 + p.pref_keys);
+  } else {
+    blk -= pref_blocks;
+    const int gc = blk % p.gch;
+    blk /= p.gch;
+    kvh = blk % a.nkv;
+    blk /= a.nkv;
+    const int b = blk % a.nseq;
+    split = blk / a.nseq;
+    row0 = b * G + 8 * gc;
+    nrow = min(8, G - 8 * gc);
+    table = a.pages + (size_t)b * a.max_pages;
+    const int len = __ldg(a.lens + b);
+    if (len > a.max_len && a.err && threadIdx.x == 0) *a.err = 1;
+    k0 = split * p.suf_keys;
+    k1 = min(min(len, a.max_len), k0 + p.suf_keys);
+    if (k0 >= k1) return;
+    split += p.n_pref;
+  }
+
+  unsigned char* st = sm + warp * W::kStages * W::kBytes;
+  const int ntile = (k1 - k0 + kPage - 1) / kPage;
+  // the warp's tiles: warp, warp + kWarps, ...
+  auto page_of = [&](int t) -> uint32_t { return t < ntile ? __ldg(table + k0 / kPage + t) : 0u; };
+  auto issue = [&](int t, uint32_t page, int stage) -> int {
+    int nv = t < ntile ? min(kPage, k1 - k0 - t * kPage) : 0;
+    if (nv > 0 && page >= a.n_pages) {  // a page outside the pool: its keys are left out
+      nv = 0;
+      if (a.err && lane == 0) *a.err = 1;
+    }
+    if (t < ntile) tile_load<KVT>(st + stage * W::kBytes, a, kvh, nv > 0 ? page : 0u, nv);
+    cp_async_commit();
+    return nv;
+  };
+  int nv_cur = issue(warp, page_of(warp), 0);
+  uint32_t page_next = page_of(warp + kWarps);
+
+  // q of the rows as B fragments: lane (g, tq) holds row g's dims 2 tq.. of each k-step
+  uint32_t qh[8][2], ql[8][2];
+  {
+    const int r = row0 + g;
+    const bool on = g < nrow;
+    const float* q = a.q + (on ? (long long)(r / G) * a.ldq + (kvh * G + r % G) * kHeadDim : 0) + 2 * tq;
+    const float c = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const float2 x = on ? __ldg(reinterpret_cast<const float2*>(q + 16 * ks + 8 * j)) : make_float2(0.f, 0.f);
+        split2(x.x * c, x.y * c, qh[ks][j], ql[ks][j]);
+      }
+  }
+  float O[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; j++) O[j][0] = O[j][1] = O[j][2] = O[j][3] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows 2 tq and 2 tq + 1
+
+  int stage = 0;
+  for (int t = warp; t < ntile; t += kWarps) {
+    const int nv_next = issue(t + kWarps, page_next, stage ^ 1);
+    page_next = page_of(t + 2 * kWarps);
+    cp_async_wait<1>();
+    __syncwarp();
+    const unsigned char* ks_ = st + stage * W::kBytes;
+    const unsigned char* vs_ = ks_ + kPage * W::kRow;
+    float S[4] = {0.f, 0.f, 0.f, 0.f}, S2[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t fh[4], fl[4];
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++) {
+      k_frag(ks_, ks, fh, fl, KVT());
+      mma16816(S, fh, qh[ks][0], qh[ks][1]);
+      mma16816(S2, fh, ql[ks][0], ql[ks][1]);
+      if (F32) mma16816(S2, fl, qh[ks][0], qh[ks][1]);
+    }
+    // keys g (S[0], S[1]) and g + 8 (S[2], S[3]) for rows 2 tq, 2 tq + 1
+    const bool v0 = g < nv_cur, v1 = g + 8 < nv_cur;
+    const float s0 = v0 ? S[0] + S2[0] : -INFINITY, s1 = v0 ? S[1] + S2[1] : -INFINITY;
+    const float s2 = v1 ? S[2] + S2[2] : -INFINITY, s3 = v1 ? S[3] + S2[3] : -INFINITY;
+    float n0 = fmaxf(s0, s2), n1 = fmaxf(s1, s3);
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) {
+      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+    }
+    n0 = fmaxf(n0, m0);
+    n1 = fmaxf(n1, m1);
+    // no key so far (or every score -inf): a finite base keeps 2^(-inf - base) = 0
+    const float b0 = n0 == -INFINITY ? 0.f : n0 - kPBits, b1 = n1 == -INFINITY ? 0.f : n1 - kPBits;
+    const float c0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), c1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
+    m0 = n0;
+    m1 = n1;
+    const float p0 = exp2f(s0 - b0), p1 = exp2f(s1 - b1), p2 = exp2f(s2 - b0), p3 = exp2f(s3 - b1);
+    l0 = l0 * c0 + (p0 + p2);
+    l1 = l1 * c1 + (p1 + p3);
+    uint32_t ph0, pl0, ph1, pl1;
+    split2(p0, p1, ph0, pl0);
+    split2(p2, p3, ph1, pl1);
+    ph0 = movmatrix(ph0);
+    ph1 = movmatrix(ph1);
+    pl0 = movmatrix(pl0);
+    pl1 = movmatrix(pl1);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      O[j][0] *= c0;
+      O[j][1] *= c1;
+      O[j][2] *= c0;
+      O[j][3] *= c1;
+      v_frag(vs_, j, fh, fl, KVT());
+      mma16816(O[j], fh, ph0, ph1);
+      mma16816(O[j], fh, pl0, pl1);
+      if (F32) mma16816(O[j], fl, ph0, ph1);
+    }
+    __syncwarp();
+    nv_cur = nv_next;
+    stage ^= 1;
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int o = 4; o <= 16; o <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+  }
+  if (g == 0) {
+    sm_m[warp][2 * tq] = m0;
+    sm_m[warp][2 * tq + 1] = m1;
+    sm_l[warp][2 * tq] = l0;
+    sm_l[warp][2 * tq + 1] = l1;
+  }
+  __syncthreads();  // every warp's tiles are consumed: the staging becomes [warp][8][128] f32
+  float* so = reinterpret_cast<float*>(sm);
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    float* d = so + (warp * 8 + 2 * tq) * kHeadDim + 16 * j + g;
+    d[0] = O[j][0];
+    d[kHeadDim] = O[j][1];
+    d[8] = O[j][2];
+    d[kHeadDim + 8] = O[j][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nrow * 32; i += 32 * kWarps) {
+    const int r = i >> 5, c = i & 31;
+    float mm = sm_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kWarps; w++) mm = fmaxf(mm, sm_m[w][r]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+      const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2f(sm_m[w][r] - mm);
+      const float4 x = reinterpret_cast<const float4*>(so + (w * 8 + r) * kHeadDim)[c];
+      l += f * sm_l[w][r];
+      o.x += f * x.x;
+      o.y += f * x.y;
+      o.z += f * x.z;
+      o.w += f * x.w;
+    }
+    const int rr = row0 + r;
+    const size_t at = (size_t)split * a.nseq * a.nh + (size_t)(rr / G) * a.nh + kvh * G + rr % G;
+    if (c == 0) {
+      a.pm[at] = mm;
+      a.pl[at] = l;
+    }
+    reinterpret_cast<float4*>(a.po + at * kHeadDim)[c] = o;
+  }
+}
+
+// One warp per (sequence, head): the splits' (m, l, o) weighed and divided.
+__global__ void __launch_bounds__(128) attn_shared_combine(const __grid_constant__ SharedArgs a) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.nseq * a.nh) return;
+  const int b = row / a.nh, len = __ldg(a.lens + b);
+  if (len < 0) return;  // a padding sequence: its row stays as it is
+  const size_t n = (size_t)a.nseq * a.nh;
+  const int ns = a.p.n_pref + (min(len, a.max_len) + a.p.suf_keys - 1) / a.p.suf_keys;
+  float m = -INFINITY;
+  for (int s = 0; s < ns; s++) m = fmaxf(m, __ldg(a.pm + s * n + row));
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < ns; s++) {
+    const float ms = __ldg(a.pm + s * n + row);
+    const float f = ms == -INFINITY ? 0.f : exp2f(ms - m);
+    const float4 x = __ldg(reinterpret_cast<const float4*>(a.po + (s * n + row) * kHeadDim) + lane);
+    l += f * __ldg(a.pl + s * n + row);
+    o.x += f * x.x;
+    o.y += f * x.y;
+    o.z += f * x.z;
+    o.w += f * x.w;
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;  // no key at all: zeros
+  reinterpret_cast<float4*>(a.out + b * a.ldo + (row % a.nh) * kHeadDim)[lane] =
+      make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+template <typename KVT>
+cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
+  const long long pref = (long long)a.p.n_pref * a.p.row_groups * a.nkv;
+  const long long suf = (long long)a.p.n_suf * a.nseq * a.nkv * a.p.gch;
+  const int smem = kWarps * WarpTile<KVT>::kStages * WarpTile<KVT>::kBytes;
+  if (pref + suf > 0) {
+    cudaError_t e = cudaFuncSetAttribute(attn_shared_kernel<KVT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    attn_shared_kernel<KVT><<<(unsigned)(pref + suf), 32 * kWarps, smem, st>>>(a);
+  }
+  attn_shared_combine<<<(a.nseq * a.nh + 3) / 4, 128, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+bool misaligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) & (to - 1); }
+
+size_t shared_bytes(const SharedPlan& p, int nseq, int nh) {
+  return (size_t)(p.n_pref + p.n_suf) * nseq * nh * (kHeadDim + 2) * sizeof(float);
+}
+
+const char* shared_dims(int nseq, int nh, int nkv, int prefix_len, int max_len) {
+  if (nseq < 1 || nseq > 65536) return "need 1 <= nseq <= 65536";
+  if (nkv < 1 || nh < nkv || nh % nkv || nh > 1024) return "need nh a multiple of nkv, at most 1024";
+  if (prefix_len < 0 || max_len < 0 || prefix_len > (1 << 28) || max_len > (1 << 28))
+    return "need 0 <= prefix_len, max_len <= 2^28";
+  return nullptr;
+}
+
+}  // namespace
+}  // namespace eg
+
+using namespace eg;
+
+extern "C" {
+
+EG_API eg_status eg_op_kv_append_paged(const float* qkv, int64_t ld, int T, const int* pos, const int* slot,
+                                       const uint32_t* pages, int n_slots, int max_pages, int n_pages,
+                                       int prefix_len, void* k_cache, void* v_cache, const float* cos_t,
+                                       const float* sin_t, int table_len, int nh, int nkv, int kv_f16,
+                                       float* q_out, int64_t ldq, int* err, void* stream) {
+  if (T < 0 || nh < 0 || nkv < 1 || nh > 1024 || nkv > 1024) return fail(EG_ERR_ARG, "kv_append_paged: bad T or heads");
+  if (n_slots < 1 || max_pages < 1 || n_pages < 1 || prefix_len < 0 || table_len < 1)
+    return fail(EG_ERR_ARG, "kv_append_paged: bad page table, pool or table length");
+  if (n_pages > (1 << 27)) return fail(EG_ERR_ARG, "kv_append_paged: more than 2^27 pages");
+  if (T == 0) return EG_OK;
+  if (!qkv || !pos || !slot || !pages || !k_cache || !v_cache || !cos_t || !sin_t)
+    return fail(EG_ERR_ARG, "kv_append_paged: null argument");
+  const int H = nh + 2 * nkv;
+  if (ld < (int64_t)H * kHeadDim || ld % 4) return fail(EG_ERR_ARG, "kv_append_paged: row stride %lld below %d or not a multiple of 4", (long long)ld, H * kHeadDim);
+  if (q_out && (ldq < (int64_t)nh * kHeadDim || ldq % 4))
+    return fail(EG_ERR_ARG, "kv_append_paged: q_out row stride %lld below %d or not a multiple of 4", (long long)ldq, nh * kHeadDim);
+  if (misaligned(qkv, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16) || misaligned(cos_t, 16) ||
+      misaligned(sin_t, 16) || misaligned(q_out, 16))
+    return fail(EG_ERR_ARG, "kv_append_paged: 16-byte aligned buffers required");
+  AppendArgs a = {qkv, ld, T, pos, slot, pages, n_slots, max_pages, n_pages, prefix_len, k_cache, v_cache,
+                  cos_t, sin_t, table_len, nh, nkv, q_out, ldq, err};
+  const long long blocks = ((long long)T * H + 15) / 16;
+  if (blocks > 0x7fffffffLL) return fail(EG_ERR_ARG, "kv_append_paged: too many rows");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (kv_f16)
+    kv_append_paged_kernel<__half><<<(unsigned)blocks, 256, 0, st>>>(a);
+  else
+    kv_append_paged_kernel<float><<<(unsigned)blocks, 256, 0, st>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(EG_ERR_CUDA, "kv_append_paged: %s", cudaGetErrorString(e));
+  return EG_OK;
+}
+
+EG_API eg_status eg_op_attn_shared_prefix_bytes(int nseq, int nh, int nkv, int prefix_len, int max_len,
+                                                uint64_t* bytes) {
+  if (!bytes) return fail(EG_ERR_ARG, "attn_shared_prefix: null argument");
+  if (const char* why = shared_dims(nseq, nh, nkv, prefix_len, max_len)) return fail(EG_ERR_ARG, "attn_shared_prefix: %s", why);
+  *bytes = std::max<size_t>(16, shared_bytes(shared_plan(nseq, nh, nkv, prefix_len, max_len), nseq, nh));
+  return EG_OK;
+}
+
+EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq, const void* k_cache,
+                                          const void* v_cache, int n_pages, const uint32_t* prefix_pages,
+                                          int prefix_len, const uint32_t* pages, int max_pages, const int* lens,
+                                          int max_len, int nh, int nkv, int kv_f16, float* out, int64_t ldo,
+                                          void* ws, uint64_t ws_bytes, int* err, void* stream) {
+  if (const char* why = shared_dims(nseq, nh, nkv, prefix_len, max_len)) return fail(EG_ERR_ARG, "attn_shared_prefix: %s", why);
+  if (!q || !k_cache || !v_cache || !lens || !out || !ws || (prefix_len > 0 && !prefix_pages) || (max_len > 0 && !pages))
+    return fail(EG_ERR_ARG, "attn_shared_prefix: null argument");
+  if (n_pages < 1 || max_pages < 0 || n_pages > (1 << 27)) return fail(EG_ERR_ARG, "attn_shared_prefix: bad pool or page table");
+  if ((long long)max_pages * kPage < max_len)
+    return fail(EG_ERR_ARG, "attn_shared_prefix: max_len %d > %d pages of %d", max_len, max_pages, kPage);
+  if (ldq < (int64_t)nh * kHeadDim || ldq % 4 || ldo < (int64_t)nh * kHeadDim || ldo % 4)
+    return fail(EG_ERR_ARG, "attn_shared_prefix: row strides must be multiples of 4, at least %d", nh * kHeadDim);
+  if (misaligned(q, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16) || misaligned(out, 16) || misaligned(ws, 16))
+    return fail(EG_ERR_ARG, "attn_shared_prefix: 16-byte aligned buffers required");
+  SharedArgs a = {};
+  a.p = shared_plan(nseq, nh, nkv, prefix_len, max_len);
+  const size_t need = shared_bytes(a.p, nseq, nh);
+  if (ws_bytes < need)
+    return fail(EG_ERR_ARG, "attn_shared_prefix: workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes, (unsigned long long)need);
+  a.q = q;
+  a.ldq = ldq;
+  a.nseq = nseq;
+  a.nh = nh;
+  a.nkv = nkv;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.n_pages = (uint32_t)n_pages;
+  a.prefix_pages = prefix_pages;
+  a.prefix_len = prefix_len;
+  a.pages = pages;
+  a.max_pages = max_pages;
+  a.lens = lens;
+  a.max_len = max_len;
+  a.out = out;
+  a.ldo = ldo;
+  const size_t rows = (size_t)(a.p.n_pref + a.p.n_suf) * nseq * nh;
+  a.po = static_cast<float*>(ws);
+  a.pm = a.po + rows * kHeadDim;
+  a.pl = a.pm + rows;
+  a.err = err;
+  const long long blocks = (long long)a.p.n_pref * a.p.row_groups * nkv + (long long)a.p.n_suf * nseq * nkv * a.p.gch;
+  if (blocks > 0x7fffffffLL) return fail(EG_ERR_ARG, "attn_shared_prefix: too many splits");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = kv_f16 ? launch_shared<__half>(a, st) : launch_shared<float>(a, st);
+  if (e != cudaSuccess) return fail(EG_ERR_CUDA, "attn_shared_prefix: %s", cudaGetErrorString(e));
+  return EG_OK;
+}
+
+}  // extern "C"
