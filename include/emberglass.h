@@ -460,7 +460,7 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
  * temp <= 0 reads as 1 as in SAMPLE_TOPK (kernels.js:814-883; greedy is
  * top_k = 1).  top_k <= 0, top_p >= 1 and min_p <= 0 are off; top_p keeps the
  * shortest leading part with top_p of the mass that top-k left, min_p the
- * tokens with w >= min_p; the best token always stays.  ids[row] = the first
+ * tokens with w >= min_p; the best token always stays.  n <= 2^20.  ids[row] = the first
  * token whose running mass reaches r times the mass kept, probs[row] (NULL:
  * not wanted) its share of that mass.  A row with nothing to take: id
  * 0xffffffff, share 0.  Masses are sums of integers: the same inputs give the

@@ -6,6 +6,7 @@
 // a sequence at physical row pages[t / 16] * 16 + t % 16.  Page ids and
 // lengths live on the device, so a captured graph serves every step.
 #include <math.h>
+#include <string.h>
 #include <algorithm>
 #include <type_traits>
 
@@ -149,10 +150,12 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len) {
   p.gch = (p.G + 7) / 8;
   p.rows = nseq * p.G;
   p.row_groups = (p.rows + 7) / 8;
-  // about four CTAs an SM, never under 128 keys a split
+  // about four CTAs an SM, never under 128 keys a split and never above 1024:
+  // the tensor core's f32 sums lose about 2^-25.5 a step, all one way, so a
+  // warp's 16 tiles stay below 2^-20 (256 tiles of a 16384-key split: 1e-5)
   const long long units = (long long)p.row_groups * nkv;
   const long long want = std::max(1LL, 4LL * kSms / units);
-  p.pref_keys = std::max(128, round_up((int)((prefix_len + want - 1) / want), 64));
+  p.pref_keys = std::min(1024, std::max(128, round_up((int)((prefix_len + want - 1) / want), 64)));
   p.n_pref = (prefix_len + p.pref_keys - 1) / p.pref_keys;
   p.suf_keys = 128;
   p.n_suf = (max_len + p.suf_keys - 1) / p.suf_keys;
@@ -574,6 +577,26 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
   const cudaError_t e = kv_f16 ? launch_shared<__half>(a, st) : launch_shared<float>(a, st);
   if (e != cudaSuccess) return fail(EG_ERR_CUDA, "attn_shared_prefix: %s", cudaGetErrorString(e));
   return EG_OK;
+}
+
+// The same calls with their arguments as a block of 64-bit values, in order
+// (the Python wrappers').
+EG_API eg_status eg_packed_kv_append_paged(const char* block) {
+  int64_t a[22];
+  memcpy(a, block, sizeof a);
+  return eg_op_kv_append_paged((const float*)a[0], a[1], (int)a[2], (const int*)a[3], (const int*)a[4],
+                               (const uint32_t*)a[5], (int)a[6], (int)a[7], (int)a[8], (int)a[9], (void*)a[10],
+                               (void*)a[11], (const float*)a[12], (const float*)a[13], (int)a[14], (int)a[15],
+                               (int)a[16], (int)a[17], (float*)a[18], a[19], (int*)a[20], (void*)a[21]);
+}
+
+EG_API eg_status eg_packed_attn_shared_prefix(const char* block) {
+  int64_t a[21];
+  memcpy(a, block, sizeof a);
+  return eg_op_attn_shared_prefix((const float*)a[0], a[1], (int)a[2], (const void*)a[3], (const void*)a[4],
+                                  (int)a[5], (const uint32_t*)a[6], (int)a[7], (const uint32_t*)a[8], (int)a[9],
+                                  (const int*)a[10], (int)a[11], (int)a[12], (int)a[13], (int)a[14], (float*)a[15],
+                                  a[16], (void*)a[17], (uint64_t)a[18], (int*)a[19], (void*)a[20]);
 }
 
 }  // extern "C"

@@ -11,7 +11,10 @@
 //
 // Masses are sums of integers (w in fixed point), so no order of additions
 // changes a result.
+#include <cooperative_groups.h>
 #include <math.h>
+#include <string.h>
+#include <algorithm>
 
 #include "eg_common.cuh"
 #include "eg_host.h"
@@ -20,7 +23,7 @@
 namespace eg {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 
 struct SampleArgs {
   const float* logits;
@@ -168,9 +171,11 @@ __device__ void block_sums(long long& n, unsigned long long& m, GenericSmem& S) 
   m = b;
 }
 
-__global__ void __launch_bounds__(kThreads) sample_generic_kernel(SampleArgs a) {
-  __shared__ GenericSmem S;
-  const int row = blockIdx.x, n = a.n;
+// The whole row by one CTA, from global memory: right for every row, and the
+// path of those that the histogram form below leaves (an infinite maximum,
+// more than kList tokens in the bins that decide).
+__device__ __noinline__ void sample_generic(const SampleArgs& a, int row, GenericSmem& S) {
+  const int n = a.n;
   const float* x = a.logits + row * a.ld;
   const RowParams q = row_params(a, row);
   // the maximum and the number of candidates
@@ -249,6 +254,449 @@ __global__ void __launch_bounds__(kThreads) sample_generic_kernel(SampleArgs a) 
   }
 }
 
+// ======================================================================
+// Histogram form: a cluster of CTAs holds one row in shared memory
+// ======================================================================
+// Bins are equal steps of x below the maximum.  A token's weight is
+// 2^-26 q e^(-b step): b its bin, q an integer (26 bits + the half step's
+// spread), so one 64-bit shared-memory atomic adds its count (upper 18 bits)
+// and its q (lower 46).  The leader CTA turns the merged bins into running
+// counts and masses, which fix each filter's and the sample's bin; only the
+// tokens of those few bins are gathered and put in order, in the same integers.
+// Tokens past the last bin (64 below the maximum in x / t or more) weigh
+// nothing: 150,000 of them are 2^-74 of the best token.
+namespace cg = cooperative_groups;
+
+constexpr int kBins = 2048;        // the last one: past the range
+constexpr int kList = 1024;        // gathered tokens
+constexpr int kPer = kBins / kThreads;
+constexpr int kSlice = 19456;      // most tokens that a CTA stages (76 KB: two CTAs an SM)
+constexpr int kQBits = 26;
+constexpr unsigned long long kCountOne = 1ull << 46;
+
+struct Ranges {  // bins [lo, hi] of: top-k, top-p, min-p, the sample; slow: leave the row to sample_generic
+  int lo[4], hi[4], top, slow;
+};
+
+struct FastSmem {
+  union {
+    unsigned long long hist[kBins];  // then, in the leader, the mass above each bin
+    double above[kBins];
+  };
+  uint32_t count_above[kBins];
+  unsigned long long list[kList];    // order key << 32 | ~id: falling is TOPK_SELECT's order
+  uint32_t n_list;
+  float mx, mn;
+  float red[2][kThreads / 32];
+  double wsum[kThreads / 32];
+  uint32_t wcnt[kThreads / 32];
+  int cross[4];
+  Ranges rg;
+  // the leader's last reductions
+  double z, mass_p, mass_m, mass;
+  unsigned long long best;
+  uint32_t n_p, n_m;
+};
+
+struct Bins {
+  float xmax, sh, sl, step;  // 1 / bin width as a hi + lo pair; step: bin width / t
+  bool poly;                 // step <= 1/16: e^-u by its series
+  double stepd;
+};
+
+// The bin of a candidate and its q.  pos = (xmax - x) / width carried as
+// p + e (the difference exact by a two-term sum, the product by fma), so the
+// part beyond the bin is right to 2^-36 of the range.
+__device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
+  const float d = B.xmax - x;
+  const float bb = d - B.xmax;
+  const float dl = (B.xmax - (d - bb)) - (x + bb);  // d + dl = xmax - x
+  const float p = __fmul_rn(d, B.sh);  // not to be fused with p - r below: e holds its rounding
+  if (!(p < (float)(kBins - 2) + 0.5f)) {
+    q = 0;
+    return kBins - 1;
+  }
+  const float e = fmaf(d, B.sh, -p) + fmaf(d, B.sl, dl * B.sh);
+  const float r = rintf(p);
+  const float u = ((p - r) + e) * B.step;  // |u| <= step / 2 (a little more by e)
+  if (B.poly) {
+    // 1 - e^-u = u (1 - u/2 (1 - u/3 (1 - u/4 (1 - u/5)))): the next term is below 2^-39 for u <= 1/32
+    const float y = u * (1.f - u * 0.5f * (1.f - u * (1.f / 3.f) * (1.f - u * 0.25f * (1.f - u * 0.2f))));
+    q = (uint32_t)((1 << kQBits) - __float2int_rn(y * (float)(1 << kQBits)));
+  } else {
+    q = (uint32_t)__double2ll_rn(exp(-(double)u) * (double)(1 << kQBits));
+  }
+  return (int)r;
+}
+
+__device__ __forceinline__ double bin_unit(const Bins& B, int b) {  // the weight of q = 1 in bin b
+  return exp(-(double)b * B.stepd) * (1.0 / (1 << kQBits));
+}
+
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a, int staged) {
+  extern __shared__ __align__(16) unsigned char dsm[];
+  FastSmem& S = *reinterpret_cast<FastSmem*>(dsm);
+  float* xs = reinterpret_cast<float*>(dsm + sizeof(FastSmem));  // the slice; the leader's scratch at the end
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float* x = a.logits + row * a.ld;
+  const int per = (a.n + C - 1) / C, e0 = min(a.n, rank * per), e1 = min(a.n, e0 + per);
+  const RowParams P = row_params(a, row);
+
+  for (int i = tid; i < kBins; i += kThreads) S.hist[i] = 0;
+  if (tid == 0) S.n_list = 0;
+  // ---- the slice, its largest and smallest candidate
+  float mx = -INFINITY, mn = INFINITY;
+#pragma unroll 8
+  for (int i = e0 + tid; i < e1; i += kThreads) {
+    const float v = __ldg(x + i) + 0.f;
+    if (staged) xs[i - e0] = v;
+    if (v >= -1e30f) mx = fmaxf(mx, v), mn = fminf(mn, v);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+  }
+  if (lane == 0) S.red[0][warp] = mx, S.red[1][warp] = mn;
+  __syncthreads();
+  if (warp == 0) {
+    mx = lane < kThreads / 32 ? S.red[0][lane] : -INFINITY;
+    mn = lane < kThreads / 32 ? S.red[1][lane] : INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+    if (lane == 0) S.mx = mx, S.mn = mn;
+  }
+  cl.sync();
+  mx = -INFINITY, mn = INFINITY;
+  for (int c = 0; c < C; c++) {
+    const FastSmem* R = cl.map_shared_rank(&S, c);
+    mx = fmaxf(mx, R->mx);
+    mn = fminf(mn, R->mn);
+  }
+  const bool none = mx == -INFINITY, slow0 = mx == INFINITY;
+  Bins B;
+  if (!none && !slow0) {
+    // the range: all candidates, but at most 64 in x and 64 in x / t (whichever is more, steps of at most 2)
+    const double cap = fmax(64.0 * P.t, fmin(64.0, 2.0 * (kBins - 2) * P.t));
+    const double range = fmin((double)mx - (double)mn, cap);
+    const double s = fmin((kBins - 2) / range, 1e30);  // equal logits: one bin
+    B.xmax = mx;
+    B.sh = (float)s;
+    B.sl = (float)(s - (double)B.sh);
+    B.stepd = 1.0 / (s * P.t);
+    B.step = (float)B.stepd;
+    B.poly = B.stepd <= 0.0625;
+    for (int i = e0 + tid; i < e1; i += kThreads) {
+      const float v = staged ? xs[i - e0] : __ldg(x + i) + 0.f;
+      if (v >= -1e30f) {
+        uint32_t q;
+        const int b = bin_of(B, v, q);
+        atomicAdd(&S.hist[b], kCountOne + q);
+      }
+    }
+  }
+  cl.sync();
+  if (none || slow0) {  // the same in every CTA of the cluster
+    if (rank == 0) {
+      if (none) {
+        if (tid == 0) {
+          a.ids[row] = 0xffffffffu;
+          if (a.probs) a.probs[row] = 0.f;
+        }
+      } else {
+        sample_generic(a, row, *reinterpret_cast<GenericSmem*>(dsm));
+      }
+    }
+    return;
+  }
+  uint32_t ncand = 0;
+  double total = 0.0;
+  if (rank == 0) {
+    // ---- running counts and masses over the bins, kPer of them a thread
+    unsigned long long q[kPer];
+    uint32_t cnt[kPer];
+    double m[kPer], unit[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; j++) q[j] = 0, cnt[j] = 0;
+    for (int c = 0; c < C; c++) {
+      const ulonglong2* h = reinterpret_cast<const ulonglong2*>(cl.map_shared_rank(&S, c)->hist + tid * kPer);
+#pragma unroll
+      for (int j = 0; j < kPer; j += 2) {
+        const ulonglong2 v = h[j / 2];
+        q[j] += v.x & (kCountOne - 1);
+        cnt[j] += (uint32_t)(v.x >> 46);
+        q[j + 1] += v.y & (kCountOne - 1);
+        cnt[j + 1] += (uint32_t)(v.y >> 46);
+      }
+    }
+    double ms = 0.0;
+    uint32_t cs = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      const int b = tid * kPer + j;
+      unit[j] = b == kBins - 1 ? 0.0 : bin_unit(B, b);
+      m[j] = (double)q[j] * unit[j];
+      ms += m[j];
+      cs += cnt[j];
+    }
+    double mi = ms;
+    uint32_t ci = cs;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, mi, o);
+      const uint32_t w = __shfl_up_sync(0xffffffffu, ci, o);
+      if (lane >= o) mi += v, ci += w;
+    }
+    if (lane == 31) S.wsum[warp] = mi, S.wcnt[warp] = ci;
+    if (tid < 4) S.cross[tid] = kBins;
+    __syncthreads();  // every thread has read the bins; the sums are there
+    double mb = 0.0;
+    uint32_t cb = 0;
+    for (int w = 0; w < kThreads / 32; w++) {
+      if (w < warp) mb += S.wsum[w], cb += S.wcnt[w];
+      total += S.wsum[w];
+      ncand += S.wcnt[w];
+    }
+    double ab[kPer];
+    uint32_t ca[kPer];
+    double am = mb + (mi - ms);
+    uint32_t ac = cb + (ci - cs);
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      ab[j] = am;
+      ca[j] = ac;
+      S.above[tid * kPer + j] = am;
+      S.count_above[tid * kPer + j] = ac;
+      am += m[j];
+      ac += cnt[j];
+    }
+    // the first bin with tokens whose inclusive mass (count) reaches a target
+    auto cross_mass = [&](double t, int slot) {
+#pragma unroll
+      for (int j = 0; j < kPer; j++)
+        if (cnt[j] && tid * kPer + j < kBins - 1 && ab[j] + m[j] >= t) {
+          atomicMin(&S.cross[slot], tid * kPer + j);
+          break;
+        }
+    };
+    const bool k_on = P.k > 0 && (uint32_t)P.k < ncand;
+    if (k_on) {
+#pragma unroll
+      for (int j = 0; j < kPer; j++)
+        if (ca[j] < (uint32_t)P.k && (uint32_t)P.k <= ca[j] + cnt[j]) S.cross[0] = tid * kPer + j;
+    }
+    // the last bin that weighs anything: where a target at the very end falls
+    int last = -1;
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+      if (cnt[j] && tid * kPer + j < kBins - 1) last = tid * kPer + j;
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) S.red[0][warp] = (float)last;
+    __syncthreads();
+    for (int w = 0; w < kThreads / 32; w++) last = max(last, (int)S.red[0][w]);
+    const int kb = k_on ? S.cross[0] : kBins;
+    const bool k_in = kb < kBins - 1;  // top-k cuts inside the bins that weigh anything
+    auto mass_above = [&](int b) { return S.above[b]; };  // b = kBins - 1: all that weighs
+    const double z_lo = k_in ? mass_above(kb) : total, z_hi = k_in ? mass_above(kb + 1) : total;
+    int p_lo = -1, p_hi = -1, m_lo = -1, m_hi = -1;
+    double lo = z_lo, hi = z_hi;
+    if (P.p < 1.0) {
+      cross_mass(P.p * z_lo * (1.0 - 1e-12), 1);
+      cross_mass(P.p * z_hi * (1.0 + 1e-12), 2);
+      __syncthreads();
+      p_lo = min(S.cross[1], last);
+      p_hi = min(S.cross[2], last);
+      lo = fmin(lo, mass_above(p_lo));
+      hi = fmin(hi, mass_above(p_hi + 1));
+      __syncthreads();
+      if (tid < 4) S.cross[tid] = kBins;
+      __syncthreads();
+    }
+    if (P.minp > 0.0) {
+      const double pos = B.stepd > 0.0 ? -log(P.minp) / B.stepd : 0.0;
+      if (pos < kBins - 2) {
+        m_lo = max(0, (int)rint(pos - 0.01));
+        m_hi = max(0, min(kBins - 2, (int)rint(pos + 0.01)));
+        lo = fmin(lo, mass_above(m_lo));
+        hi = fmin(hi, mass_above(m_hi + 1));
+      }
+    }
+    hi = fmax(hi, 1.0);  // one token at least
+    cross_mass(P.r * lo * (1.0 - 1e-12), 1);
+    cross_mass(P.r * hi * (1.0 + 1e-12), 2);
+    __syncthreads();
+    if (tid == 0) {
+      const int s_lo = min(S.cross[1], last), s_hi = min(S.cross[2], last);
+      Ranges& R = S.rg;
+      R.lo[0] = k_in ? kb : 1, R.hi[0] = k_in ? kb : 0;
+      R.lo[1] = p_lo < 0 ? 1 : p_lo, R.hi[1] = p_lo < 0 ? 0 : p_hi;
+      R.lo[2] = m_lo < 0 ? 1 : m_lo, R.hi[2] = m_lo < 0 ? 0 : m_hi;
+      R.lo[3] = s_lo, R.hi[3] = s_hi;
+      R.top = max(max(R.hi[0], R.hi[1]), max(R.hi[2], R.hi[3]));
+      S.z = total;
+      S.n_p = S.n_m = 0xffffffffu;
+      S.best = ~0ull;
+    }
+  }
+  cl.sync();
+  // ---- the tokens of those bins, gathered in the leader
+  FastSmem* L = cl.map_shared_rank(&S, 0);
+  {
+    const Ranges R = L->rg;
+    for (int i0 = e0; i0 < e1; i0 += kThreads) {
+      const int i = i0 + tid;
+      float v = -INFINITY;
+      if (i < e1) v = staged ? xs[i - e0] : __ldg(x + i) + 0.f;
+      bool in = false;
+      if (v >= -1e30f) {
+        const float p = __fmul_rn(B.xmax - v, B.sh);
+        if (p <= (float)R.top + 0.5f || R.top >= kBins - 2) {
+          uint32_t q;
+          const int b = bin_of(B, v, q);
+#pragma unroll
+          for (int j = 0; j < 4; j++) in |= b >= R.lo[j] && b <= R.hi[j];
+        }
+      }
+      const uint32_t vote = __ballot_sync(0xffffffffu, in);
+      if (!vote) continue;
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&L->n_list, (uint32_t)__popc(vote));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(vote & ((1u << lane) - 1));
+      if (in && at < kList) L->list[at] = (unsigned long long)order_key(v) << 32 | (uint32_t)~i;
+    }
+  }
+  cl.sync();
+  if (rank != 0) return;
+
+  const int nl = (int)S.n_list;
+  if (nl > kList) {
+    __syncthreads();
+    sample_generic(a, row, *reinterpret_cast<GenericSmem*>(dsm));
+    return;
+  }
+  // ---- place and running mass of each gathered token, inside its bin
+  uint32_t* lq = reinterpret_cast<uint32_t*>(xs);  // the slice is done with
+  uint32_t* lb = lq + kList;
+  for (int i = tid; i < nl; i += kThreads) {
+    uint32_t q;
+    lb[i] = (uint32_t)bin_of(B, key_value((uint32_t)(S.list[i] >> 32)), q);
+    lq[i] = q;
+  }
+  __syncthreads();
+  constexpr int kMine = kList / kThreads;
+  uint32_t num[kMine];
+  double cum[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid + j * kThreads;
+    num[j] = 0xffffffffu;
+    cum[j] = 0.0;
+    if (i < nl) {
+      const unsigned long long me = S.list[i];
+      const uint32_t b = lb[i];
+      uint32_t c = 1;
+      unsigned long long q = lq[i];
+      for (int f = 0; f < nl; f++)
+        if (lb[f] == b && S.list[f] > me) c++, q += lq[f];
+      num[j] = S.count_above[b] + c;
+      cum[j] = S.above[b] + (double)q * bin_unit(B, (int)b);
+      if ((uint32_t)P.k == num[j] && P.k > 0) S.z = cum[j];
+    }
+  }
+  __syncthreads();
+  const Ranges R = S.rg;
+  const bool k_in = R.lo[0] <= R.hi[0];
+  const double z = S.z;
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid + j * kThreads;
+    if (i >= nl) continue;
+    if (P.p < 1.0 && cum[j] >= P.p * z) atomicMin(&S.n_p, num[j]);
+    if (R.lo[2] <= R.hi[2] && (int)lb[i] >= R.lo[2] && (int)lb[i] <= R.hi[2] &&
+        weight(key_value((uint32_t)(S.list[i] >> 32)), B.xmax, P.t) >= P.minp)
+      atomicMin(&S.n_m, ~num[j]);  // the largest place
+  }
+  __syncthreads();
+  uint32_t n_keep = k_in ? (uint32_t)P.k : 0xffffffffu;  // 0xffffffff: everything that weighs
+  double mass = z;
+  const uint32_t n_p = S.n_p;
+  uint32_t n_m = 0xffffffffu;
+  if (R.lo[2] <= R.hi[2]) n_m = S.n_m == 0xffffffffu ? S.count_above[R.lo[2]] : ~S.n_m;
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    if (num[j] == n_p && n_p != 0xffffffffu) S.mass_p = cum[j];
+    if (num[j] == n_m) S.mass_m = cum[j];
+  }
+  if (tid == 0 && R.lo[2] <= R.hi[2] && S.n_m == 0xffffffffu) S.mass_m = S.above[R.lo[2]];
+  __syncthreads();
+  if (n_p < n_keep) n_keep = n_p, mass = S.mass_p;
+  if (n_m < n_keep) n_keep = n_m, mass = S.mass_m;
+  if (n_keep == 0) n_keep = 1, mass = 1.0;  // min_p above 1: the best token stays
+  const double target = P.r * mass;
+#pragma unroll
+  for (int j = 0; j < kMine; j++)
+    if (num[j] <= n_keep && num[j] != 0xffffffffu && (cum[j] >= target || num[j] == n_keep))
+      atomicMin(&S.best, (unsigned long long)num[j]);
+  __syncthreads();
+  if (S.best == ~0ull) {  // the target lies past the gathered tokens by a rounding: the last of them
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < kMine; j++)
+      if (num[j] != 0xffffffffu && num[j] <= n_keep) most = max(most, num[j]);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) S.wcnt[warp] = most;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < kThreads / 32; w++) most = max(most, S.wcnt[w]);
+      S.best = most;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid + j * kThreads;
+    if (i < nl && num[j] == (uint32_t)S.best) {
+      const unsigned long long me = S.list[i];
+      a.ids[row] = ~(uint32_t)me;
+      if (a.probs) a.probs[row] = (float)(weight(key_value((uint32_t)(me >> 32)), B.xmax, P.t) / mass);
+    }
+  }
+}
+
+// CTAs of a row's cluster: enough that a slice fits, and more (slices of 2048
+// tokens or longer) while the rows leave SMs idle.
+int cluster_size(int rows, int n) {
+  int c = 1;
+  while (c < 8 && (long long)c * kSlice < n) c *= 2;
+  while (c < 8 && 2LL * rows * c <= 148 && n / (2 * c) >= 2048) c *= 2;
+  return c;
+}
+
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
+  const int c = cluster_size(a.rows, a.n), per = (a.n + c - 1) / c, staged = per <= kSlice;
+  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 : 0, kList * 8);
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)(sizeof(FastSmem) + kSlice * 4));
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = c;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.rows * c);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel, a, staged);
+}
+
 }  // namespace
 }  // namespace eg
 
@@ -259,16 +707,25 @@ extern "C" {
 EG_API eg_status eg_op_sample_filtered(const float* logits, int64_t ld, int rows, int n, const float* temp,
                                        const int* top_k, const float* top_p, const float* min_p, const float* r,
                                        uint32_t* ids, float* probs, void* stream) {
-  if (rows < 0 || n < 1 || n > (1 << 28)) return fail(EG_ERR_ARG, "sample_filtered: need rows >= 0 and 1 <= n <= 2^28");
+  if (rows < 0 || n < 1 || n > (1 << 20) || rows > (1 << 24)) return fail(EG_ERR_ARG, "sample_filtered: need rows >= 0 and 1 <= n <= 2^20");
   if (ld < n) return fail(EG_ERR_ARG, "sample_filtered: row stride %lld below n = %d", (long long)ld, n);
   if (rows == 0) return EG_OK;
   if (!logits || !r || !ids) return fail(EG_ERR_ARG, "sample_filtered: null argument");
   if (reinterpret_cast<uintptr_t>(logits) & 3) return fail(EG_ERR_ARG, "sample_filtered: logits must be 4-byte aligned");
   SampleArgs a = {logits, ld, rows, n, temp, top_k, top_p, min_p, r, ids, probs};
-  sample_generic_kernel<<<rows, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_sample(a, reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(EG_ERR_CUDA, "sample_filtered: %s", cudaGetErrorString(e));
   return EG_OK;
+}
+
+// The same call with its arguments as a block of 64-bit values, in order (the
+// Python wrapper's).
+EG_API eg_status eg_packed_sample_filtered(const char* block) {
+  int64_t a[12];
+  memcpy(a, block, sizeof a);
+  return eg_op_sample_filtered((const float*)a[0], a[1], (int)a[2], (int)a[3], (const float*)a[4], (const int*)a[5],
+                               (const float*)a[6], (const float*)a[7], (const float*)a[8], (uint32_t*)a[9],
+                               (float*)a[10], (void*)a[11]);
 }
 
 }  // extern "C"
