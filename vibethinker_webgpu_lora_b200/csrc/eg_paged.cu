@@ -5,6 +5,7 @@
 // kernels.js:1657-1911): pools [n_pages][16][nkv][128] of f16 or f32, row t of
 // a sequence at physical row pages[t / 16] * 16 + t % 16.  Page ids and
 // lengths live on the device, so a captured graph serves every step.
+#include <cuda.h>
 #include <math.h>
 #include <string.h>
 #include <algorithm>
@@ -13,6 +14,7 @@
 #include "eg_common.cuh"
 #include "eg_device.cuh"
 #include "eg_host.h"
+#include "eg_tc.cuh"
 #include "emberglass.h"
 
 namespace eg {
@@ -119,6 +121,7 @@ struct SharedPlan {
   int G, gch;          // query heads per KV head; chunks of 8 of them
   int rows;            // nseq * G rows per KV head
   int pref_keys, n_pref, row_groups;  // keys per prefix split, splits, groups of 8 rows
+  int tc, row_tiles;   // prefix on the tcgen05 tensor cores, in tiles of 128 rows
   int suf_keys, n_suf;                // keys per suffix split, most splits of a sequence
 };
 
@@ -144,18 +147,26 @@ struct SharedArgs {
 
 int round_up(int x, int m) { return (x + m - 1) / m * m; }
 
-SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len) {
+SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, int kv_f16) {
   SharedPlan p;
   p.G = nh / nkv;
   p.gch = (p.G + 7) / 8;
   p.rows = nseq * p.G;
   p.row_groups = (p.rows + 7) / 8;
+  p.row_tiles = (p.rows + 127) / 128;
+  p.tc = kv_f16 && p.rows > 8 && prefix_len >= 256;
+  if (p.tc) {
+    // one CTA an SM, an even number of 128-key blocks each
+    const int units = p.row_tiles * nkv, want = std::max(1, kSms / units);
+    p.pref_keys = round_up((prefix_len + want - 1) / want, 256);
+  } else {
   // about four CTAs an SM, never under 128 keys a split and never above 1024:
   // the tensor core's f32 sums lose about 2^-25.5 a step, all one way, so a
   // warp's 16 tiles stay below 2^-20 (256 tiles of a 16384-key split: 1e-5)
   const long long units = (long long)p.row_groups * nkv;
   const long long want = std::max(1LL, 4LL * kSms / units);
   p.pref_keys = std::min(1024, std::max(128, round_up((int)((prefix_len + want - 1) / want), 64)));
+  }
   p.n_pref = (prefix_len + p.pref_keys - 1) / p.pref_keys;
   p.suf_keys = 128;
   p.n_suf = (max_len + p.suf_keys - 1) / p.suf_keys;
@@ -251,7 +262,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
   int kvh, row0, nrow, k0, k1, split;
   const uint32_t* table;
   int blk = blockIdx.x;
-  const int pref_blocks = p.n_pref * p.row_groups * a.nkv;
+  const int pref_blocks = p.tc ? 0 : p.n_pref * p.row_groups * a.nkv;
   if (blk < pref_blocks) {
     const int rg = blk % p.row_groups;
     blk /= p.row_groups;
@@ -277,8 +288,11 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
     if (len > a.max_len && a.err && threadIdx.x == 0) *a.err = 1;
     k0 = split * p.suf_keys;
     k1 = min(min(len, a.max_len), k0 + p.suf_keys);
-    if (k0 >= k1) return;
     split += p.n_pref;
+    if (k0 >= k1) {
+      if (p.tc) pdl_wait();
+      return;
+    }
   }
 
   unsigned char* st = sm + warp * W::kStages * W::kBytes;
@@ -425,47 +439,488 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
     }
     reinterpret_cast<float4*>(a.po + at * kHeadDim)[c] = o;
   }
+  // launched beside the prefix kernel, whose results it does not need: its end
+  // waits for that kernel's, so that the combine, which follows it, finds both
+  if (p.tc) pdl_wait();
 }
 
-// One warp per (sequence, head): the splits' (m, l, o) weighed and divided.
+// ======================================================================
+// The prefix for many rows on the tcgen05 tensor cores (f16 cache)
+// ======================================================================
+// A CTA takes 128 rows of one KV head over one split of the prefix, in blocks
+// of 128 keys: S = q K^T (M = rows, N = keys; q as f16 hi + lo stacked on the
+// same K: 16 MMAs of K = 16), softmax by one thread a row from TMEM, P back to
+// TMEM as f16 hi + lo over S's own columns, O = P V (A from TMEM, V^T as the
+// key-major tile read MN-major; 16 MMAs).  Two warpgroups take the blocks in
+// turn, so one's softmax runs under the other's products.  O of a block is a
+// fresh accumulator added to the row's f32 registers: a TMEM sum over many
+// blocks would lose 2^-25.5 a step, all one way.
+// Warps: 0-3 and 4-7 softmax, 8 copies K, 9 copies V (TMA: a page of one KV
+// head is two boxes of 16 rows x 64 dims, 128-byte swizzle), 10 issues MMAs and
+// owns TMEM.
+constexpr int kTcThreads = 384, kTcBlock = 128;
+constexpr uint32_t kTcTile = 128 * kHeadDim * 2;  // 32 KB: 128 rows or keys of f16
+constexpr uint32_t kTcHalf = kTcTile / 2;         // 128 keys x 64 dims, 128-byte rows
+constexpr int kTcSmem = 6 * kTcTile;              // q hi, q lo, 2 x (K, V)
+constexpr uint32_t kTcCols = 512;                 // per warpgroup 128 of S / P and 128 of O
+constexpr int kTcPitch = kHeadDim + 4;            // floats a row of the closing exchange
+
+struct TcSmem {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], v_raw;
+  uint32_t tmem;
+  int err;
+  int nv[2][8];  // valid keys of each page of a stage's block
+  float m[128], l[128];
+};
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+// A from tensor memory: 128 lanes x 8 columns of f16 pairs
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Descriptor of a tile of 128-byte rows with the 128-byte swizzle: 8-row groups
+// sbo apart; MN-major: 64-element columns lbo apart (K-major: one column, the
+// next at another start).
+__device__ __forceinline__ uint64_t smem_desc_sw128(const void* p, uint32_t lbo, uint32_t sbo) {
+  return smem_desc(p, lbo, sbo) | (2ull << 61);
+}
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int dim, int head, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_addr(dst)),
+      "l"(map), "r"(dim), "r"(head), "r"(row), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// 16-byte chunk c of row r in a 128-row tile of core matrices (8 rows x 16 bytes)
+__device__ __forceinline__ uint32_t core_off(int r, int c) { return c * 2048 + (r >> 3) * 128 + (r & 7) * 16; }
+
+__global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __grid_constant__ SharedArgs a,
+                                                                      const __grid_constant__ CUtensorMap kmap,
+                                                                      const __grid_constant__ CUtensorMap vmap) {
+  extern __shared__ __align__(1024) unsigned char tsm[];
+  __shared__ TcSmem S;
+  unsigned char* qs = tsm;                  // q hi, then q lo
+  unsigned char* kvs = tsm + 2 * kTcTile;   // stage s: K at 2 s tiles, V one further
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const SharedPlan& p = a.p;
+  pdl_launch_dependents();
+  int blk = blockIdx.x;
+  const int tile = blk % p.row_tiles;
+  blk /= p.row_tiles;
+  const int kvh = blk % a.nkv, split = blk / a.nkv;
+  const int k0 = split * p.pref_keys, k1 = min(a.prefix_len, k0 + p.pref_keys);
+  const int nblk = (k1 - k0 + kTcBlock - 1) / kTcBlock;
+
+  if (tid == 0) {
+    S.err = 0;
+    mbar_init(&S.q_full, 256);
+    mbar_init(&S.v_raw, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&S.k_full[i], 1);
+      mbar_init(&S.k_empty[i], 1);
+      mbar_init(&S.v_full[i], 1);
+      mbar_init(&S.v_empty[i], 1);
+      mbar_init(&S.s_full[i], 1);
+      mbar_init(&S.p_full[i], 128);
+      mbar_init(&S.o_full[i], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 10) tmem_alloc(&S.tmem, kTcCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = S.tmem;
+  bool dead = false;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp < 10) {
+      // ------------------------------------------------ K (warp 8) and V (warp 9) of every block
+      const bool is_v = warp == 9;
+      const CUtensorMap* map = is_v ? &vmap : &kmap;
+      uint32_t raw = 0;
+      for (int j = 0; j < nblk; j++) {
+        const int st = j & 1, key0 = k0 + j * kTcBlock;
+        const int g = lane & 7, half = (lane >> 3) & 1;  // lanes 0-15: one box each
+        const int left = k1 - key0 - g * kPage;
+        uint32_t page = 0;
+        int nv = 0;
+        if (left > 0) {
+          page = __ldg(a.prefix_pages + key0 / kPage + g);
+          nv = min(kPage, left);
+          if (page >= a.n_pages) {  // a page outside the pool: its keys are left out
+            nv = 0;
+            if (a.err) *a.err = 1;
+          }
+        }
+        uint64_t* full = is_v ? &S.v_full[st] : &S.k_full[st];
+        if (!dead && !tc_wait(is_v ? &S.v_empty[st] : &S.k_empty[st], ((j >> 1) & 1) ^ 1, &S.err)) dead = true;
+        unsigned char* dst = kvs + (2 * st + is_v) * kTcTile;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, nv > 0 && lane < 16)) * (kTcTile / 16);
+        const bool whole = __all_sync(0xffffffffu, nv == kPage);
+        if (is_v && lane < 8) S.nv[st][lane] = nv;
+        // masked rows of V must be zeros (0 x NaN): such a block lands on v_raw, is mended, then is full
+        uint64_t* bar = is_v && !whole ? &S.v_raw : full;
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(bar, bytes);
+        __syncwarp();
+        if (lane < 16 && nv > 0)
+          tma_page(dst + half * kTcHalf + g * (kPage * 128), map, 64 * half, kvh, (int)(page * kPage), bar);
+        if (is_v && !whole) {
+          if (!dead && !tc_wait(&S.v_raw, raw, &S.err)) dead = true;
+          raw ^= 1;
+          for (int i = lane; i < 2 * 128 * 8; i += 32) {  // 16-byte pieces; a row's place is swizzled within itself only
+            const int hf = i >> 10, rr = (i >> 3) & 127;
+            const int n = __shfl_sync(0xffffffffu, nv, rr >> 4);
+            if ((rr & 15) >= n)
+              *reinterpret_cast<uint4*>(dst + hf * kTcHalf + rr * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full);
+        }
+      }
+      // every copy has landed before the CTA may end
+      for (int j = max(0, nblk - 2); j < nblk; j++)
+        tc_wait_bounded(is_v ? &S.v_full[j & 1] : &S.k_full[j & 1], (j >> 1) & 1);
+    } else if (warp == 10) {
+      // ------------------------------------------------ MMA issue
+      // D f32, A and B f16, M = N = 128; for P V the B operand (V) is MN-major
+      const uint32_t id_s = (1u << 4) | (16u << 17) | (8u << 24), id_o = id_s | (1u << 16);
+      if (!tc_wait(&S.q_full, 0, &S.err)) dead = true;
+      auto issue_s = [&](int j) {
+        const int w = j & 1;
+        if (!dead && !tc_wait(&S.k_full[w], (j >> 1) & 1, &S.err)) dead = true;
+        tc_fence_after();
+        if (lane == 0) {
+          const unsigned char* K = kvs + 2 * w * kTcTile;
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            mma_f16_ss(tmem + w * 256, smem_desc(qs + i * 4096, 2048, 128),
+                       smem_desc_sw128(K + ((i >> 2) & 1) * kTcHalf + (i & 3) * 32, 16, 1024), id_s, i > 0);
+          mma_commit(&S.s_full[w]);
+          mma_commit(&S.k_empty[w]);
+        }
+        __syncwarp();
+      };
+      issue_s(0);
+      if (nblk > 1) issue_s(1);
+      for (int j = 0; j < nblk; j++) {
+        const int w = j & 1;
+        if (!dead && !tc_wait(&S.v_full[w], (j >> 1) & 1, &S.err)) dead = true;
+        if (!dead && !tc_wait(&S.p_full[w], (j >> 1) & 1, &S.err)) dead = true;
+        tc_fence_after();
+        if (lane == 0) {
+          const unsigned char* V = kvs + (2 * w + 1) * kTcTile;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const uint32_t pc = tmem + w * 256 + 32 * (i >> 1) + 8 * (i & 1);
+            const uint64_t vd = smem_desc_sw128(V + i * 2048, kTcHalf, 1024);  // 16 keys of all dims
+            mma_f16_ts(tmem + w * 256 + 128, pc, vd, id_o, i > 0);
+            mma_f16_ts(tmem + w * 256 + 128, pc + 16, vd, id_o, true);
+          }
+          mma_commit(&S.o_full[w]);
+          mma_commit(&S.v_empty[w]);
+        }
+        __syncwarp();
+        if (j + 2 < nblk) issue_s(j + 2);  // over P of block j: the tensor core runs these in order
+      }
+      // every MMA is done before TMEM is freed, also when a wait gave up
+      for (int j = max(0, nblk - 2); j < nblk; j++) tc_wait_bounded(&S.o_full[j & 1], (j >> 1) & 1);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // ------------------------------------------------ softmax, one thread a row
+    const int w = warp >> 2, r = tid & 127, row = tile * 128 + r, G = p.G;
+    {
+      // q of the row, dims 64 w .. 64 w + 63, times log2(e) / sqrt(128), as f16 hi and lo
+      const bool on = row < p.rows;
+      const float c = 1.4426950408889634f * 0.08838834764831845f;
+      const float* q = a.q + (on ? (long long)(row / G) * a.ldq + (kvh * G + row % G) * kHeadDim + 64 * w : 0);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (on) {
+          x = __ldg(reinterpret_cast<const float4*>(q) + 2 * i);
+          y = __ldg(reinterpret_cast<const float4*>(q) + 2 * i + 1);
+        }
+        uint4 h, l;
+        split2(x.x * c, x.y * c, h.x, l.x);
+        split2(x.z * c, x.w * c, h.y, l.y);
+        split2(y.x * c, y.y * c, h.z, l.z);
+        split2(y.z * c, y.w * c, h.w, l.w);
+        *reinterpret_cast<uint4*>(qs + core_off(r, 8 * w + i)) = h;
+        *reinterpret_cast<uint4*>(qs + kTcTile + core_off(r, 8 * w + i)) = l;
+      }
+      fence_async_smem();
+      mbar_arrive(&S.q_full);
+    }
+    const uint32_t base = tmem + w * 256 + ((uint32_t)(32 * (warp & 3)) << 16);
+    float O[kHeadDim];
+#pragma unroll
+    for (int i = 0; i < kHeadDim; i++) O[i] = 0.f;
+    float m = -INFINITY, l = 0.f, corr = 0.f;
+    // O (scaled by corr of its block) += the block's accumulator
+    auto take_o = [&](int j) {
+      if (!dead && !tc_wait(&S.o_full[w], (j >> 1) & 1, &S.err)) dead = true;
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t v[32];
+        tmem_ld32(base + 128 + 32 * i, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int d = 0; d < 32; d++) O[32 * i + d] = fmaf(O[32 * i + d], corr, __uint_as_float(v[d]));
+      }
+    };
+    for (int j = w; j < nblk; j += 2) {
+      const int nkey = k1 - k0 - j * kTcBlock;
+      if (!dead && !tc_wait(&S.s_full[w], (j >> 1) & 1, &S.err)) dead = true;
+      if (j >= 2) take_o(j - 2);
+      // the block's valid keys: every page whole, but at the end of the prefix (or beside a bad page)
+      if (!dead && !tc_wait(&S.v_full[w], (j >> 1) & 1, &S.err)) dead = true;
+      bool whole = nkey >= kTcBlock;
+#pragma unroll
+      for (int g = 0; g < 8; g++) whole &= S.nv[w][g] == kPage;
+      tc_fence_after();
+      float mx = m;
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t v[32];
+          tmem_ld32(base + 32 * i, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int d = 0; d < 32; d++) mx = fmaxf(mx, __uint_as_float(v[d]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t v[32];
+          tmem_ld32(base + 32 * i, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int d = 0; d < 32; d++) {
+            if (d % kPage >= S.nv[w][2 * i + d / kPage]) v[d] = __float_as_uint(-INFINITY);
+            mx = fmaxf(mx, __uint_as_float(v[d]));
+          }
+          tmem_st32(base + 32 * i, v);
+        }
+        tmem_wait_st();
+      }
+      const float b = mx == -INFINITY ? 0.f : mx - kPBits;
+      corr = m == -INFINITY ? 0.f : ex2(m - mx);
+      m = mx;
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t v[32], o[32];
+        tmem_ld32(base + 32 * i, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int d = 0; d < 16; d++) {
+          const float x = ex2(__uint_as_float(v[2 * d]) - b), y = ex2(__uint_as_float(v[2 * d + 1]) - b);
+          s0 += x;
+          s1 += y;
+          split2(x, y, o[d], o[16 + d]);
+        }
+        tmem_st32(base + 32 * i, o);
+      }
+      l = l * corr + (s0 + s1);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&S.p_full[w]);
+    }
+    const int lastj = nblk - 1 - ((nblk - 1 - w) & 1);  // the warpgroup's last block
+    if (lastj >= 0 && w < nblk) take_o(lastj);
+    // ---- the two warpgroups' parts of a row joined (every MMA is done: both have their last O)
+    float* ex = reinterpret_cast<float*>(kvs);
+    if (w == 1) {
+      S.m[r] = m;
+      S.l[r] = l;
+    }
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    if (w == 1) {
+#pragma unroll
+      for (int i = 0; i < kHeadDim; i += 4)
+        *reinterpret_cast<float4*>(ex + r * kTcPitch + i) = make_float4(O[i], O[i + 1], O[i + 2], O[i + 3]);
+    }
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    if (w == 0) {
+      const float m1 = S.m[r], mm = fmaxf(m, m1);
+      const float f0 = m == -INFINITY ? 0.f : ex2(m - mm), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
+#pragma unroll
+      for (int i = 0; i < kHeadDim; i += 4) {
+        float4* d = reinterpret_cast<float4*>(ex + r * kTcPitch + i);
+        float4 x = *d;
+        x.x = O[i] * f0 + x.x * f1;
+        x.y = O[i + 1] * f0 + x.y * f1;
+        x.z = O[i + 2] * f0 + x.z * f1;
+        x.w = O[i + 3] * f0 + x.w * f1;
+        *d = x;
+      }
+      if (row < p.rows) {
+        const size_t at = (size_t)split * a.nseq * a.nh + (size_t)(row / G) * a.nh + kvh * G + row % G;
+        a.pm[at] = mm;
+        a.pl[at] = l * f0 + S.l[r] * f1;
+      }
+    }
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    for (int i = tid; i < 128 * 32; i += 256) {
+      const int rr = i >> 5, c = i & 31, gr = tile * 128 + rr;
+      if (gr >= p.rows) break;
+      const size_t at = (size_t)split * a.nseq * a.nh + (size_t)(gr / G) * a.nh + kvh * G + gr % G;
+      reinterpret_cast<float4*>(a.po + at * kHeadDim)[c] = reinterpret_cast<const float4*>(ex + rr * kTcPitch)[c];
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (tid == 0 && S.err && a.err) *a.err = 1;  // a bounded wait gave up
+  if (warp == 10) tmem_free(tmem, kTcCols);
+}
+
+// One warp per (sequence, head): lane s first holds split s's maximum and sum
+// (32 splits at a time), then the warp adds the splits' rows, eight loads in
+// flight.
 __global__ void __launch_bounds__(128) attn_shared_combine(const __grid_constant__ SharedArgs a) {
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  pdl_wait();
   if (row >= a.nseq * a.nh) return;
   const int b = row / a.nh, len = __ldg(a.lens + b);
   if (len < 0) return;  // a padding sequence: its row stays as it is
   const size_t n = (size_t)a.nseq * a.nh;
   const int ns = a.p.n_pref + (min(len, a.max_len) + a.p.suf_keys - 1) / a.p.suf_keys;
-  float m = -INFINITY;
-  for (int s = 0; s < ns; s++) m = fmaxf(m, __ldg(a.pm + s * n + row));
-  float l = 0.f;
+  float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < ns; s++) {
-    const float ms = __ldg(a.pm + s * n + row);
-    const float f = ms == -INFINITY ? 0.f : exp2f(ms - m);
-    const float4 x = __ldg(reinterpret_cast<const float4*>(a.po + (s * n + row) * kHeadDim) + lane);
-    l += f * __ldg(a.pl + s * n + row);
-    o.x += f * x.x;
-    o.y += f * x.y;
-    o.z += f * x.z;
-    o.w += f * x.w;
+  for (int s0 = 0; s0 < ns; s0 += 32) {
+    const int s = s0 + lane, cnt = min(32, ns - s0);
+    const float ms = s < ns ? __ldcg(a.pm + s * n + row) : -INFINITY, ls = s < ns ? __ldcg(a.pl + s * n + row) : 0.f;
+    const float nm = fmaxf(m, warp_max(ms));
+    const float f = ms == -INFINITY ? 0.f : exp2f(ms - nm), c = m == -INFINITY ? 0.f : exp2f(m - nm);
+    m = nm;
+    l = l * c + warp_sum(f * ls);
+    o.x *= c;
+    o.y *= c;
+    o.z *= c;
+    o.w *= c;
+    for (int j0 = 0; j0 < cnt; j0 += 8) {
+      float4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (j0 + j < cnt) x[j] = __ldcg(reinterpret_cast<const float4*>(a.po + ((s0 + j0 + j) * n + row) * kHeadDim) + lane);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
+        if (j0 + j < cnt) {
+          o.x += w * x[j].x;
+          o.y += w * x[j].y;
+          o.z += w * x[j].z;
+          o.w += w * x[j].w;
+        }
+      }
+    }
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;  // no key at all: zeros
   reinterpret_cast<float4*>(a.out + b * a.ldo + (row % a.nh) * kHeadDim)[lane] =
       make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-template <typename KVT>
-cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
-  const long long pref = (long long)a.p.n_pref * a.p.row_groups * a.nkv;
-  const long long suf = (long long)a.p.n_suf * a.nseq * a.nkv * a.p.gch;
-  const int smem = kWarps * WarpTile<KVT>::kStages * WarpTile<KVT>::kBytes;
-  if (pref + suf > 0) {
-    cudaError_t e = cudaFuncSetAttribute(attn_shared_kernel<KVT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+// The launches of one call: the prefix kernel (tcgen05), the suffix kernel
+// beside it, the combine after both.
+cudaError_t launch_pdl(const void* fn, unsigned blocks, int threads, int smem, bool early, void** args,
+                       cudaStream_t st) {
+  if (smem > 48 << 10) {
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    attn_shared_kernel<KVT><<<(unsigned)(pref + suf), 32 * kWarps, smem, st>>>(a);
   }
-  attn_shared_combine<<<(a.nseq * a.nh + 3) / 4, 128, 0, st>>>(a);
-  return cudaGetLastError();
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+// The pool as a tensor of [rows][KV heads][128 dims], read in boxes of 16 rows
+// x 1 head x 64 dims with the 128-byte swizzle.
+cudaError_t page_map(CUtensorMap* map, const void* pool, const SharedArgs& a) {
+  static const auto encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                         const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                         CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill)>(f);
+  }();
+  if (!encode) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {kHeadDim, (cuuint64_t)a.nkv, (cuuint64_t)a.n_pages * kPage};
+  const cuuint64_t strides[2] = {kHeadDim * 2, (cuuint64_t)a.nkv * kHeadDim * 2};
+  const cuuint32_t box[3] = {64, 1, kPage}, step[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(pool), dims, strides, box, step,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? cudaSuccess
+             : cudaErrorInvalidValue;
+}
+
+cudaError_t launch_shared(const SharedArgs& a, int kv_f16, long long blocks, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  void* args[3] = {const_cast<SharedArgs*>(&a), nullptr, nullptr};
+  if (a.p.tc) {
+    CUtensorMap km, vm;
+    e = page_map(&km, a.kc, a);
+    if (e == cudaSuccess) e = page_map(&vm, a.vc, a);
+    args[1] = &km;
+    args[2] = &vm;
+    if (e == cudaSuccess)
+      e = launch_pdl((const void*)attn_prefix_tc_kernel, (unsigned)(a.p.n_pref * a.nkv * a.p.row_tiles), kTcThreads,
+                     kTcSmem, false, args, st);
+  }
+  if (e == cudaSuccess && blocks > 0)
+    e = kv_f16 ? launch_pdl((const void*)attn_shared_kernel<__half>, (unsigned)blocks, 32 * kWarps,
+                            kWarps * WarpTile<__half>::kStages * WarpTile<__half>::kBytes, a.p.tc, args, st)
+               : launch_pdl((const void*)attn_shared_kernel<float>, (unsigned)blocks, 32 * kWarps,
+                            kWarps * WarpTile<float>::kStages * WarpTile<float>::kBytes, a.p.tc, args, st);
+  if (e == cudaSuccess)
+    e = launch_pdl((const void*)attn_shared_combine, (unsigned)((a.nseq * a.nh + 3) / 4), 128, 0, blocks > 0 || a.p.tc,
+                   args, st);
+  return e;
 }
 
 bool misaligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) & (to - 1); }
@@ -526,7 +981,10 @@ EG_API eg_status eg_op_attn_shared_prefix_bytes(int nseq, int nh, int nkv, int p
                                                 uint64_t* bytes) {
   if (!bytes) return fail(EG_ERR_ARG, "attn_shared_prefix: null argument");
   if (const char* why = shared_dims(nseq, nh, nkv, prefix_len, max_len)) return fail(EG_ERR_ARG, "attn_shared_prefix: %s", why);
-  *bytes = std::max<size_t>(16, shared_bytes(shared_plan(nseq, nh, nkv, prefix_len, max_len), nseq, nh));
+  size_t n = 16;  // enough for either cache type
+  for (int f16 = 0; f16 < 2; f16++)
+    n = std::max(n, shared_bytes(shared_plan(nseq, nh, nkv, prefix_len, max_len, f16), nseq, nh));
+  *bytes = n;
   return EG_OK;
 }
 
@@ -546,7 +1004,7 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
   if (misaligned(q, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16) || misaligned(out, 16) || misaligned(ws, 16))
     return fail(EG_ERR_ARG, "attn_shared_prefix: 16-byte aligned buffers required");
   SharedArgs a = {};
-  a.p = shared_plan(nseq, nh, nkv, prefix_len, max_len);
+  a.p = shared_plan(nseq, nh, nkv, prefix_len, max_len, kv_f16);
   const size_t need = shared_bytes(a.p, nseq, nh);
   if (ws_bytes < need)
     return fail(EG_ERR_ARG, "attn_shared_prefix: workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes, (unsigned long long)need);
@@ -571,10 +1029,11 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
   a.pm = a.po + rows * kHeadDim;
   a.pl = a.pm + rows;
   a.err = err;
-  const long long blocks = (long long)a.p.n_pref * a.p.row_groups * nkv + (long long)a.p.n_suf * nseq * nkv * a.p.gch;
+  const long long blocks = (a.p.tc ? 0 : (long long)a.p.n_pref * a.p.row_groups * nkv) +
+                           (long long)a.p.n_suf * nseq * nkv * a.p.gch;
   if (blocks > 0x7fffffffLL) return fail(EG_ERR_ARG, "attn_shared_prefix: too many splits");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const cudaError_t e = kv_f16 ? launch_shared<__half>(a, st) : launch_shared<float>(a, st);
+  const cudaError_t e = launch_shared(a, kv_f16, blocks, st);
   if (e != cudaSuccess) return fail(EG_ERR_CUDA, "attn_shared_prefix: %s", cudaGetErrorString(e));
   return EG_OK;
 }
