@@ -290,6 +290,7 @@ struct FastSmem {
   float red[2][kThreads / 32];
   double wsum[kThreads / 32];
   uint32_t wcnt[kThreads / 32];
+  unsigned long long lsum[kThreads / 32];
   int cross[4];
   Ranges rg;
   // the leader's last reductions
@@ -579,33 +580,80 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     sample_generic(a, row, *reinterpret_cast<GenericSmem*>(dsm));
     return;
   }
-  // ---- place and running mass of each gathered token, inside its bin
-  uint32_t* lq = reinterpret_cast<uint32_t*>(xs);  // the slice is done with
-  uint32_t* lb = lq + kList;
-  for (int i = tid; i < nl; i += kThreads) {
-    uint32_t q;
-    lb[i] = (uint32_t)bin_of(B, key_value((uint32_t)(S.list[i] >> 32)), q);
-    lq[i] = q;
-  }
+  // ---- the gathered tokens in order (a bitonic sort, falling), then the place
+  // and running mass of each: sums from the first token of its bin on
+  int np = 32;
+  while (np < nl) np *= 2;
+  for (int i = nl + tid; i < np; i += kThreads) S.list[i] = 0;
+  for (int size = 2; size <= np; size *= 2)
+    for (int d = size / 2; d > 0; d /= 2) {
+      __syncthreads();
+      for (int t = tid; t < np / 2; t += kThreads) {
+        const int i = 2 * t - (t & (d - 1)), k = i + d;
+        const unsigned long long x = S.list[i], y = S.list[k];
+        if ((x < y) == ((i & size) == 0)) {
+          S.list[i] = y;
+          S.list[k] = x;
+        }
+      }
+    }
   __syncthreads();
-  constexpr int kMine = kList / kThreads;
+  constexpr int kMine = kList / kThreads;  // consecutive tokens of a thread
+  unsigned long long* before = reinterpret_cast<unsigned long long*>(xs);  // sum of q before each; the slice is done with
+  int* bins = reinterpret_cast<int*>(before + kList);
+  int lb[kMine], start[kMine];
+  unsigned long long q[kMine], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid * kMine + j;
+    uint32_t v = 0;
+    lb[j] = i < nl ? bin_of(B, key_value((uint32_t)(S.list[i] >> 32)), v) : kBins;
+    bins[i] = lb[j];
+    q[j] = v;
+    sum += v;
+  }
+  unsigned long long incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) S.lsum[warp] = incl;
+  __syncthreads();
+  unsigned long long at = incl - sum;
+  for (int w = 0; w < warp; w++) at += S.lsum[w];
+  int first = 0;
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid * kMine + j;
+    before[i] = at;
+    at += q[j];
+    if (i > 0 && bins[i - 1] != lb[j]) first = i;
+    start[j] = first;
+  }
+  int most = first;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, most, o);
+    if (lane >= o) most = max(most, v);
+  }
+  int prev = __shfl_up_sync(0xffffffffu, most, 1);
+  if (lane == 0) prev = 0;
+  if (lane == 31) S.wcnt[warp] = (uint32_t)most;
+  __syncthreads();
+  for (int w = 0; w < warp; w++) prev = max(prev, (int)S.wcnt[w]);
   uint32_t num[kMine];
   double cum[kMine];
 #pragma unroll
   for (int j = 0; j < kMine; j++) {
-    const int i = tid + j * kThreads;
+    const int i = tid * kMine + j;
     num[j] = 0xffffffffu;
     cum[j] = 0.0;
     if (i < nl) {
-      const unsigned long long me = S.list[i];
-      const uint32_t b = lb[i];
-      uint32_t c = 1;
-      unsigned long long q = lq[i];
-      for (int f = 0; f < nl; f++)
-        if (lb[f] == b && S.list[f] > me) c++, q += lq[f];
-      num[j] = S.count_above[b] + c;
-      cum[j] = S.above[b] + (double)q * bin_unit(B, (int)b);
-      if ((uint32_t)P.k == num[j] && P.k > 0) S.z = cum[j];
+      const int s0 = max(start[j], prev);
+      num[j] = S.count_above[lb[j]] + (uint32_t)(i - s0) + 1;
+      cum[j] = S.above[lb[j]] + (double)(before[i] - before[s0] + q[j]) * bin_unit(B, lb[j]);
+      if (P.k > 0 && (uint32_t)P.k == num[j]) S.z = cum[j];
     }
   }
   __syncthreads();
@@ -614,10 +662,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const double z = S.z;
 #pragma unroll
   for (int j = 0; j < kMine; j++) {
-    const int i = tid + j * kThreads;
+    const int i = tid * kMine + j;
     if (i >= nl) continue;
     if (P.p < 1.0 && cum[j] >= P.p * z) atomicMin(&S.n_p, num[j]);
-    if (R.lo[2] <= R.hi[2] && (int)lb[i] >= R.lo[2] && (int)lb[i] <= R.hi[2] &&
+    if (R.lo[2] <= R.hi[2] && lb[j] >= R.lo[2] && lb[j] <= R.hi[2] &&
         weight(key_value((uint32_t)(S.list[i] >> 32)), B.xmax, P.t) >= P.minp)
       atomicMin(&S.n_m, ~num[j]);  // the largest place
   }
@@ -644,22 +692,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       atomicMin(&S.best, (unsigned long long)num[j]);
   __syncthreads();
   if (S.best == ~0ull) {  // the target lies past the gathered tokens by a rounding: the last of them
-    uint32_t most = 0;
+    uint32_t end = 0;
 #pragma unroll
     for (int j = 0; j < kMine; j++)
-      if (num[j] != 0xffffffffu && num[j] <= n_keep) most = max(most, num[j]);
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) S.wcnt[warp] = most;
+      if (num[j] != 0xffffffffu && num[j] <= n_keep) end = max(end, num[j]);
+    end = __reduce_max_sync(0xffffffffu, end);
+    if (lane == 0) S.wcnt[warp] = end;
     __syncthreads();
     if (tid == 0) {
-      for (int w = 0; w < kThreads / 32; w++) most = max(most, S.wcnt[w]);
-      S.best = most;
+      for (int w = 0; w < kThreads / 32; w++) end = max(end, S.wcnt[w]);
+      S.best = end;
     }
     __syncthreads();
   }
 #pragma unroll
   for (int j = 0; j < kMine; j++) {
-    const int i = tid + j * kThreads;
+    const int i = tid * kMine + j;
     if (i < nl && num[j] == (uint32_t)S.best) {
       const unsigned long long me = S.list[i];
       a.ids[row] = ~(uint32_t)me;
@@ -679,7 +727,7 @@ int cluster_size(int rows, int n) {
 
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
   const int c = cluster_size(a.rows, a.n), per = (a.n + c - 1) / c, staged = per <= kSlice;
-  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 : 0, kList * 8);
+  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 : 0, kList * 12);
   cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)(sizeof(FastSmem) + kSlice * 4));
   if (e != cudaSuccess) return e;
