@@ -258,11 +258,15 @@ __device__ __noinline__ void sample_generic(const SampleArgs& a, int row, Generi
 // Histogram form: a cluster of CTAs holds one row in shared memory
 // ======================================================================
 // Bins are equal steps of x below the maximum.  A token's weight is
-// 2^-26 q e^(-b step): b its bin, q an integer (26 bits + the half step's
-// spread), so one 64-bit shared-memory atomic adds its count (upper 18 bits)
-// and its q (lower 46).  The leader CTA turns the merged bins into running
-// counts and masses, which fix each filter's and the sample's bin; only the
-// tokens of those few bins are gathered and put in order, in the same integers.
+// 2^-26 q e^(-b step): b its bin, q = 2^26 e^-u an integer, u its distance from
+// the bin's middle.  The histogram holds each bin's count and sum of q; in the
+// usual form q stays within 2^26 +- 2^22 and two 32-bit shared-memory atomics
+// take the count and the part of q above 2^26 - 2^22 (below 2^23: 512 tokens of
+// a CTA in one bin cannot overflow it; rows with more, or with steps of x / t
+// above 1/16, are counted again with 64-bit atomics, which cost three times as
+// much).  The leader CTA turns the merged bins into running counts and masses,
+// which fix each filter's and the sample's bin; only the tokens of those few
+// bins are gathered and put in order, in the same integers.
 // Tokens past the last bin (64 below the maximum in x / t or more) weigh
 // nothing: 150,000 of them are 2^-74 of the best token.
 namespace cg = cooperative_groups;
@@ -272,16 +276,22 @@ constexpr int kList = 1024;        // gathered tokens
 constexpr int kPer = kBins / kThreads;
 constexpr int kSlice = 19456;      // most tokens that a CTA stages (76 KB: two CTAs an SM)
 constexpr int kQBits = 26;
+constexpr uint32_t kQBase = (1u << kQBits) - (1u << 22);
+constexpr uint32_t kDense = 512;   // tokens of a CTA in one bin, at most, in the usual form
 constexpr unsigned long long kCountOne = 1ull << 46;
+constexpr float kRound = 12582912.f;  // 1.5 2^23: x + kRound rounds |x| < 2^22 to an integer in the low bits
 
-struct Ranges {  // bins [lo, hi] of: top-k, top-p, min-p, the sample; slow: leave the row to sample_generic
-  int lo[4], hi[4], top, slow;
+struct Ranges {  // bins [lo, hi] of: top-k, top-p, min-p, the sample (lo > hi: none)
+  int lo[4], hi[4], redo;
 };
 
-struct FastSmem {
+struct __align__(16) FastSmem {
   union {
-    unsigned long long hist[kBins];  // then, in the leader, the mass above each bin
-    double above[kBins];
+    struct {
+      uint32_t cnt[kBins], sum[kBins];
+    };
+    unsigned long long hist[kBins];  // 64-bit form: count << 46 | sum of q
+    double above[kBins];             // then, in the leader, the mass above each bin
   };
   uint32_t count_above[kBins];
   unsigned long long list[kList];    // order key << 32 | ~id: falling is TOPK_SELECT's order
@@ -291,7 +301,8 @@ struct FastSmem {
   double wsum[kThreads / 32];
   uint32_t wcnt[kThreads / 32];
   unsigned long long lsum[kThreads / 32];
-  int cross[4];
+  double unit[kPer];
+  int cross[4], dense;
   Ranges rg;
   // the leader's last reductions
   double z, mass_p, mass_m, mass;
@@ -305,33 +316,263 @@ struct Bins {
   double stepd;
 };
 
-// The bin of a candidate and its q.  pos = (xmax - x) / width carried as
-// p + e (the difference exact by a two-term sum, the product by fma), so the
-// part beyond the bin is right to 2^-36 of the range.
-__device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
+// A candidate's place p = (xmax - x) / width, its bin the nearest integer.
+__device__ __forceinline__ float bin_place(const Bins& B, float x) {
+  return __fmul_rn(B.xmax - x, B.sh);  // not to be fused with p - r below: e holds its rounding
+}
+__device__ __forceinline__ bool in_range(float p) { return p < (float)(kBins - 2) + 0.5f; }
+// u of a candidate in bin r (a float).  The place is carried as p + e (the
+// difference exact by a two-term sum, the product by fma), so the part beyond
+// the bin is right to 2^-36 of the range.
+__device__ __forceinline__ float bin_rest(const Bins& B, float x, float p, float r) {
   const float d = B.xmax - x;
   const float bb = d - B.xmax;
   const float dl = (B.xmax - (d - bb)) - (x + bb);  // d + dl = xmax - x
-  const float p = __fmul_rn(d, B.sh);  // not to be fused with p - r below: e holds its rounding
-  if (!(p < (float)(kBins - 2) + 0.5f)) {
+  const float e = __fadd_rn(fmaf(d, B.sh, -p), fmaf(d, B.sl, __fmul_rn(dl, B.sh)));
+  return __fmul_rn(__fadd_rn(p - r, e), B.step);  // |u| <= step / 2 (a little more by e)
+}
+// 2^26 (1 - e^-u) + kRound, an integer in the low bits, for |u| <= 1/32:
+// 1 - e^-u = u (1 - u/2 (1 - u/3 (1 - u/4 (1 - u/5)))), the next term below 2^-39
+__device__ __forceinline__ int q_short(float u) {
+  float y = fmaf(u, -0.2f, 1.f);  // fused as written: every caller gets the same q
+  y = fmaf(__fmul_rn(u, -0.25f), y, 1.f);
+  y = fmaf(__fmul_rn(u, -1.f / 3.f), y, 1.f);
+  y = fmaf(__fmul_rn(u, -0.5f), y, 1.f);
+  y = __fmul_rn(u, y);
+  return __float_as_int(fmaf(y, (float)(1 << kQBits), kRound)) - __float_as_int(kRound);
+}
+__device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
+  const float p = bin_place(B, x);
+  if (!in_range(p)) {
     q = 0;
     return kBins - 1;
   }
-  const float e = fmaf(d, B.sh, -p) + fmaf(d, B.sl, dl * B.sh);
-  const float r = rintf(p);
-  const float u = ((p - r) + e) * B.step;  // |u| <= step / 2 (a little more by e)
-  if (B.poly) {
-    // 1 - e^-u = u (1 - u/2 (1 - u/3 (1 - u/4 (1 - u/5)))): the next term is below 2^-39 for u <= 1/32
-    const float y = u * (1.f - u * 0.5f * (1.f - u * (1.f / 3.f) * (1.f - u * 0.25f * (1.f - u * 0.2f))));
-    q = (uint32_t)((1 << kQBits) - __float2int_rn(y * (float)(1 << kQBits)));
-  } else {
-    q = (uint32_t)__double2ll_rn(exp(-(double)u) * (double)(1 << kQBits));
-  }
+  const float r = (p + kRound) - kRound;
+  const float u = bin_rest(B, x, p, r);
+  q = B.poly ? (1u << kQBits) - q_short(u) : (uint32_t)__double2ll_rn(exp(-(double)u) * (double)(1 << kQBits));
   return (int)r;
 }
 
-__device__ __forceinline__ double bin_unit(const Bins& B, int b) {  // the weight of q = 1 in bin b
-  return exp(-(double)b * B.stepd) * (1.0 / (1 << kQBits));
+// The weight of q = 1 in bin b; units[j]: of bin j (kPer of them).
+__device__ __forceinline__ double bin_unit(const Bins& B, const double* units, int b) {
+  return exp(-(double)(b & ~(kPer - 1)) * B.stepd) * units[b & (kPer - 1)];
+}
+
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async16g(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src)
+               : "memory");
+}
+
+// list[0 .. np) (np a power of two from 64 to 1024) into falling order: 32
+// pairs a warp in registers and shuffles, shared memory where a step spans
+// more than a warp's 64 values.
+__device__ __forceinline__ void bitonic_falling(unsigned long long* list, int np) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int base = 64 * warp;
+  const bool on = base < np;
+  auto inside = [&](int size, int dmax) {  // the steps of distances dmax <= 32 .. 1 of one size
+    if (on) {
+      unsigned long long x = list[base + lane], y = list[base + 32 + lane];
+      // values base + lane and base + 32 + lane
+      for (int d = dmax; d > 0; d /= 2) {
+        if (d == 32) {
+          const bool fall = ((base + lane) & size) == 0;
+          if ((x < y) == fall) {
+            const unsigned long long t = x;
+            x = y;
+            y = t;
+          }
+        } else {
+          const unsigned long long px = __shfl_xor_sync(0xffffffffu, x, d), py = __shfl_xor_sync(0xffffffffu, y, d);
+          const bool low = (lane & d) == 0;
+          const bool fx = ((base + lane) & size) == 0, fy = ((base + 32 + lane) & size) == 0;
+          if ((x < px) == (low == fx)) x = px;  // the pair's larger value where falling, at its lower place
+          if ((y < py) == (low == fy)) y = py;
+        }
+      }
+      list[base + lane] = x;
+      list[base + 32 + lane] = y;
+    }
+  };
+  for (int size = 2; size <= np; size *= 2) {
+    for (int d = size / 2; d > 32; d /= 2) {
+      __syncthreads();
+      for (int t = threadIdx.x; t < np / 2; t += kThreads) {
+        const int i = 2 * t - (t & (d - 1)), k = i + d;
+        const unsigned long long x = list[i], y = list[k];
+        if ((x < y) == ((i & size) == 0)) {
+          list[i] = y;
+          list[k] = x;
+        }
+      }
+      __syncthreads();
+    }
+    inside(size, min(32, size / 2));
+    if (size >= 64) __syncthreads();
+    else __syncwarp();
+  }
+  __syncthreads();
+}
+
+// The leader's part between the two passes: merged bins to running counts and
+// masses (S.above, S.count_above) and the bins that decide (S.rg), or the wish
+// for the 64-bit form.
+__device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl, const Bins& B, const RowParams& P, int C,
+                                              bool wide) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // ---- running counts and masses over the bins, kPer of them a thread
+  unsigned long long q[kPer];
+  uint32_t cnt[kPer];
+  double m[kPer], unit[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; j++) q[j] = 0, cnt[j] = 0;
+  if (wide) {
+    for (int c = 0; c < C; c++) {
+      const unsigned long long* h = cl.map_shared_rank(&S, c)->hist + tid * kPer;
+#pragma unroll
+      for (int j = 0; j < kPer; j++) {
+        q[j] += h[j] & (kCountOne - 1);
+        cnt[j] += (uint32_t)(h[j] >> 46);
+      }
+    }
+  } else {
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < 8; c++) {  // up to 16 remote loads in flight
+      if (c >= C) break;
+      const FastSmem* R = cl.map_shared_rank(&S, c);
+      const uint4 n = *reinterpret_cast<const uint4*>(R->cnt + tid * kPer), v = *reinterpret_cast<const uint4*>(R->sum + tid * kPer);
+      const uint32_t nn[4] = {n.x, n.y, n.z, n.w}, vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < kPer; j++) {
+        cnt[j] += nn[j];
+        q[j] += (unsigned long long)nn[j] * kQBase + vv[j];
+        if (tid * kPer + j < kBins - 1) most = max(most, nn[j]);
+      }
+    }
+    if (most > kDense) S.dense = 1;
+  }
+  const double e4 = exp(-(double)(tid * kPer) * B.stepd);  // bin_unit's two factors
+  double ms = 0.0;
+  uint32_t cs = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    const int b = tid * kPer + j;
+    unit[j] = b == kBins - 1 ? 0.0 : e4 * S.unit[j];
+    m[j] = (double)q[j] * unit[j];
+    ms += m[j];
+    cs += cnt[j];
+  }
+  double mi = ms;
+  uint32_t ci = cs;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double v = __shfl_up_sync(0xffffffffu, mi, o);
+    const uint32_t w = __shfl_up_sync(0xffffffffu, ci, o);
+    if (lane >= o) mi += v, ci += w;
+  }
+  if (lane == 31) S.wsum[warp] = mi, S.wcnt[warp] = ci;
+  if (tid < 4) S.cross[tid] = kBins;
+  __syncthreads();  // every thread has read the bins; the sums are there
+  if (!wide && S.dense) {
+    if (tid == 0) S.rg.redo = 1;
+    return;
+  }
+  double mb = 0.0, total = 0.0;
+  uint32_t cb = 0, ncand = 0;
+  for (int w = 0; w < kThreads / 32; w++) {
+    if (w < warp) mb += S.wsum[w], cb += S.wcnt[w];
+    total += S.wsum[w];
+    ncand += S.wcnt[w];
+  }
+  double ab[kPer];
+  uint32_t ca[kPer];
+  double am = mb + (mi - ms);
+  uint32_t ac = cb + (ci - cs);
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    ab[j] = am;
+    ca[j] = ac;
+    S.above[tid * kPer + j] = am;
+    S.count_above[tid * kPer + j] = ac;
+    am += m[j];
+    ac += cnt[j];
+  }
+  // the first bin with tokens whose inclusive mass (count) reaches a target
+  auto cross_mass = [&](double t, int slot) {
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+      if (cnt[j] && tid * kPer + j < kBins - 1 && ab[j] + m[j] >= t) {
+        atomicMin(&S.cross[slot], tid * kPer + j);
+        break;
+      }
+  };
+  const bool k_on = P.k > 0 && (uint32_t)P.k < ncand;
+  if (k_on) {
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+      if (ca[j] < (uint32_t)P.k && (uint32_t)P.k <= ca[j] + cnt[j]) S.cross[0] = tid * kPer + j;
+  }
+  // the last bin that weighs anything: where a target at the very end falls
+  int last = -1;
+#pragma unroll
+  for (int j = 0; j < kPer; j++)
+    if (cnt[j] && tid * kPer + j < kBins - 1) last = tid * kPer + j;
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0) S.red[0][warp] = (float)last;
+  __syncthreads();
+  for (int w = 0; w < kThreads / 32; w++) last = max(last, (int)S.red[0][w]);
+  const int kb = k_on ? S.cross[0] : kBins;
+  const bool k_in = kb < kBins - 1;  // top-k cuts inside the bins that weigh anything
+  auto mass_above = [&](int b) { return S.above[b]; };  // b = kBins - 1: all that weighs
+  const double z_lo = k_in ? mass_above(kb) : total, z_hi = k_in ? mass_above(kb + 1) : total;
+  int p_lo = -1, p_hi = -1, m_lo = -1, m_hi = -1;
+  double lo = z_lo, hi = z_hi;
+  if (P.p < 1.0) {
+    cross_mass(P.p * z_lo * (1.0 - 1e-12), 1);
+    cross_mass(P.p * z_hi * (1.0 + 1e-12), 2);
+    __syncthreads();
+    p_lo = min(S.cross[1], last);
+    p_hi = min(S.cross[2], last);
+    lo = fmin(lo, mass_above(p_lo));
+    hi = fmin(hi, mass_above(p_hi + 1));
+    __syncthreads();
+    if (tid < 4) S.cross[tid] = kBins;
+    __syncthreads();
+  }
+  if (P.minp > 0.0) {
+    const double pos = B.stepd > 0.0 ? -log(P.minp) / B.stepd : 0.0;
+    if (pos < kBins - 2) {
+      m_lo = max(0, (int)rint(pos - 0.01));
+      m_hi = max(0, min(kBins - 2, (int)rint(pos + 0.01)));
+      lo = fmin(lo, mass_above(m_lo));
+      hi = fmin(hi, mass_above(m_hi + 1));
+    }
+  }
+  hi = fmax(hi, 1.0);  // one token at least
+  cross_mass(P.r * lo * (1.0 - 1e-12), 1);
+  cross_mass(P.r * hi * (1.0 + 1e-12), 2);
+  __syncthreads();
+  if (tid == 0) {
+    const int s_lo = min(S.cross[1], last), s_hi = min(S.cross[2], last);
+    Ranges& R = S.rg;
+    R.lo[0] = k_in ? kb : 1, R.hi[0] = k_in ? kb : 0;
+    R.lo[1] = p_lo < 0 ? 1 : p_lo, R.hi[1] = p_lo < 0 ? 0 : p_hi;
+    R.lo[2] = m_lo < 0 ? 1 : m_lo, R.hi[2] = m_lo < 0 ? 0 : m_hi;
+    R.lo[3] = s_lo, R.hi[3] = s_hi;
+    R.redo = 0;
+    S.z = total;
+    S.n_p = S.n_m = 0xffffffffu;
+    S.best = ~0ull;
+  }
 }
 
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a, int staged) {
@@ -342,17 +583,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float* x = a.logits + row * a.ld;
-  const int per = (a.n + C - 1) / C, e0 = min(a.n, rank * per), e1 = min(a.n, e0 + per);
+  const int per = ((a.n + C - 1) / C + 3) & ~3, e0 = min(a.n, rank * per), e1 = min(a.n, e0 + per);
   const RowParams P = row_params(a, row);
 
+  if (staged) {  // 16 bytes a copy where the row allows it
+    const int len = e1 - e0, quads = (reinterpret_cast<uintptr_t>(x) & 15) == 0 ? len / 4 : 0;
+    for (int i = tid; i < quads; i += kThreads) cp_async16g(xs + 4 * i, x + e0 + 4 * i);
+    for (int i = 4 * quads + tid; i < len; i += kThreads) cp_async4(xs + i, x + e0 + i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
   for (int i = tid; i < kBins; i += kThreads) S.hist[i] = 0;
-  if (tid == 0) S.n_list = 0;
-  // ---- the slice, its largest and smallest candidate
+  if (tid == 0) S.n_list = 0, S.dense = 0;
+  if (staged) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+  }
+  // ---- the slice's largest and smallest candidate
+  auto at = [&](int i) { return (staged ? xs[i - e0] : __ldg(x + i)) + 0.f; };
   float mx = -INFINITY, mn = INFINITY;
 #pragma unroll 8
   for (int i = e0 + tid; i < e1; i += kThreads) {
-    const float v = __ldg(x + i) + 0.f;
-    if (staged) xs[i - e0] = v;
+    const float v = at(i);
     if (v >= -1e30f) mx = fmaxf(mx, v), mn = fminf(mn, v);
   }
 #pragma unroll
@@ -392,12 +643,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     B.stepd = 1.0 / (s * P.t);
     B.step = (float)B.stepd;
     B.poly = B.stepd <= 0.0625;
-    for (int i = e0 + tid; i < e1; i += kThreads) {
-      const float v = staged ? xs[i - e0] : __ldg(x + i) + 0.f;
-      if (v >= -1e30f) {
-        uint32_t q;
-        const int b = bin_of(B, v, q);
-        atomicAdd(&S.hist[b], kCountOne + q);
+  }
+  FastSmem* L = cl.map_shared_rank(&S, 0);
+  bool wide = !none && !slow0 && !B.poly;  // the 64-bit form
+  if (!none && !slow0) {
+    if (tid < kPer) S.unit[tid] = exp(-(double)tid * B.stepd) * (1.0 / (1 << kQBits));
+    if (!wide) {
+#pragma unroll 4
+      for (int i = e0 + tid; i < e1; i += kThreads) {
+        const float v = at(i);
+        if (v >= -1e30f) {
+          const float p = bin_place(B, v), pr = p + kRound;
+          int b = kBins - 1;
+          if (in_range(p)) {
+            b = __float_as_int(pr) - __float_as_int(kRound);
+            atomicAdd(&S.sum[b], (uint32_t)((1 << 22) - q_short(bin_rest(B, v, p, pr - kRound))));
+          }
+          atomicAdd(&S.cnt[b], 1u);
+        }
       }
     }
   }
@@ -415,160 +678,44 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     return;
   }
-  uint32_t ncand = 0;
-  double total = 0.0;
-  if (rank == 0) {
-    // ---- running counts and masses over the bins, kPer of them a thread
-    unsigned long long q[kPer];
-    uint32_t cnt[kPer];
-    double m[kPer], unit[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; j++) q[j] = 0, cnt[j] = 0;
-    for (int c = 0; c < C; c++) {
-      const ulonglong2* h = reinterpret_cast<const ulonglong2*>(cl.map_shared_rank(&S, c)->hist + tid * kPer);
-#pragma unroll
-      for (int j = 0; j < kPer; j += 2) {
-        const ulonglong2 v = h[j / 2];
-        q[j] += v.x & (kCountOne - 1);
-        cnt[j] += (uint32_t)(v.x >> 46);
-        q[j + 1] += v.y & (kCountOne - 1);
-        cnt[j + 1] += (uint32_t)(v.y >> 46);
-      }
-    }
-    double ms = 0.0;
-    uint32_t cs = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      const int b = tid * kPer + j;
-      unit[j] = b == kBins - 1 ? 0.0 : bin_unit(B, b);
-      m[j] = (double)q[j] * unit[j];
-      ms += m[j];
-      cs += cnt[j];
-    }
-    double mi = ms;
-    uint32_t ci = cs;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double v = __shfl_up_sync(0xffffffffu, mi, o);
-      const uint32_t w = __shfl_up_sync(0xffffffffu, ci, o);
-      if (lane >= o) mi += v, ci += w;
-    }
-    if (lane == 31) S.wsum[warp] = mi, S.wcnt[warp] = ci;
-    if (tid < 4) S.cross[tid] = kBins;
-    __syncthreads();  // every thread has read the bins; the sums are there
-    double mb = 0.0;
-    uint32_t cb = 0;
-    for (int w = 0; w < kThreads / 32; w++) {
-      if (w < warp) mb += S.wsum[w], cb += S.wcnt[w];
-      total += S.wsum[w];
-      ncand += S.wcnt[w];
-    }
-    double ab[kPer];
-    uint32_t ca[kPer];
-    double am = mb + (mi - ms);
-    uint32_t ac = cb + (ci - cs);
-#pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      ab[j] = am;
-      ca[j] = ac;
-      S.above[tid * kPer + j] = am;
-      S.count_above[tid * kPer + j] = ac;
-      am += m[j];
-      ac += cnt[j];
-    }
-    // the first bin with tokens whose inclusive mass (count) reaches a target
-    auto cross_mass = [&](double t, int slot) {
-#pragma unroll
-      for (int j = 0; j < kPer; j++)
-        if (cnt[j] && tid * kPer + j < kBins - 1 && ab[j] + m[j] >= t) {
-          atomicMin(&S.cross[slot], tid * kPer + j);
-          break;
-        }
-    };
-    const bool k_on = P.k > 0 && (uint32_t)P.k < ncand;
-    if (k_on) {
-#pragma unroll
-      for (int j = 0; j < kPer; j++)
-        if (ca[j] < (uint32_t)P.k && (uint32_t)P.k <= ca[j] + cnt[j]) S.cross[0] = tid * kPer + j;
-    }
-    // the last bin that weighs anything: where a target at the very end falls
-    int last = -1;
-#pragma unroll
-    for (int j = 0; j < kPer; j++)
-      if (cnt[j] && tid * kPer + j < kBins - 1) last = tid * kPer + j;
-    last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0) S.red[0][warp] = (float)last;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 32; w++) last = max(last, (int)S.red[0][w]);
-    const int kb = k_on ? S.cross[0] : kBins;
-    const bool k_in = kb < kBins - 1;  // top-k cuts inside the bins that weigh anything
-    auto mass_above = [&](int b) { return S.above[b]; };  // b = kBins - 1: all that weighs
-    const double z_lo = k_in ? mass_above(kb) : total, z_hi = k_in ? mass_above(kb + 1) : total;
-    int p_lo = -1, p_hi = -1, m_lo = -1, m_hi = -1;
-    double lo = z_lo, hi = z_hi;
-    if (P.p < 1.0) {
-      cross_mass(P.p * z_lo * (1.0 - 1e-12), 1);
-      cross_mass(P.p * z_hi * (1.0 + 1e-12), 2);
-      __syncthreads();
-      p_lo = min(S.cross[1], last);
-      p_hi = min(S.cross[2], last);
-      lo = fmin(lo, mass_above(p_lo));
-      hi = fmin(hi, mass_above(p_hi + 1));
-      __syncthreads();
-      if (tid < 4) S.cross[tid] = kBins;
-      __syncthreads();
-    }
-    if (P.minp > 0.0) {
-      const double pos = B.stepd > 0.0 ? -log(P.minp) / B.stepd : 0.0;
-      if (pos < kBins - 2) {
-        m_lo = max(0, (int)rint(pos - 0.01));
-        m_hi = max(0, min(kBins - 2, (int)rint(pos + 0.01)));
-        lo = fmin(lo, mass_above(m_lo));
-        hi = fmin(hi, mass_above(m_hi + 1));
-      }
-    }
-    hi = fmax(hi, 1.0);  // one token at least
-    cross_mass(P.r * lo * (1.0 - 1e-12), 1);
-    cross_mass(P.r * hi * (1.0 + 1e-12), 2);
-    __syncthreads();
-    if (tid == 0) {
-      const int s_lo = min(S.cross[1], last), s_hi = min(S.cross[2], last);
-      Ranges& R = S.rg;
-      R.lo[0] = k_in ? kb : 1, R.hi[0] = k_in ? kb : 0;
-      R.lo[1] = p_lo < 0 ? 1 : p_lo, R.hi[1] = p_lo < 0 ? 0 : p_hi;
-      R.lo[2] = m_lo < 0 ? 1 : m_lo, R.hi[2] = m_lo < 0 ? 0 : m_hi;
-      R.lo[3] = s_lo, R.hi[3] = s_hi;
-      R.top = max(max(R.hi[0], R.hi[1]), max(R.hi[2], R.hi[3]));
-      S.z = total;
-      S.n_p = S.n_m = 0xffffffffu;
-      S.best = ~0ull;
-    }
-  }
-  cl.sync();
-  // ---- the tokens of those bins, gathered in the leader
-  FastSmem* L = cl.map_shared_rank(&S, 0);
-  {
-    const Ranges R = L->rg;
-    for (int i0 = e0; i0 < e1; i0 += kThreads) {
-      const int i = i0 + tid;
-      float v = -INFINITY;
-      if (i < e1) v = staged ? xs[i - e0] : __ldg(x + i) + 0.f;
-      bool in = false;
-      if (v >= -1e30f) {
-        const float p = __fmul_rn(B.xmax - v, B.sh);
-        if (p <= (float)R.top + 0.5f || R.top >= kBins - 2) {
+  for (;;) {
+    if (wide) {
+      for (int i = e0 + tid; i < e1; i += kThreads) {
+        const float v = at(i);
+        if (v >= -1e30f) {
           uint32_t q;
           const int b = bin_of(B, v, q);
-#pragma unroll
-          for (int j = 0; j < 4; j++) in |= b >= R.lo[j] && b <= R.hi[j];
+          atomicAdd(&S.hist[b], kCountOne + q);
         }
       }
+      cl.sync();
+    }
+    if (rank == 0) leader_ranges(S, cl, B, P, C, wide);
+    cl.sync();
+    if (!L->rg.redo) break;
+    wide = true;  // a bin holds too many tokens for the 32-bit sums: once more
+    for (int i = tid; i < kBins; i += kThreads) S.hist[i] = 0;
+    __syncthreads();
+  }
+  // ---- the tokens of those bins, gathered in the leader
+  {
+    const Ranges R = L->rg;
+#pragma unroll 2
+    for (int i0 = e0; i0 < e1; i0 += kThreads) {
+      const int i = i0 + tid;
+      const float v = i < e1 ? at(i) : -INFINITY;
+      const float p = bin_place(B, v);
+      const int b = __float_as_int(p + kRound) - __float_as_int(kRound);  // as bin_of, where in_range
+      bool in = false;
+#pragma unroll
+      for (int j = 0; j < 4; j++) in |= b >= R.lo[j] && b <= R.hi[j];
+      in = in && v >= -1e30f && in_range(p);
       const uint32_t vote = __ballot_sync(0xffffffffu, in);
       if (!vote) continue;
-      uint32_t at = 0;
-      if (lane == 0) at = atomicAdd(&L->n_list, (uint32_t)__popc(vote));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(vote & ((1u << lane) - 1));
-      if (in && at < kList) L->list[at] = (unsigned long long)order_key(v) << 32 | (uint32_t)~i;
+      uint32_t to = 0;
+      if (lane == 0) to = atomicAdd(&L->n_list, (uint32_t)__popc(vote));
+      to = __shfl_sync(0xffffffffu, to, 0) + __popc(vote & ((1u << lane) - 1));
+      if (in && to < kList) L->list[to] = (unsigned long long)order_key(v) << 32 | (uint32_t)~i;
     }
   }
   cl.sync();
@@ -582,22 +729,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   // ---- the gathered tokens in order (a bitonic sort, falling), then the place
   // and running mass of each: sums from the first token of its bin on
-  int np = 32;
+  int np = 64;
   while (np < nl) np *= 2;
   for (int i = nl + tid; i < np; i += kThreads) S.list[i] = 0;
-  for (int size = 2; size <= np; size *= 2)
-    for (int d = size / 2; d > 0; d /= 2) {
-      __syncthreads();
-      for (int t = tid; t < np / 2; t += kThreads) {
-        const int i = 2 * t - (t & (d - 1)), k = i + d;
-        const unsigned long long x = S.list[i], y = S.list[k];
-        if ((x < y) == ((i & size) == 0)) {
-          S.list[i] = y;
-          S.list[k] = x;
-        }
-      }
-    }
   __syncthreads();
+  bitonic_falling(S.list, np);
   constexpr int kMine = kList / kThreads;  // consecutive tokens of a thread
   unsigned long long* before = reinterpret_cast<unsigned long long*>(xs);  // sum of q before each; the slice is done with
   int* bins = reinterpret_cast<int*>(before + kList);
@@ -620,14 +756,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   if (lane == 31) S.lsum[warp] = incl;
   __syncthreads();
-  unsigned long long at = incl - sum;
-  for (int w = 0; w < warp; w++) at += S.lsum[w];
+  unsigned long long pre = incl - sum;
+  for (int w = 0; w < warp; w++) pre += S.lsum[w];
   int first = 0;
 #pragma unroll
   for (int j = 0; j < kMine; j++) {
     const int i = tid * kMine + j;
-    before[i] = at;
-    at += q[j];
+    before[i] = pre;
+    pre += q[j];
     if (i > 0 && bins[i - 1] != lb[j]) first = i;
     start[j] = first;
   }
@@ -652,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (i < nl) {
       const int s0 = max(start[j], prev);
       num[j] = S.count_above[lb[j]] + (uint32_t)(i - s0) + 1;
-      cum[j] = S.above[lb[j]] + (double)(before[i] - before[s0] + q[j]) * bin_unit(B, lb[j]);
+      cum[j] = S.above[lb[j]] + (double)(before[i] - before[s0] + q[j]) * bin_unit(B, S.unit, lb[j]);
       if (P.k > 0 && (uint32_t)P.k == num[j]) S.z = cum[j];
     }
   }
@@ -726,7 +862,7 @@ int cluster_size(int rows, int n) {
 }
 
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
-  const int c = cluster_size(a.rows, a.n), per = (a.n + c - 1) / c, staged = per <= kSlice;
+  const int c = cluster_size(a.rows, a.n), per = ((a.n + c - 1) / c + 3) & ~3, staged = per <= kSlice;
   const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 : 0, kList * 12);
   cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)(sizeof(FastSmem) + kSlice * 4));
