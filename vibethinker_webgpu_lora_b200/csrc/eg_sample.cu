@@ -598,14 +598,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
   }
+  // f(value, id) over the slice, the whole warp at a time (-inf past its end)
+  const bool vec = !staged && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  auto each = [&](auto f) {
+    if (staged) {
+#pragma unroll 4
+      for (int i0 = e0; i0 < e1; i0 += kThreads) {
+        const int i = i0 + tid;
+        f(i < e1 ? xs[i - e0] + 0.f : -INFINITY, i);
+      }
+    } else if (vec) {
+#pragma unroll 2
+      for (int i0 = e0; i0 < e1; i0 += 4 * kThreads) {
+        const int i = i0 + 4 * tid;
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (i + 3 < e1) {
+          v = __ldg(reinterpret_cast<const float4*>(x + i));
+        } else if (i < e1) {
+          v.x = __ldg(x + i);
+          if (i + 1 < e1) v.y = __ldg(x + i + 1);
+          if (i + 2 < e1) v.z = __ldg(x + i + 2);
+        }
+        f(v.x + 0.f, i);
+        f(v.y + 0.f, i + 1);
+        f(v.z + 0.f, i + 2);
+        f(v.w + 0.f, i + 3);
+      }
+    } else {
+#pragma unroll 4
+      for (int i0 = e0; i0 < e1; i0 += kThreads) {
+        const int i = i0 + tid;
+        f(i < e1 ? __ldg(x + i) + 0.f : -INFINITY, i);
+      }
+    }
+  };
   // ---- the slice's largest and smallest candidate
-  auto at = [&](int i) { return (staged ? xs[i - e0] : __ldg(x + i)) + 0.f; };
   float mx = -INFINITY, mn = INFINITY;
-#pragma unroll 8
-  for (int i = e0 + tid; i < e1; i += kThreads) {
-    const float v = at(i);
+  each([&](float v, int) {
     if (v >= -1e30f) mx = fmaxf(mx, v), mn = fminf(mn, v);
-  }
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -648,10 +679,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   bool wide = !none && !slow0 && !B.poly;  // the 64-bit form
   if (!none && !slow0) {
     if (tid < kPer) S.unit[tid] = exp(-(double)tid * B.stepd) * (1.0 / (1 << kQBits));
-    if (!wide) {
-#pragma unroll 4
-      for (int i = e0 + tid; i < e1; i += kThreads) {
-        const float v = at(i);
+    if (!wide)
+      each([&](float v, int) {
         if (v >= -1e30f) {
           const float p = bin_place(B, v), pr = p + kRound;
           int b = kBins - 1;
@@ -661,8 +690,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           }
           atomicAdd(&S.cnt[b], 1u);
         }
-      }
-    }
+      });
   }
   cl.sync();
   if (none || slow0) {  // the same in every CTA of the cluster
@@ -680,14 +708,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   for (;;) {
     if (wide) {
-      for (int i = e0 + tid; i < e1; i += kThreads) {
-        const float v = at(i);
+      each([&](float v, int) {
         if (v >= -1e30f) {
           uint32_t q;
           const int b = bin_of(B, v, q);
           atomicAdd(&S.hist[b], kCountOne + q);
         }
-      }
+      });
       cl.sync();
     }
     if (rank == 0) leader_ranges(S, cl, B, P, C, wide);
@@ -697,25 +724,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     for (int i = tid; i < kBins; i += kThreads) S.hist[i] = 0;
     __syncthreads();
   }
-  // ---- the tokens of those bins, gathered in the leader
+  // ---- the tokens of those bins: gathered in the CTA, then in the leader
   {
     const Ranges R = L->rg;
-#pragma unroll 2
-    for (int i0 = e0; i0 < e1; i0 += kThreads) {
-      const int i = i0 + tid;
-      const float v = i < e1 ? at(i) : -INFINITY;
+    each([&](float v, int i) {
       const float p = bin_place(B, v);
       const int b = __float_as_int(p + kRound) - __float_as_int(kRound);  // as bin_of, where in_range
       bool in = false;
 #pragma unroll
       for (int j = 0; j < 4; j++) in |= b >= R.lo[j] && b <= R.hi[j];
-      in = in && v >= -1e30f && in_range(p);
-      const uint32_t vote = __ballot_sync(0xffffffffu, in);
-      if (!vote) continue;
-      uint32_t to = 0;
-      if (lane == 0) to = atomicAdd(&L->n_list, (uint32_t)__popc(vote));
-      to = __shfl_sync(0xffffffffu, to, 0) + __popc(vote & ((1u << lane) - 1));
-      if (in && to < kList) L->list[to] = (unsigned long long)order_key(v) << 32 | (uint32_t)~i;
+      if (in && v >= -1e30f && in_range(p)) {
+        const uint32_t to = atomicAdd(&S.n_list, 1u);
+        if (to < kList) S.list[to] = (unsigned long long)order_key(v) << 32 | (uint32_t)~i;
+      }
+    });
+    if (C > 1) {
+      __syncthreads();
+      if (rank != 0) {
+        const uint32_t n = S.n_list;
+        if (tid == 0) S.wcnt[0] = n ? atomicAdd(&L->n_list, n) : 0u;
+        __syncthreads();
+        const uint32_t to = S.wcnt[0];
+        for (uint32_t i = tid; i < min(n, (uint32_t)kList); i += kThreads)
+          if (to + i < kList) L->list[to + i] = S.list[i];
+      }
     }
   }
   cl.sync();
@@ -852,12 +884,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
 }
 
-// CTAs of a row's cluster: enough that a slice fits, and more (slices of 2048
-// tokens or longer) while the rows leave SMs idle.
+// CTAs of a row's cluster: as many as all rows' CTAs can be resident at once
+// (two an SM) with slices of 2048 tokens or longer.  A slice is staged in
+// shared memory where it fits; few CTAs a row read it from L2 in each pass
+// instead (256 rows of 151936: one unstaged CTA a row 120 us, eight staged 276).
 int cluster_size(int rows, int n) {
   int c = 1;
-  while (c < 8 && (long long)c * kSlice < n) c *= 2;
-  while (c < 8 && 2LL * rows * c <= 148 && n / (2 * c) >= 2048) c *= 2;
+  while (c < 8 && 2LL * rows * c <= 2 * 148 && n / (2 * c) >= 2048) c *= 2;
   return c;
 }
 
