@@ -23,7 +23,6 @@
 namespace eg {
 namespace {
 
-constexpr int kThreads = 512;
 
 struct SampleArgs {
   const float* logits;
@@ -88,6 +87,7 @@ struct GenericSmem {
 // The shortest leading part with at least `count` tokens (by_mass = 0) or
 // with a mass of at least `target` (by_mass = 1): a descent over the keys' four
 // bytes, each level a histogram of the tokens that share the bytes above.
+template <int kThreads>
 __device__ Cut generic_cut(const float* x, int n, float xmax, double t, double scale, int by_mass, long long count,
                            double target, GenericSmem& S) {
   uint32_t prefix = 0;
@@ -152,6 +152,7 @@ __device__ Cut generic_cut(const float* x, int n, float xmax, double t, double s
 }
 
 // sums of a count and a mass over the CTA
+template <int kThreads>
 __device__ void block_sums(long long& n, unsigned long long& m, GenericSmem& S) {
   unsigned long long a = (unsigned long long)n, b = m;
 #pragma unroll
@@ -174,6 +175,7 @@ __device__ void block_sums(long long& n, unsigned long long& m, GenericSmem& S) 
 // The whole row by one CTA, from global memory: right for every row, and the
 // path of those that the histogram form below leaves (an infinite maximum,
 // more than kList tokens in the bins that decide).
+template <int kThreads>
 __device__ __noinline__ void sample_generic(const SampleArgs& a, int row, GenericSmem& S) {
   const int n = a.n;
   const float* x = a.logits + row * a.ld;
@@ -207,10 +209,10 @@ __device__ __noinline__ void sample_generic(const SampleArgs& a, int row, Generi
     total += m;
     if (w >= q.minp) n_m++, mass_m += m;
   }
-  block_sums(cand, total, S);
-  block_sums(n_m, mass_m, S);
+  block_sums<kThreads>(cand, total, S);
+  block_sums<kThreads>(n_m, mass_m, S);
   Cut best{cand, total, 0, 0};
-  if (q.k > 0 && q.k < cand) best = generic_cut(x, n, xmax, q.t, scale, 0, q.k, 0.0, S);
+  if (q.k > 0 && q.k < cand) best = generic_cut<kThreads>(x, n, xmax, q.t, scale, 0, q.k, 0.0, S);
   if (best.n < cand) {  // the mass of the first k (the descent by count sums none)
     long long nn = 0;
     unsigned long long mm = 0;
@@ -218,16 +220,16 @@ __device__ __noinline__ void sample_generic(const SampleArgs& a, int row, Generi
       const float v = __ldg(x + i);
       if (order_key(v) > best.key) nn++, mm += __double2ll_rn(weight(v, xmax, q.t) * scale);
     }
-    block_sums(nn, mm, S);
+    block_sums<kThreads>(nn, mm, S);
     best.mass = mm + best.tie * (unsigned long long)__double2ll_rn(weight(key_value(best.key), xmax, q.t) * scale);
   }
   if (q.p < 1.0) {
-    const Cut c = generic_cut(x, n, xmax, q.t, scale, 1, 0, q.p * (double)best.mass, S);
+    const Cut c = generic_cut<kThreads>(x, n, xmax, q.t, scale, 1, 0, q.p * (double)best.mass, S);
     if (c.n < best.n) best = c;
   }
   if (n_m < best.n) best.n = n_m, best.mass = mass_m;
   if (best.n < 1) best.n = 1, best.mass = (unsigned long long)scale;
-  const Cut c = generic_cut(x, n, xmax, q.t, scale, 1, 0, q.r * (double)best.mass, S);
+  const Cut c = generic_cut<kThreads>(x, n, xmax, q.t, scale, 1, 0, q.r * (double)best.mass, S);
   // the c.tie-th token with c.key: each thread counts its stretch of the row
   const int per = (n + kThreads - 1) / kThreads, i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
   uint32_t mine = 0;
@@ -273,7 +275,6 @@ namespace cg = cooperative_groups;
 
 constexpr int kBins = 2048;        // the last one: past the range
 constexpr int kList = 1024;        // gathered tokens
-constexpr int kPer = kBins / kThreads;
 constexpr int kSlice = 19456;      // most tokens that a CTA stages (76 KB: two CTAs an SM)
 constexpr int kQBits = 26;
 constexpr uint32_t kQBase = (1u << kQBits) - (1u << 22);
@@ -297,12 +298,12 @@ struct __align__(16) FastSmem {
   unsigned long long list[kList];    // order key << 32 | ~id: falling is TOPK_SELECT's order
   uint32_t n_list;
   float mx, mn;
-  float red[2][kThreads / 32];
-  double wsum[kThreads / 32];
-  uint32_t wcnt[kThreads / 32];
-  unsigned long long lsum[kThreads / 32];
-  double unit[kPer];
-  int cross[4], dense;
+  float red[2][32];
+  double wsum[32];
+  uint32_t wcnt[32];
+  unsigned long long lsum[32];
+  double unit[4];
+  int cross[6], dense;
   Ranges rg;
   // the leader's last reductions
   double z, mass_p, mass_m, mass;
@@ -353,9 +354,22 @@ __device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
   return (int)r;
 }
 
-// The weight of q = 1 in bin b; units[j]: of bin j (kPer of them).
+// The weight of q = 1 in bin b; units[j]: of bin j (4 of them).
 __device__ __forceinline__ double bin_unit(const Bins& B, const double* units, int b) {
-  return exp(-(double)(b & ~(kPer - 1)) * B.stepd) * units[b & (kPer - 1)];
+  return exp(-(double)(b & ~3) * B.stepd) * units[b & 3];
+}
+// sums over the warps before this one and over all, of one value a warp in shared memory
+template <int kThreads, typename T>
+__device__ __forceinline__ void warp_sums(const T* v, T& before, T& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  T x = lane < kThreads / 32 ? v[lane] : T(0), y = lane < warp ? x : T(0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    x += __shfl_xor_sync(0xffffffffu, x, o);
+    y += __shfl_xor_sync(0xffffffffu, y, o);
+  }
+  before = y;
+  all = x;
 }
 
 __device__ __forceinline__ void cp_async4(void* dst, const void* src) {
@@ -374,6 +388,7 @@ __device__ __forceinline__ void cp_async16g(void* dst, const void* src) {
 // list[0 .. np) (np a power of two from 64 to 1024) into falling order: 32
 // pairs a warp in registers and shuffles, shared memory where a step spans
 // more than a warp's 64 values.
+template <int kThreads>
 __device__ __forceinline__ void bitonic_falling(unsigned long long* list, int np) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int base = 64 * warp;
@@ -425,15 +440,17 @@ __device__ __forceinline__ void bitonic_falling(unsigned long long* list, int np
 // The leader's part between the two passes: merged bins to running counts and
 // masses (S.above, S.count_above) and the bins that decide (S.rg), or the wish
 // for the 64-bit form.
+template <int kThreads>
 __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl, const Bins& B, const RowParams& P, int C,
-                                              bool wide) {
+                                              bool wide, double e4) {
+  constexpr int kPer = kBins / kThreads;  // consecutive bins of a thread: 2 or 4
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // ---- running counts and masses over the bins, kPer of them a thread
   unsigned long long q[kPer];
   uint32_t cnt[kPer];
-  double m[kPer], unit[kPer];
+  double m[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; j++) q[j] = 0, cnt[j] = 0;
+  if (tid < 6) S.cross[tid] = kBins;
   if (wide) {
     for (int c = 0; c < C; c++) {
       const unsigned long long* h = cl.map_shared_rank(&S, c)->hist + tid * kPer;
@@ -446,28 +463,27 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
   } else {
     uint32_t most = 0;
 #pragma unroll
-    for (int c = 0; c < 8; c++) {  // up to 16 remote loads in flight
+    for (int c = 0; c < 8; c++) {  // all remote loads in flight
       if (c >= C) break;
       const FastSmem* R = cl.map_shared_rank(&S, c);
-      const uint4 n = *reinterpret_cast<const uint4*>(R->cnt + tid * kPer), v = *reinterpret_cast<const uint4*>(R->sum + tid * kPer);
-      const uint32_t nn[4] = {n.x, n.y, n.z, n.w}, vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < kPer; j++) {
-        cnt[j] += nn[j];
-        q[j] += (unsigned long long)nn[j] * kQBase + vv[j];
-        if (tid * kPer + j < kBins - 1) most = max(most, nn[j]);
+      for (int j = 0; j < kPer; j += 2) {
+        const uint2 n = *reinterpret_cast<const uint2*>(R->cnt + tid * kPer + j);
+        const uint2 v = *reinterpret_cast<const uint2*>(R->sum + tid * kPer + j);
+        cnt[j] += n.x;
+        cnt[j + 1] += n.y;
+        q[j] += (unsigned long long)n.x * kQBase + v.x;
+        q[j + 1] += (unsigned long long)n.y * kQBase + v.y;
+        most = max(most, max(n.x, n.y));
       }
     }
     if (most > kDense) S.dense = 1;
   }
-  const double e4 = exp(-(double)(tid * kPer) * B.stepd);  // bin_unit's two factors
   double ms = 0.0;
   uint32_t cs = 0;
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
-    const int b = tid * kPer + j;
-    unit[j] = b == kBins - 1 ? 0.0 : e4 * S.unit[j];
-    m[j] = (double)q[j] * unit[j];
+    m[j] = (double)q[j] * (e4 * S.unit[(tid * kPer + j) & 3]);
     ms += m[j];
     cs += cnt[j];
   }
@@ -479,24 +495,26 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
     const uint32_t w = __shfl_up_sync(0xffffffffu, ci, o);
     if (lane >= o) mi += v, ci += w;
   }
-  if (lane == 31) S.wsum[warp] = mi, S.wcnt[warp] = ci;
-  if (tid < 4) S.cross[tid] = kBins;
+  // the last bin with tokens: where a target at the very end falls
+  int last = -1;
+#pragma unroll
+  for (int j = 0; j < kPer; j++)
+    if (cnt[j]) last = tid * kPer + j;
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 31) S.wsum[warp] = mi, S.wcnt[warp] = ci, S.red[0][warp] = (float)last;
   __syncthreads();  // every thread has read the bins; the sums are there
   if (!wide && S.dense) {
     if (tid == 0) S.rg.redo = 1;
     return;
   }
-  double mb = 0.0, total = 0.0;
-  uint32_t cb = 0, ncand = 0;
-  for (int w = 0; w < kThreads / 32; w++) {
-    if (w < warp) mb += S.wsum[w], cb += S.wcnt[w];
-    total += S.wsum[w];
-    ncand += S.wcnt[w];
-  }
-  double ab[kPer];
-  uint32_t ca[kPer];
+  double mb, total, ab[kPer];
+  uint32_t cb, ncand, ca[kPer];
+  warp_sums<kThreads>(S.wsum, mb, total);
+  warp_sums<kThreads>(S.wcnt, cb, ncand);
+  last = (int)warp_max(lane < kThreads / 32 ? S.red[0][lane] : -1.f);
   double am = mb + (mi - ms);
   uint32_t ac = cb + (ci - cs);
+  const bool k_on = P.k > 0 && (uint32_t)P.k < ncand;
 #pragma unroll
   for (int j = 0; j < kPer; j++) {
     ab[j] = am;
@@ -505,36 +523,22 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
     S.count_above[tid * kPer + j] = ac;
     am += m[j];
     ac += cnt[j];
+    if (k_on && ca[j] < (uint32_t)P.k && (uint32_t)P.k <= ac) S.cross[0] = tid * kPer + j;
   }
-  // the first bin with tokens whose inclusive mass (count) reaches a target
+  // the first bin with tokens whose inclusive mass reaches a target
   auto cross_mass = [&](double t, int slot) {
 #pragma unroll
     for (int j = 0; j < kPer; j++)
-      if (cnt[j] && tid * kPer + j < kBins - 1 && ab[j] + m[j] >= t) {
+      if (cnt[j] && ab[j] + m[j] >= t) {
         atomicMin(&S.cross[slot], tid * kPer + j);
         break;
       }
   };
-  const bool k_on = P.k > 0 && (uint32_t)P.k < ncand;
-  if (k_on) {
-#pragma unroll
-    for (int j = 0; j < kPer; j++)
-      if (ca[j] < (uint32_t)P.k && (uint32_t)P.k <= ca[j] + cnt[j]) S.cross[0] = tid * kPer + j;
-  }
-  // the last bin that weighs anything: where a target at the very end falls
-  int last = -1;
-#pragma unroll
-  for (int j = 0; j < kPer; j++)
-    if (cnt[j] && tid * kPer + j < kBins - 1) last = tid * kPer + j;
-  last = __reduce_max_sync(0xffffffffu, last);
-  if (lane == 0) S.red[0][warp] = (float)last;
   __syncthreads();
-  for (int w = 0; w < kThreads / 32; w++) last = max(last, (int)S.red[0][w]);
-  const int kb = k_on ? S.cross[0] : kBins;
-  const bool k_in = kb < kBins - 1;  // top-k cuts inside the bins that weigh anything
-  auto mass_above = [&](int b) { return S.above[b]; };  // b = kBins - 1: all that weighs
-  const double z_lo = k_in ? mass_above(kb) : total, z_hi = k_in ? mass_above(kb + 1) : total;
-  int p_lo = -1, p_hi = -1, m_lo = -1, m_hi = -1;
+  auto mass_above = [&](int b) { return b < kBins ? S.above[b] : total; };
+  const int kb = S.cross[0];
+  const double z_lo = k_on ? mass_above(kb) : total, z_hi = k_on ? mass_above(kb + 1) : total;
+  int p_lo = 1, p_hi = 0, m_lo = 1, m_hi = 0;  // none
   double lo = z_lo, hi = z_hi;
   if (P.p < 1.0) {
     cross_mass(P.p * z_lo * (1.0 - 1e-12), 1);
@@ -544,12 +548,9 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
     p_hi = min(S.cross[2], last);
     lo = fmin(lo, mass_above(p_lo));
     hi = fmin(hi, mass_above(p_hi + 1));
-    __syncthreads();
-    if (tid < 4) S.cross[tid] = kBins;
-    __syncthreads();
   }
   if (P.minp > 0.0) {
-    const double pos = B.stepd > 0.0 ? -log(P.minp) / B.stepd : 0.0;
+    const double pos = -log(P.minp) / B.stepd;
     if (pos < kBins - 2) {
       m_lo = max(0, (int)rint(pos - 0.01));
       m_hi = max(0, min(kBins - 2, (int)rint(pos + 0.01)));
@@ -558,16 +559,15 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
     }
   }
   hi = fmax(hi, 1.0);  // one token at least
-  cross_mass(P.r * lo * (1.0 - 1e-12), 1);
-  cross_mass(P.r * hi * (1.0 + 1e-12), 2);
+  cross_mass(P.r * lo * (1.0 - 1e-12), 3);
+  cross_mass(P.r * hi * (1.0 + 1e-12), 4);
   __syncthreads();
   if (tid == 0) {
-    const int s_lo = min(S.cross[1], last), s_hi = min(S.cross[2], last);
     Ranges& R = S.rg;
-    R.lo[0] = k_in ? kb : 1, R.hi[0] = k_in ? kb : 0;
-    R.lo[1] = p_lo < 0 ? 1 : p_lo, R.hi[1] = p_lo < 0 ? 0 : p_hi;
-    R.lo[2] = m_lo < 0 ? 1 : m_lo, R.hi[2] = m_lo < 0 ? 0 : m_hi;
-    R.lo[3] = s_lo, R.hi[3] = s_hi;
+    R.lo[0] = k_on ? kb : 1, R.hi[0] = k_on ? kb : 0;
+    R.lo[1] = p_lo, R.hi[1] = p_hi;
+    R.lo[2] = m_lo, R.hi[2] = m_hi;
+    R.lo[3] = min(S.cross[3], last), R.hi[3] = min(S.cross[4], last);
     R.redo = 0;
     S.z = total;
     S.n_p = S.n_m = 0xffffffffu;
@@ -575,7 +575,8 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
   }
 }
 
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a, int staged) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const __grid_constant__ SampleArgs a, int staged) {
   extern __shared__ __align__(16) unsigned char dsm[];
   FastSmem& S = *reinterpret_cast<FastSmem*>(dsm);
   float* xs = reinterpret_cast<float*>(dsm + sizeof(FastSmem));  // the slice; the leader's scratch at the end
@@ -608,9 +609,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         f(i < e1 ? xs[i - e0] + 0.f : -INFINITY, i);
       }
     } else if (vec) {
-#pragma unroll 2
-      for (int i0 = e0; i0 < e1; i0 += 4 * kThreads) {
-        const int i = i0 + 4 * tid;
+      // eight tokens a thread, the next eight already on their way
+      auto load = [&](int i) {
         float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         if (i + 3 < e1) {
           v = __ldg(reinterpret_cast<const float4*>(x + i));
@@ -619,10 +619,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           if (i + 1 < e1) v.y = __ldg(x + i + 1);
           if (i + 2 < e1) v.z = __ldg(x + i + 2);
         }
+        return v;
+      };
+      auto give = [&](float4 v, int i) {
         f(v.x + 0.f, i);
         f(v.y + 0.f, i + 1);
         f(v.z + 0.f, i + 2);
         f(v.w + 0.f, i + 3);
+      };
+      int i = e0 + 4 * tid;
+      float4 v0 = load(i), v1 = load(i + 4 * kThreads);
+      for (int i0 = e0; i0 < e1; i0 += 8 * kThreads, i += 8 * kThreads) {
+        const float4 n0 = load(i + 8 * kThreads), n1 = load(i + 12 * kThreads);
+        give(v0, i);
+        give(v1, i + 4 * kThreads);
+        v0 = n0;
+        v1 = n1;
       }
     } else {
 #pragma unroll 4
@@ -661,7 +673,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     mx = fmaxf(mx, R->mx);
     mn = fminf(mn, R->mn);
   }
-  const bool none = mx == -INFINITY, slow0 = mx == INFINITY;
+  // rows of values near -1e30, or of steps that reach there, are left to the byte-wise form:
+  // below, what lies in the bins' range is a candidate
+  const bool none = mx == -INFINITY, slow0 = mx == INFINITY || (!none && (mx < -9e29f || P.t > 1e27));
   Bins B;
   if (!none && !slow0) {
     // the range: all candidates, but at most 64 in x and 64 in x / t (whichever is more, steps of at most 2)
@@ -678,20 +692,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   FastSmem* L = cl.map_shared_rank(&S, 0);
   bool wide = !none && !slow0 && !B.poly;  // the 64-bit form
   if (!none && !slow0) {
-    if (tid < kPer) S.unit[tid] = exp(-(double)tid * B.stepd) * (1.0 / (1 << kQBits));
+    if (tid < 4) S.unit[tid] = exp(-(double)tid * B.stepd) * (1.0 / (1 << kQBits));
     if (!wide)
       each([&](float v, int) {
-        if (v >= -1e30f) {
-          const float p = bin_place(B, v), pr = p + kRound;
-          int b = kBins - 1;
-          if (in_range(p)) {
-            b = __float_as_int(pr) - __float_as_int(kRound);
-            atomicAdd(&S.sum[b], (uint32_t)((1 << 22) - q_short(bin_rest(B, v, p, pr - kRound))));
-          }
+        const float p = bin_place(B, v), pr = p + kRound;
+        if (in_range(p)) {
+          const int b = __float_as_int(pr) - __float_as_int(kRound);
+          atomicAdd(&S.sum[b], (uint32_t)((1 << 22) - q_short(bin_rest(B, v, p, pr - kRound))));
           atomicAdd(&S.cnt[b], 1u);
         }
       });
   }
+  // bin_unit's factor for the leader's bins, while other CTAs count
+  const double e4 = rank == 0 && !none && !slow0 ? exp(-(double)((tid * (kBins / kThreads)) & ~3) * B.stepd) : 0.0;
   cl.sync();
   if (none || slow0) {  // the same in every CTA of the cluster
     if (rank == 0) {
@@ -701,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           if (a.probs) a.probs[row] = 0.f;
         }
       } else {
-        sample_generic(a, row, *reinterpret_cast<GenericSmem*>(dsm));
+        sample_generic<kThreads>(a, row, *reinterpret_cast<GenericSmem*>(dsm));
       }
     }
     return;
@@ -709,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   for (;;) {
     if (wide) {
       each([&](float v, int) {
-        if (v >= -1e30f) {
+        if (in_range(bin_place(B, v))) {
           uint32_t q;
           const int b = bin_of(B, v, q);
           atomicAdd(&S.hist[b], kCountOne + q);
@@ -717,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       });
       cl.sync();
     }
-    if (rank == 0) leader_ranges(S, cl, B, P, C, wide);
+    if (rank == 0) leader_ranges<kThreads>(S, cl, B, P, C, wide, e4);
     cl.sync();
     if (!L->rg.redo) break;
     wide = true;  // a bin holds too many tokens for the 32-bit sums: once more
@@ -726,16 +739,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   // ---- the tokens of those bins: gathered in the CTA, then in the leader
   {
-    const Ranges R = L->rg;
+    if (rank != 0) {
+      if (tid == 0) S.rg = L->rg;
+      __syncthreads();
+    }
+    float lo[4], hi[4];  // the ranges in places, ends included (a tie may lie on either side)
+#pragma unroll
+    for (int j = 0; j < 4; j++) lo[j] = (float)S.rg.lo[j] - 0.5f, hi[j] = (float)S.rg.hi[j] + 0.5f;
     each([&](float v, int i) {
       const float p = bin_place(B, v);
-      const int b = __float_as_int(p + kRound) - __float_as_int(kRound);  // as bin_of, where in_range
-      bool in = false;
+      if (((p >= lo[0]) & (p <= hi[0])) | ((p >= lo[1]) & (p <= hi[1])) | ((p >= lo[2]) & (p <= hi[2])) |
+          ((p >= lo[3]) & (p <= hi[3]))) {
+        const int b = __float_as_int(p + kRound) - __float_as_int(kRound);
+        bool in = false;
 #pragma unroll
-      for (int j = 0; j < 4; j++) in |= b >= R.lo[j] && b <= R.hi[j];
-      if (in && v >= -1e30f && in_range(p)) {
-        const uint32_t to = atomicAdd(&S.n_list, 1u);
-        if (to < kList) S.list[to] = (unsigned long long)order_key(v) << 32 | (uint32_t)~i;
+        for (int j = 0; j < 4; j++) in |= b >= S.rg.lo[j] && b <= S.rg.hi[j];
+        if (in && in_range(p)) {
+          const uint32_t to = atomicAdd(&S.n_list, 1u);
+          if (to < kList) S.list[to] = (unsigned long long)order_key(v) << 32 | (uint32_t)~i;
+        }
       }
     });
     if (C > 1) {
@@ -756,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const int nl = (int)S.n_list;
   if (nl > kList) {
     __syncthreads();
-    sample_generic(a, row, *reinterpret_cast<GenericSmem*>(dsm));
+    sample_generic<kThreads>(a, row, *reinterpret_cast<GenericSmem*>(dsm));
     return;
   }
   // ---- the gathered tokens in order (a bitonic sort, falling), then the place
@@ -765,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   while (np < nl) np *= 2;
   for (int i = nl + tid; i < np; i += kThreads) S.list[i] = 0;
   __syncthreads();
-  bitonic_falling(S.list, np);
+  bitonic_falling<kThreads>(S.list, np);
   constexpr int kMine = kList / kThreads;  // consecutive tokens of a thread
   unsigned long long* before = reinterpret_cast<unsigned long long*>(xs);  // sum of q before each; the slice is done with
   int* bins = reinterpret_cast<int*>(before + kList);
@@ -788,8 +810,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   if (lane == 31) S.lsum[warp] = incl;
   __syncthreads();
-  unsigned long long pre = incl - sum;
-  for (int w = 0; w < warp; w++) pre += S.lsum[w];
+  unsigned long long pre, all;
+  warp_sums<kThreads>(S.lsum, pre, all);
+  pre += incl - sum;
   int first = 0;
 #pragma unroll
   for (int j = 0; j < kMine; j++) {
@@ -809,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (lane == 0) prev = 0;
   if (lane == 31) S.wcnt[warp] = (uint32_t)most;
   __syncthreads();
-  for (int w = 0; w < warp; w++) prev = max(prev, (int)S.wcnt[w]);
+  prev = max(prev, __reduce_max_sync(0xffffffffu, lane < warp ? (int)S.wcnt[lane] : 0));
   uint32_t num[kMine];
   double cum[kMine];
 #pragma unroll
@@ -894,10 +917,11 @@ int cluster_size(int rows, int n) {
   return c;
 }
 
-cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
-  const int c = cluster_size(a.rows, a.n), per = ((a.n + c - 1) / c + 3) & ~3, staged = per <= kSlice;
+template <int kThreads>
+cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
+  const int per = ((a.n + c - 1) / c + 3) & ~3, staged = per <= kSlice;
   const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 : 0, kList * 12);
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)(sizeof(FastSmem) + kSlice * 4));
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at = {};
@@ -911,7 +935,15 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel, a, staged);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<kThreads>, a, staged);
+}
+
+// 1024 threads while every cluster finds SMs of its own (clusters of 8 do not
+// fill the GPCs' SMs: 16 rows took two rounds, 49 us against 37), else two CTAs
+// of 512 an SM.
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
+  const int c = cluster_size(a.rows, a.n);
+  return (long long)a.rows * c <= 64 && a.n / c >= 4096 ? launch_sample<1024>(a, c, st) : launch_sample<512>(a, c, st);
 }
 
 }  // namespace
