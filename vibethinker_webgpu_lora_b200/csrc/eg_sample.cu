@@ -275,7 +275,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kBins = 2048;        // the last one: past the range
 constexpr int kList = 1024;        // gathered tokens
-constexpr int kSlice = 19456;      // most tokens that a CTA stages (76 KB: two CTAs an SM)
+constexpr int kSlice = 19200;      // most tokens that a CTA stages (75 KB: two CTAs an SM)
+constexpr int kHits = 8192, kStagedHits = 1024;  // ids that a pass may pick before they are checked
 constexpr int kQBits = 26;
 constexpr uint32_t kQBase = (1u << kQBits) - (1u << 22);
 constexpr uint32_t kDense = 512;   // tokens of a CTA in one bin, at most, in the usual form
@@ -284,6 +285,7 @@ constexpr float kRound = 12582912.f;  // 1.5 2^23: x + kRound rounds |x| < 2^22 
 
 struct Ranges {  // bins [lo, hi] of: top-k, top-p, min-p, the sample (lo > hi: none)
   int lo[4], hi[4], redo;
+  float from[4], to[4];  // the same as windows of values, a little wide: the sample, top-p, top-k, min-p
 };
 
 struct __align__(16) FastSmem {
@@ -312,35 +314,31 @@ struct __align__(16) FastSmem {
 };
 
 struct Bins {
-  float xmax, sh, sl, step;  // 1 / bin width as a hi + lo pair; step: bin width / t
-  bool poly;                 // step <= 1/16: e^-u by its series
-  double stepd;
+  float xmax, width, inv_width, inv_t;  // width has 12 significant bits: r * width is exact for every bin r
+  bool poly;                            // steps of x / t up to 1/16: e^-u by its series
+  double step;                          // width / t
 };
 
-// A candidate's place p = (xmax - x) / width, its bin the nearest integer.
-__device__ __forceinline__ float bin_place(const Bins& B, float x) {
-  return __fmul_rn(B.xmax - x, B.sh);  // not to be fused with p - r below: e holds its rounding
-}
+// A candidate's place (xmax - x) / width; its bin is the nearest integer.
+__device__ __forceinline__ float bin_place(const Bins& B, float x) { return __fmul_rn(B.xmax - x, B.inv_width); }
 __device__ __forceinline__ bool in_range(float p) { return p < (float)(kBins - 2) + 0.5f; }
-// u of a candidate in bin r (a float).  The place is carried as p + e (the
-// difference exact by a two-term sum, the product by fma), so the part beyond
-// the bin is right to 2^-36 of the range.
-__device__ __forceinline__ float bin_rest(const Bins& B, float x, float p, float r) {
+// u of a candidate in bin r: d + dl = xmax - x exactly (two-term sum), d - r
+// width exactly, then one rounding of each operation: right to 2^-23 of u.
+__device__ __forceinline__ float bin_rest(const Bins& B, float x, float r) {
   const float d = B.xmax - x;
   const float bb = d - B.xmax;
-  const float dl = (B.xmax - (d - bb)) - (x + bb);  // d + dl = xmax - x
-  const float e = __fadd_rn(fmaf(d, B.sh, -p), fmaf(d, B.sl, __fmul_rn(dl, B.sh)));
-  return __fmul_rn(__fadd_rn(p - r, e), B.step);  // |u| <= step / 2 (a little more by e)
+  const float dl = (B.xmax - (d - bb)) - (x + bb);
+  return __fmul_rn(__fadd_rn(fmaf(-r, B.width, d), dl), B.inv_t);  // |u| <= step / 2 (a little more by place's rounding)
 }
-// 2^26 (1 - e^-u) + kRound, an integer in the low bits, for |u| <= 1/32:
-// 1 - e^-u = u (1 - u/2 (1 - u/3 (1 - u/4 (1 - u/5)))), the next term below 2^-39
+// 2^26 (1 - e^-u), rounded, for |u| <= 1/32: u (1 - u (1/2 - u (1/6 - u (1/24
+// - u / 120)))), the next term below 2^-39; fused as written, so that every
+// caller gets the same integer
 __device__ __forceinline__ int q_short(float u) {
-  float y = fmaf(u, -0.2f, 1.f);  // fused as written: every caller gets the same q
-  y = fmaf(__fmul_rn(u, -0.25f), y, 1.f);
-  y = fmaf(__fmul_rn(u, -1.f / 3.f), y, 1.f);
-  y = fmaf(__fmul_rn(u, -0.5f), y, 1.f);
-  y = __fmul_rn(u, y);
-  return __float_as_int(fmaf(y, (float)(1 << kQBits), kRound)) - __float_as_int(kRound);
+  float y = fmaf(-u, 1.f / 120.f, 1.f / 24.f);
+  y = fmaf(-u, y, 1.f / 6.f);
+  y = fmaf(-u, y, 0.5f);
+  y = fmaf(-u, y, 1.f);
+  return __float_as_int(fmaf(__fmul_rn(u, (float)(1 << kQBits)), y, kRound)) - __float_as_int(kRound);
 }
 __device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
   const float p = bin_place(B, x);
@@ -349,14 +347,14 @@ __device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
     return kBins - 1;
   }
   const float r = (p + kRound) - kRound;
-  const float u = bin_rest(B, x, p, r);
+  const float u = bin_rest(B, x, r);
   q = B.poly ? (1u << kQBits) - q_short(u) : (uint32_t)__double2ll_rn(exp(-(double)u) * (double)(1 << kQBits));
   return (int)r;
 }
 
 // The weight of q = 1 in bin b; units[j]: of bin j (4 of them).
 __device__ __forceinline__ double bin_unit(const Bins& B, const double* units, int b) {
-  return exp(-(double)(b & ~3) * B.stepd) * units[b & 3];
+  return exp(-(double)(b & ~3) * B.step) * units[b & 3];
 }
 // sums over the warps before this one and over all, of one value a warp in shared memory
 template <int kThreads, typename T>
@@ -550,7 +548,7 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
     hi = fmin(hi, mass_above(p_hi + 1));
   }
   if (P.minp > 0.0) {
-    const double pos = -log(P.minp) / B.stepd;
+    const double pos = -log(P.minp) / B.step;
     if (pos < kBins - 2) {
       m_lo = max(0, (int)rint(pos - 0.01));
       m_hi = max(0, min(kBins - 2, (int)rint(pos + 0.01)));
@@ -562,7 +560,16 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
   cross_mass(P.r * lo * (1.0 - 1e-12), 3);
   cross_mass(P.r * hi * (1.0 + 1e-12), 4);
   __syncthreads();
-  if (tid == 0) {
+  if (tid < 4) {
+    // a bin's tokens lie within half a width of its middle, give or take the rounding of a place
+    const int wl = tid == 0 ? min(S.cross[3], last) : tid == 1 ? p_lo : tid == 2 ? (k_on ? kb : 1) : m_lo;
+    const int wh = tid == 0 ? min(S.cross[4], last) : tid == 1 ? p_hi : tid == 2 ? (k_on ? kb : 0) : m_hi;
+    const double slack = 0.01 * B.width + 0x1p-21 * (fabs((double)B.xmax) + (wh + 1.0) * B.width);
+    const bool some = wl <= wh;
+    S.rg.from[tid] = some ? __double2float_rd((double)B.xmax - (wh + 0.5) * B.width - slack) : INFINITY;
+    S.rg.to[tid] = some ? __double2float_ru((double)B.xmax - (wl - 0.5) * B.width + slack) : -INFINITY;
+  }
+  if (tid == 32) {
     Ranges& R = S.rg;
     R.lo[0] = k_on ? kb : 1, R.hi[0] = k_on ? kb : 0;
     R.lo[1] = p_lo, R.hi[1] = p_hi;
@@ -606,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 #pragma unroll 4
       for (int i0 = e0; i0 < e1; i0 += kThreads) {
         const int i = i0 + tid;
-        f(i < e1 ? xs[i - e0] + 0.f : -INFINITY, i);
+        f(i < e1 ? xs[i - e0] : -INFINITY, i);
       }
     } else if (vec) {
       // eight tokens a thread, the next eight already on their way
@@ -622,10 +629,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         return v;
       };
       auto give = [&](float4 v, int i) {
-        f(v.x + 0.f, i);
-        f(v.y + 0.f, i + 1);
-        f(v.z + 0.f, i + 2);
-        f(v.w + 0.f, i + 3);
+        f(v.x, i);
+        f(v.y, i + 1);
+        f(v.z, i + 2);
+        f(v.w, i + 3);
       };
       int i = e0 + 4 * tid;
       float4 v0 = load(i), v1 = load(i + 4 * kThreads);
@@ -640,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 #pragma unroll 4
       for (int i0 = e0; i0 < e1; i0 += kThreads) {
         const int i = i0 + tid;
-        f(i < e1 ? __ldg(x + i) + 0.f : -INFINITY, i);
+        f(i < e1 ? __ldg(x + i) : -INFINITY, i);
       }
     }
   };
@@ -667,11 +674,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     if (lane == 0) S.mx = mx, S.mn = mn;
   }
   cl.sync();
-  mx = -INFINITY, mn = INFINITY;
-  for (int c = 0; c < C; c++) {
-    const FastSmem* R = cl.map_shared_rank(&S, c);
-    mx = fmaxf(mx, R->mx);
-    mn = fminf(mn, R->mn);
+  {
+    const FastSmem* R = cl.map_shared_rank(&S, min(lane, C - 1));
+    mx = warp_max(R->mx);
+    mn = -warp_max(-R->mn);
   }
   // rows of values near -1e30, or of steps that reach there, are left to the byte-wise form:
   // below, what lies in the bins' range is a candidate
@@ -681,30 +687,30 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     // the range: all candidates, but at most 64 in x and 64 in x / t (whichever is more, steps of at most 2)
     const double cap = fmax(64.0 * P.t, fmin(64.0, 2.0 * (kBins - 2) * P.t));
     const double range = fmin((double)mx - (double)mn, cap);
-    const double s = fmin((kBins - 2) / range, 1e30);  // equal logits: one bin
+    const float w = (float)fmax(range / (kBins - 2), 1e-30);  // equal logits: one bin
     B.xmax = mx;
-    B.sh = (float)s;
-    B.sl = (float)(s - (double)B.sh);
-    B.stepd = 1.0 / (s * P.t);
-    B.step = (float)B.stepd;
-    B.poly = B.stepd <= 0.0625;
+    B.width = __uint_as_float((__float_as_uint(w) + 0xfff) & ~0xfffu);
+    B.inv_width = 1.f / B.width;
+    B.inv_t = (float)(1.0 / P.t);
+    B.step = (double)B.width / P.t;
+    B.poly = B.step <= 0.0625;
   }
   FastSmem* L = cl.map_shared_rank(&S, 0);
   bool wide = !none && !slow0 && !B.poly;  // the 64-bit form
   if (!none && !slow0) {
-    if (tid < 4) S.unit[tid] = exp(-(double)tid * B.stepd) * (1.0 / (1 << kQBits));
+    if (tid < 4) S.unit[tid] = exp(-(double)tid * B.step) * (1.0 / (1 << kQBits));
     if (!wide)
       each([&](float v, int) {
         const float p = bin_place(B, v), pr = p + kRound;
         if (in_range(p)) {
           const int b = __float_as_int(pr) - __float_as_int(kRound);
-          atomicAdd(&S.sum[b], (uint32_t)((1 << 22) - q_short(bin_rest(B, v, p, pr - kRound))));
+          atomicAdd(&S.sum[b], (uint32_t)((1 << 22) - q_short(bin_rest(B, v, pr - kRound))));
           atomicAdd(&S.cnt[b], 1u);
         }
       });
   }
   // bin_unit's factor for the leader's bins, while other CTAs count
-  const double e4 = rank == 0 && !none && !slow0 ? exp(-(double)((tid * (kBins / kThreads)) & ~3) * B.stepd) : 0.0;
+  const double e4 = rank == 0 && !none && !slow0 ? exp(-(double)((tid * (kBins / kThreads)) & ~3) * B.step) : 0.0;
   cl.sync();
   if (none || slow0) {  // the same in every CTA of the cluster
     if (rank == 0) {
@@ -743,23 +749,45 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       if (tid == 0) S.rg = L->rg;
       __syncthreads();
     }
-    float lo[4], hi[4];  // the ranges in places, ends included (a tie may lie on either side)
-#pragma unroll
-    for (int j = 0; j < 4; j++) lo[j] = (float)S.rg.lo[j] - 0.5f, hi[j] = (float)S.rg.hi[j] + 0.5f;
+    const float from0 = S.rg.from[0], to0 = S.rg.to[0], from1 = S.rg.from[1], to1 = S.rg.to[1];
+    const float from2 = S.rg.from[2], to2 = S.rg.to[2], from3 = S.rg.from[3], to3 = S.rg.to[3];
+    const bool more = from2 <= to2 || from3 <= to3;
+    // a warp's hits go to its own part of a list of ids: no atomics in the pass
+    const uint32_t room = (staged ? kStagedHits : kHits) / (kThreads / 32);
+    uint32_t* hits = reinterpret_cast<uint32_t*>(dsm + sizeof(FastSmem) + (staged ? per * 4 : 0)) + warp * room;
+    const uint32_t below = (1u << lane) - 1;
+    uint32_t nh = 0;
     each([&](float v, int i) {
-      const float p = bin_place(B, v);
-      if (((p >= lo[0]) & (p <= hi[0])) | ((p >= lo[1]) & (p <= hi[1])) | ((p >= lo[2]) & (p <= hi[2])) |
-          ((p >= lo[3]) & (p <= hi[3]))) {
-        const int b = __float_as_int(p + kRound) - __float_as_int(kRound);
-        bool in = false;
-#pragma unroll
-        for (int j = 0; j < 4; j++) in |= b >= S.rg.lo[j] && b <= S.rg.hi[j];
-        if (in && in_range(p)) {
-          const uint32_t to = atomicAdd(&S.n_list, 1u);
-          if (to < kList) S.list[to] = (unsigned long long)order_key(v) << 32 | (uint32_t)~i;
-        }
+      bool hit = ((v >= from0) & (v <= to0)) | ((v >= from1) & (v <= to1));
+      if (more) hit |= ((v >= from2) & (v <= to2)) | ((v >= from3) & (v <= to3));
+      const uint32_t vote = __ballot_sync(0xffffffffu, hit);
+      if (vote) {
+        const uint32_t to = nh + __popc(vote & below);
+        if (hit && to < room) hits[to] = (uint32_t)i;
+        nh += __popc(vote);
       }
     });
+    __syncwarp();
+    if (nh > room && lane == 0) atomicAdd(&S.n_list, kList + 1u);
+    for (uint32_t k0 = 0; k0 < min(nh, room); k0 += 32) {
+      bool in = false;
+      uint32_t id = 0;
+      float v = 0.f;
+      if (k0 + lane < min(nh, room)) {
+        id = hits[k0 + lane];
+        v = staged ? xs[id - e0] : __ldg(x + id);
+        const float p = bin_place(B, v);
+        const int b = __float_as_int(p + kRound) - __float_as_int(kRound);  // as bin_of, where in_range
+#pragma unroll
+        for (int j = 0; j < 4; j++) in |= b >= S.rg.lo[j] && b <= S.rg.hi[j];
+        in &= in_range(p);
+      }
+      const uint32_t vote = __ballot_sync(0xffffffffu, in);
+      uint32_t to = 0;
+      if (lane == 0 && vote) to = atomicAdd(&S.n_list, (uint32_t)__popc(vote));
+      to = __shfl_sync(0xffffffffu, to, 0) + __popc(vote & below);
+      if (in && to < kList) S.list[to] = (unsigned long long)order_key(v) << 32 | ~id;
+    }
     if (C > 1) {
       __syncthreads();
       if (rank != 0) {
@@ -920,9 +948,9 @@ int cluster_size(int rows, int n) {
 template <int kThreads>
 cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
   const int per = ((a.n + c - 1) / c + 3) & ~3, staged = per <= kSlice;
-  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 : 0, kList * 12);
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)(sizeof(FastSmem) + kSlice * 4));
+  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 + kStagedHits * 4 : kHits * 4, kList * 12);
+  static_assert(sizeof(FastSmem) + kSlice * 4 + kStagedHits * 4 <= 113 << 10, "two CTAs an SM");
+  const cudaError_t e = cudaFuncSetAttribute(sample_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 << 10);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at = {};
   at.id = cudaLaunchAttributeClusterDimension;
