@@ -108,14 +108,16 @@ __global__ void __launch_bounds__(256) kv_append_paged_kernel(AppendArgs a) {
 // Row r = b * G + g of a KV head is query head kvh * G + g of sequence b
 // (G = nh / nkv).  o = softmax(q k^T / sqrt(128)) v over the prefix's keys and
 // the sequence's own.  The keys are cut into splits; each split of a row
-// gives (m, l, o) with m the running maximum of s2 = q.k * log2(e)/sqrt(128),
-// l = sum p, o = sum p v, p = 2^(s2 - m + kPBits), and the combine weighs the
-// splits by 2^(m - max m).  kPBits lifts p to (0, 2^14]: its f16 hi + lo parts
-// then keep an absolute error of 2^-39 of the largest weight, so many small
-// weights beside one large one are not lost below the f16 range.
+// gives (b, l, o) with p = 2^(s2 - b), s2 = q.k * log2(e)/sqrt(128), l = sum p,
+// o = sum p v, and the combine weighs the splits by 2^(b - max b).  The base b
+// is the running maximum less kPBits: p reaches up to 2^14, and its f16 hi + lo
+// parts keep an absolute error of 2^-39 of the largest weight, so many small
+// weights beside one large one are not lost below the f16 range.  The parts of
+// split s lie at [s][KV head][row], a row's 16-byte pieces at place c ^ (row & 7).
 constexpr float kPBits = 14.f;
 constexpr int kWarps = 4;       // warps of a CTA, each with its own 16-key tiles
 constexpr int kSms = 148;       // plans are made for the B200's SM count
+constexpr int kTcMaxKeys = 2048;  // keys of a prefix split on the tensor cores
 
 struct SharedPlan {
   int G, gch;          // query heads per KV head; chunks of 8 of them
@@ -140,7 +142,7 @@ struct SharedArgs {
   int max_len;
   float* out;
   long long ldo;
-  float *pm, *pl, *po;  // [split][nseq * nh] and [...][128]
+  float *pm, *pl, *po;  // [split][KV head][row] and [...][128]
   int* err;
   SharedPlan p;
 };
@@ -156,9 +158,16 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   p.row_tiles = (p.rows + 127) / 128;
   p.tc = kv_f16 && p.rows > 8 && prefix_len >= 256;
   if (p.tc) {
-    // one CTA an SM, an even number of 128-key blocks each
-    const int units = p.row_tiles * nkv, want = std::max(1, kSms / units);
-    p.pref_keys = round_up((prefix_len + want - 1) / want, 256);
+    // one CTA an SM: the number of splits with the shortest rounds, at about 6 us
+    // a CTA and 1.3 us a block
+    const int units = p.row_tiles * nkv;
+    double best = 1e300;
+    for (int n = (prefix_len + kTcMaxKeys - 1) / kTcMaxKeys; n <= std::max(1, prefix_len / 256); n++) {
+      const int keys = round_up((prefix_len + n - 1) / n, 128), got = (prefix_len + keys - 1) / keys;
+      const double t = (double)(((long long)units * got + kSms - 1) / kSms) * (6.0 + 1.3 * (keys / 128)) + 0.05 * got;
+      if (t < best) best = t, p.pref_keys = keys;
+      if ((long long)units * n > 4 * kSms && n > (prefix_len + kTcMaxKeys - 1) / kTcMaxKeys) break;
+    }
   } else {
   // about four CTAs an SM, never under 128 keys a split and never above 1024:
   // the tensor core's f32 sums lose about 2^-25.5 a step, all one way, so a
@@ -431,13 +440,12 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
       o.z += f * x.z;
       o.w += f * x.w;
     }
-    const int rr = row0 + r;
-    const size_t at = (size_t)split * a.nseq * a.nh + (size_t)(rr / G) * a.nh + kvh * G + rr % G;
+    const size_t at = ((size_t)split * a.nkv + kvh) * p.rows + row0 + r;
     if (c == 0) {
-      a.pm[at] = mm;
+      a.pm[at] = mm - kPBits;
       a.pl[at] = l;
     }
-    reinterpret_cast<float4*>(a.po + at * kHeadDim)[c] = o;
+    reinterpret_cast<float4*>(a.po + at * kHeadDim)[c ^ ((row0 + r) & 7)] = o;
   }
   // launched beside the prefix kernel, whose results it does not need: its end
   // waits for that kernel's, so that the combine, which follows it, finds both
@@ -450,11 +458,13 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
 // A CTA takes 128 rows of one KV head over one split of the prefix, in blocks
 // of 128 keys: S = q K^T (M = rows, N = keys; q as f16 hi + lo stacked on the
 // same K: 16 MMAs of K = 16), softmax by one thread a row from TMEM, P back to
-// TMEM as f16 hi + lo over S's own columns, O = P V (A from TMEM, V^T as the
+// TMEM as f16 hi + lo over S's own columns, O += P V (A from TMEM, V^T as the
 // key-major tile read MN-major; 16 MMAs).  Two warpgroups take the blocks in
-// turn, so one's softmax runs under the other's products.  O of a block is a
-// fresh accumulator added to the row's f32 registers: a TMEM sum over many
-// blocks would lose 2^-25.5 a step, all one way.
+// turn, so one's softmax runs under the other's products.  O stays in TMEM: a
+// row's base b moves (and its O is scaled) only when the maximum passes b by
+// kTcBits + kTcSlack bits, which after the first block is rare.  The tensor
+// core's sums lose about 2^-25.5 a step, all one way: a split's 2048 keys are
+// 128 steps a warpgroup, 2.5e-6 at most.
 // Warps: 0-3 and 4-7 softmax, 8 copies K, 9 copies V (TMA: a page of one KV
 // head is two boxes of 16 rows x 64 dims, 128-byte swizzle), 10 issues MMAs and
 // owns TMEM.
@@ -463,14 +473,14 @@ constexpr uint32_t kTcTile = 128 * kHeadDim * 2;  // 32 KB: 128 rows or keys of 
 constexpr uint32_t kTcHalf = kTcTile / 2;         // 128 keys x 64 dims, 128-byte rows
 constexpr int kTcSmem = 6 * kTcTile;              // q hi, q lo, 2 x (K, V)
 constexpr uint32_t kTcCols = 512;                 // per warpgroup 128 of S / P and 128 of O
-constexpr int kTcPitch = kHeadDim + 4;            // floats a row of the closing exchange
+constexpr float kTcBits = 7.f, kTcSlack = 8.f;    // p up to 2^15 (f16: 65504), 2^7 at the block's maximum where b was set
 
 struct TcSmem {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], v_raw;
   uint32_t tmem;
   int err;
   int nv[2][8];  // valid keys of each page of a stage's block
-  float m[128], l[128];
+  float m[128], l[128], m0[128];
 };
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
@@ -562,7 +572,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
   bool dead = false;
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < 10) {
       // ------------------------------------------------ K (warp 8) and V (warp 9) of every block
       const bool is_v = warp == 9;
@@ -645,7 +655,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
           for (int i = 0; i < 8; i++) {
             const uint32_t pc = tmem + w * 256 + 32 * (i >> 1) + 8 * (i & 1);
             const uint64_t vd = smem_desc_sw128(V + i * 2048, kTcHalf, 1024);  // 16 keys of all dims
-            mma_f16_ts(tmem + w * 256 + 128, pc, vd, id_o, i > 0);
+            mma_f16_ts(tmem + w * 256 + 128, pc, vd, id_o, i > 0 || j > 1);
             mma_f16_ts(tmem + w * 256 + 128, pc + 16, vd, id_o, true);
           }
           mma_commit(&S.o_full[w]);
@@ -658,148 +668,168 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
       for (int j = max(0, nblk - 2); j < nblk; j++) tc_wait_bounded(&S.o_full[j & 1], (j >> 1) & 1);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------ softmax, one thread a row
-    const int w = warp >> 2, r = tid & 127, row = tile * 128 + r, G = p.G;
+    const int w = warp >> 2, r = tid & 127, G = p.G;
     {
-      // q of the row, dims 64 w .. 64 w + 63, times log2(e) / sqrt(128), as f16 hi and lo
-      const bool on = row < p.rows;
+      // q times log2(e) / sqrt(128) as f16 hi and lo: 8 rows x 4 float4 a load (full sectors, 8 lines)
       const float c = 1.4426950408889634f * 0.08838834764831845f;
-      const float* q = a.q + (on ? (long long)(row / G) * a.ldq + (kvh * G + row % G) * kHeadDim + 64 * w : 0);
+      float4 x[16];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (on) {
-          x = __ldg(reinterpret_cast<const float4*>(q) + 2 * i);
-          y = __ldg(reinterpret_cast<const float4*>(q) + 2 * i + 1);
-        }
-        uint4 h, l;
-        split2(x.x * c, x.y * c, h.x, l.x);
-        split2(x.z * c, x.w * c, h.y, l.y);
-        split2(y.x * c, y.y * c, h.z, l.z);
-        split2(y.z * c, y.w * c, h.w, l.w);
-        *reinterpret_cast<uint4*>(qs + core_off(r, 8 * w + i)) = h;
-        *reinterpret_cast<uint4*>(qs + kTcTile + core_off(r, 8 * w + i)) = l;
+      for (int g = 0; g < 2; g++) {
+        const int rr = 16 * warp + 8 * g + (lane & 7), gr = tile * 128 + rr;
+        const float* q = a.q + (gr < p.rows ? (long long)(gr / G) * a.ldq + (kvh * G + gr % G) * kHeadDim : 0);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          x[8 * g + i] = gr < p.rows ? __ldg(reinterpret_cast<const float4*>(q) + 4 * i + (lane >> 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+#pragma unroll
+      for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int rr = 16 * warp + 8 * g + (lane & 7), f = 4 * i + (lane >> 3);  // the row's f-th float4: half a chunk
+          const float4 v = x[8 * g + i];
+          uint2 h, l;
+          split2(v.x * c, v.y * c, h.x, l.x);
+          split2(v.z * c, v.w * c, h.y, l.y);
+          const uint32_t at = core_off(rr, f >> 1) + (f & 1) * 8;
+          *reinterpret_cast<uint2*>(qs + at) = h;
+          *reinterpret_cast<uint2*>(qs + kTcTile + at) = l;
+        }
       fence_async_smem();
       mbar_arrive(&S.q_full);
     }
     const uint32_t base = tmem + w * 256 + ((uint32_t)(32 * (warp & 3)) << 16);
-    float O[kHeadDim];
-#pragma unroll
-    for (int i = 0; i < kHeadDim; i++) O[i] = 0.f;
-    float m = -INFINITY, l = 0.f, corr = 0.f;
-    // O (scaled by corr of its block) += the block's accumulator
-    auto take_o = [&](int j) {
-      if (!dead && !tc_wait(&S.o_full[w], (j >> 1) & 1, &S.err)) dead = true;
-      tc_fence_after();
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        uint32_t v[32];
-        tmem_ld32(base + 128 + 32 * i, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int d = 0; d < 32; d++) O[32 * i + d] = fmaf(O[32 * i + d], corr, __uint_as_float(v[d]));
-      }
-    };
+    float m = -INFINITY, l = 0.f;  // the base b is m - kTcBits
     for (int j = w; j < nblk; j += 2) {
       const int nkey = k1 - k0 - j * kTcBlock;
+      // S is there, and with it the warpgroup's last O (the commit covers what was issued before)
       if (!dead && !tc_wait(&S.s_full[w], (j >> 1) & 1, &S.err)) dead = true;
-      if (j >= 2) take_o(j - 2);
       // the block's valid keys: every page whole, but at the end of the prefix (or beside a bad page)
       if (!dead && !tc_wait(&S.v_full[w], (j >> 1) & 1, &S.err)) dead = true;
       bool whole = nkey >= kTcBlock;
 #pragma unroll
       for (int g = 0; g < 8; g++) whole &= S.nv[w][g] == kPage;
       tc_fence_after();
-      float mx = m;
-      if (whole) {
+      uint32_t v[4][32];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          uint32_t v[32];
-          tmem_ld32(base + 32 * i, v);
-          tmem_wait_ld();
+      for (int i = 0; i < 4; i++) tmem_ld32(base + 32 * i, v[i]);
+      tmem_wait_ld();
+      if (!whole) {
 #pragma unroll
-          for (int d = 0; d < 32; d++) mx = fmaxf(mx, __uint_as_float(v[d]));
-        }
-      } else {
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          uint32_t v[32];
-          tmem_ld32(base + 32 * i, v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int d = 0; d < 32; d++) {
-            if (d % kPage >= S.nv[w][2 * i + d / kPage]) v[d] = __float_as_uint(-INFINITY);
-            mx = fmaxf(mx, __uint_as_float(v[d]));
-          }
-          tmem_st32(base + 32 * i, v);
-        }
-        tmem_wait_st();
+          for (int d = 0; d < 32; d++)
+            if (d % kPage >= S.nv[w][2 * i + d / kPage]) v[i][d] = __float_as_uint(-INFINITY);
       }
-      const float b = mx == -INFINITY ? 0.f : mx - kPBits;
-      corr = m == -INFINITY ? 0.f : ex2(m - mx);
-      m = mx;
+      float mx[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        mx[i] = __uint_as_float(v[i][0]);
+#pragma unroll
+        for (int d = 1; d < 32; d++) mx[i] = fmaxf(mx[i], __uint_as_float(v[i][d]));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      if (j < 2) {
+        m = top;
+      } else {
+        const bool up = top > m + kTcSlack;
+        if (__any_sync(0xffffffffu, up)) {
+          const float f = up && m != -INFINITY ? ex2(m - top) : 1.f;
+          l *= f;
+          if (up) m = top;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint32_t o[32];
+            tmem_ld32(base + 128 + 32 * i, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int d = 0; d < 32; d++) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
+            tmem_st32(base + 128 + 32 * i, o);
+          }
+        }
+      }
+      const float b = m == -INFINITY ? 0.f : m - kTcBits;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        uint32_t v[32], o[32];
-        tmem_ld32(base + 32 * i, v);
-        tmem_wait_ld();
+        uint32_t o[32];
 #pragma unroll
         for (int d = 0; d < 16; d++) {
-          const float x = ex2(__uint_as_float(v[2 * d]) - b), y = ex2(__uint_as_float(v[2 * d + 1]) - b);
+          const float x = ex2(__uint_as_float(v[i][2 * d]) - b), y = ex2(__uint_as_float(v[i][2 * d + 1]) - b);
           s0 += x;
           s1 += y;
           split2(x, y, o[d], o[16 + d]);
         }
         tmem_st32(base + 32 * i, o);
       }
-      l = l * corr + (s0 + s1);
+      l += s0 + s1;
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&S.p_full[w]);
     }
+    // ---- the two warpgroups' parts of a row joined, and out: the tile's rows are one run of memory
     const int lastj = nblk - 1 - ((nblk - 1 - w) & 1);  // the warpgroup's last block
-    if (lastj >= 0 && w < nblk) take_o(lastj);
-    // ---- the two warpgroups' parts of a row joined (every MMA is done: both have their last O)
-    float* ex = reinterpret_cast<float*>(kvs);
+    if (w < nblk && !dead && !tc_wait(&S.o_full[w], (lastj >> 1) & 1, &S.err)) dead = true;
+    tc_fence_after();
+    float4* ex = reinterpret_cast<float4*>(kvs) + r * 32;  // [row][32 pieces, swizzled]
     if (w == 1) {
       S.m[r] = m;
       S.l[r] = l;
+    } else {
+      S.m0[r] = m;
     }
-    asm volatile("bar.sync 2, 256;" ::: "memory");
+    asm volatile("bar.sync 2, 256;" ::: "memory");  // both are past their last MMA: K and V are free
+    const float m0 = S.m0[r], m1 = S.m[r], mm = fmaxf(m0, m1);
+    const float f = m == -INFINITY ? 0.f : ex2(m - mm);
     if (w == 1) {
 #pragma unroll
-      for (int i = 0; i < kHeadDim; i += 4)
-        *reinterpret_cast<float4*>(ex + r * kTcPitch + i) = make_float4(O[i], O[i + 1], O[i + 2], O[i + 3]);
-    }
-    asm volatile("bar.sync 2, 256;" ::: "memory");
-    if (w == 0) {
-      const float m1 = S.m[r], mm = fmaxf(m, m1);
-      const float f0 = m == -INFINITY ? 0.f : ex2(m - mm), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
+      for (int i = 0; i < 4; i++) {
+        uint32_t o[32];
+        if (nblk > 1) {
+          tmem_ld32(base + 128 + 32 * i, o);
+          tmem_wait_ld();
+        }
 #pragma unroll
-      for (int i = 0; i < kHeadDim; i += 4) {
-        float4* d = reinterpret_cast<float4*>(ex + r * kTcPitch + i);
-        float4 x = *d;
-        x.x = O[i] * f0 + x.x * f1;
-        x.y = O[i + 1] * f0 + x.y * f1;
-        x.z = O[i + 2] * f0 + x.z * f1;
-        x.w = O[i + 3] * f0 + x.w * f1;
-        *d = x;
-      }
-      if (row < p.rows) {
-        const size_t at = (size_t)split * a.nseq * a.nh + (size_t)(row / G) * a.nh + kvh * G + row % G;
-        a.pm[at] = mm;
-        a.pl[at] = l * f0 + S.l[r] * f1;
+        for (int d = 0; d < 8; d++) {
+          const float* x = reinterpret_cast<const float*>(o) + 4 * d;
+          ex[(8 * i + d) ^ (r & 7)] = nblk > 1 ? make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
       }
     }
     asm volatile("bar.sync 2, 256;" ::: "memory");
-    for (int i = tid; i < 128 * 32; i += 256) {
-      const int rr = i >> 5, c = i & 31, gr = tile * 128 + rr;
-      if (gr >= p.rows) break;
-      const size_t at = (size_t)split * a.nseq * a.nh + (size_t)(gr / G) * a.nh + kvh * G + gr % G;
-      reinterpret_cast<float4*>(a.po + at * kHeadDim)[c] = reinterpret_cast<const float4*>(ex + rr * kTcPitch)[c];
+    const int nrow = min(128, p.rows - tile * 128);
+    const size_t at = ((size_t)split * a.nkv + kvh) * p.rows + tile * 128;
+    if (w == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t o[32];
+        tmem_ld32(base + 128 + 32 * i, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+          const float* x = reinterpret_cast<const float*>(o) + 4 * d;
+          float4 y = ex[(8 * i + d) ^ (r & 7)];
+          y.x += x[0] * f;
+          y.y += x[1] * f;
+          y.z += x[2] * f;
+          y.w += x[3] * f;
+          ex[(8 * i + d) ^ (r & 7)] = y;
+        }
+      }
+      if (r < nrow) {
+        a.pm[at + r] = mm - kTcBits;
+        a.pl[at + r] = l * f + (m1 == -INFINITY ? 0.f : S.l[r] * ex2(m1 - mm));
+      }
+      fence_async_smem();
+      asm volatile("bar.sync 3, 128;" ::: "memory");
+      if (tid == 0) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.po + at * kHeadDim),
+                     "r"(smem_addr(kvs)), "r"(nrow * kHeadDim * 4)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      }
     }
     tc_fence_before();
   }
@@ -817,13 +847,15 @@ __global__ void __launch_bounds__(128) attn_shared_combine(const __grid_constant
   if (row >= a.nseq * a.nh) return;
   const int b = row / a.nh, len = __ldg(a.lens + b);
   if (len < 0) return;  // a padding sequence: its row stays as it is
-  const size_t n = (size_t)a.nseq * a.nh;
+  const size_t n = (size_t)a.nseq * a.nh;  // rows of a split
+  const int G = a.p.G, h = row % a.nh, r = b * G + h % G;
+  const size_t at = (size_t)(h / G) * a.p.rows + r;
   const int ns = a.p.n_pref + (min(len, a.max_len) + a.p.suf_keys - 1) / a.p.suf_keys;
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < ns; s0 += 32) {
     const int s = s0 + lane, cnt = min(32, ns - s0);
-    const float ms = s < ns ? __ldcg(a.pm + s * n + row) : -INFINITY, ls = s < ns ? __ldcg(a.pl + s * n + row) : 0.f;
+    const float ms = s < ns ? __ldcg(a.pm + s * n + at) : -INFINITY, ls = s < ns ? __ldcg(a.pl + s * n + at) : 0.f;
     const float nm = fmaxf(m, warp_max(ms));
     const float f = ms == -INFINITY ? 0.f : exp2f(ms - nm), c = m == -INFINITY ? 0.f : exp2f(m - nm);
     m = nm;
@@ -836,7 +868,7 @@ __global__ void __launch_bounds__(128) attn_shared_combine(const __grid_constant
       float4 x[8];
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        if (j0 + j < cnt) x[j] = __ldcg(reinterpret_cast<const float4*>(a.po + ((s0 + j0 + j) * n + row) * kHeadDim) + lane);
+        if (j0 + j < cnt) x[j] = __ldcg(reinterpret_cast<const float4*>(a.po + ((s0 + j0 + j) * n + at) * kHeadDim) + (lane ^ (r & 7)));
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
@@ -850,7 +882,7 @@ __global__ void __launch_bounds__(128) attn_shared_combine(const __grid_constant
     }
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;  // no key at all: zeros
-  reinterpret_cast<float4*>(a.out + b * a.ldo + (row % a.nh) * kHeadDim)[lane] =
+  reinterpret_cast<float4*>(a.out + b * a.ldo + h * kHeadDim)[lane] =
       make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
