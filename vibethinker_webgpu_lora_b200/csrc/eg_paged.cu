@@ -112,17 +112,20 @@ __global__ void __launch_bounds__(256) kv_append_paged_kernel(AppendArgs a) {
 // o = sum p v, and the combine weighs the splits by 2^(b - max b).  The base b
 // is the running maximum less kPBits: p reaches up to 2^14, and its f16 hi + lo
 // parts keep an absolute error of 2^-39 of the largest weight, so many small
-// weights beside one large one are not lost below the f16 range.  The parts of
-// split s lie at [s][KV head][row], a row's 16-byte pieces at place c ^ (row & 7).
+// weights beside one large one are not lost below the f16 range.  Split s has
+// its bases and sums at [s][KV head][row] and its o at [s][KV head][row / 8]
+// [16-byte piece][row % 8]: a thread a row writes whole sectors, and so does a
+// group of 8 rows.
 constexpr float kPBits = 14.f;
 constexpr int kWarps = 4;       // warps of a CTA, each with its own 16-key tiles
+constexpr int kSoPitch = kHeadDim + 4;  // floats a row of the warps' outputs in shared memory
 constexpr int kSms = 148;       // plans are made for the B200's SM count
 constexpr int kTcMaxKeys = 2048;  // keys of a prefix split on the tensor cores
 
 struct SharedPlan {
   int G, gch;          // query heads per KV head; chunks of 8 of them
-  int rows;            // nseq * G rows per KV head
-  int pref_keys, n_pref, row_groups;  // keys per prefix split, splits, groups of 8 rows
+  int rows, groups;    // nseq * G rows per KV head, in groups of 8
+  int pref_keys, n_pref;  // keys per prefix split, splits
   int tc, row_tiles;   // prefix on the tcgen05 tensor cores, in tiles of 128 rows
   int suf_keys, n_suf;                // keys per suffix split, most splits of a sequence
 };
@@ -142,10 +145,17 @@ struct SharedArgs {
   int max_len;
   float* out;
   long long ldo;
-  float *pm, *pl, *po;  // [split][KV head][row] and [...][128]
+  float *pm, *pl;  // [split][KV head][8 groups rows]
+  float4* po;      // 32 for each of these
   int* err;
   SharedPlan p;
 };
+
+// Where piece c of row r lies in a split's o; its base and sum are at part_row.
+__device__ __forceinline__ size_t part_row(const SharedArgs& a, int split, int kvh, int r) {
+  return ((size_t)split * a.nkv + kvh) * a.p.groups * 8 + r;
+}
+__device__ __forceinline__ size_t part_at(size_t row, int c) { return (row >> 3) * 256 + c * 8 + (row & 7); }
 
 int round_up(int x, int m) { return (x + m - 1) / m * m; }
 
@@ -154,7 +164,7 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   p.G = nh / nkv;
   p.gch = (p.G + 7) / 8;
   p.rows = nseq * p.G;
-  p.row_groups = (p.rows + 7) / 8;
+  p.groups = (p.rows + 7) / 8;
   p.row_tiles = (p.rows + 127) / 128;
   p.tc = kv_f16 && p.rows > 8 && prefix_len >= 256;
   if (p.tc) {
@@ -172,12 +182,14 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   // about four CTAs an SM, never under 128 keys a split and never above 1024:
   // the tensor core's f32 sums lose about 2^-25.5 a step, all one way, so a
   // warp's 16 tiles stay below 2^-20 (256 tiles of a 16384-key split: 1e-5)
-  const long long units = (long long)p.row_groups * nkv;
+  const long long units = (long long)p.groups * nkv;
   const long long want = std::max(1LL, 4LL * kSms / units);
   p.pref_keys = std::min(1024, std::max(128, round_up((int)((prefix_len + want - 1) / want), 64)));
   }
   p.n_pref = (prefix_len + p.pref_keys - 1) / p.pref_keys;
-  p.suf_keys = 128;
+  // suffix: two rounds of CTAs (three an SM) or more, 128 keys a split at least
+  const int pairs = nseq * nkv * p.gch, want = std::max(1, 6 * kSms / pairs);
+  p.suf_keys = std::max(128, round_up((max_len + want - 1) / want, 64));
   p.n_suf = (max_len + p.suf_keys - 1) / p.suf_keys;
   return p;
 }
@@ -271,10 +283,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
   int kvh, row0, nrow, k0, k1, split;
   const uint32_t* table;
   int blk = blockIdx.x;
-  const int pref_blocks = p.tc ? 0 : p.n_pref * p.row_groups * a.nkv;
+  const int pref_blocks = p.tc ? 0 : p.n_pref * p.groups * a.nkv;
   if (blk < pref_blocks) {
-    const int rg = blk % p.row_groups;
-    blk /= p.row_groups;
+    const int rg = blk % p.groups;
+    blk /= p.groups;
     kvh = blk % a.nkv;
     split = blk / a.nkv;
     row0 = 8 * rg;
@@ -412,19 +424,20 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
     sm_l[warp][2 * tq] = l0;
     sm_l[warp][2 * tq + 1] = l1;
   }
-  __syncthreads();  // every warp's tiles are consumed: the staging becomes [warp][8][128] f32
+  __syncthreads();  // every warp's tiles are consumed: the staging becomes [warp][8][kSoPitch] f32
   float* so = reinterpret_cast<float*>(sm);
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    float* d = so + (warp * 8 + 2 * tq) * kHeadDim + 16 * j + g;
+    float* d = so + (warp * 8 + 2 * tq) * kSoPitch + 16 * j + g;
     d[0] = O[j][0];
-    d[kHeadDim] = O[j][1];
+    d[kSoPitch] = O[j][1];
     d[8] = O[j][2];
-    d[kHeadDim + 8] = O[j][3];
+    d[kSoPitch + 8] = O[j][3];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nrow * 32; i += 32 * kWarps) {
-    const int r = i >> 5, c = i & 31;
+  for (int i = threadIdx.x; i < 8 * 32; i += 32 * kWarps) {
+    const int r = i & 7, c = i >> 3;
+    if (r >= nrow) continue;
     float mm = sm_m[0][r];
 #pragma unroll
     for (int w = 1; w < kWarps; w++) mm = fmaxf(mm, sm_m[w][r]);
@@ -433,19 +446,19 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
 #pragma unroll
     for (int w = 0; w < kWarps; w++) {
       const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2f(sm_m[w][r] - mm);
-      const float4 x = reinterpret_cast<const float4*>(so + (w * 8 + r) * kHeadDim)[c];
+      const float4 x = reinterpret_cast<const float4*>(so + (w * 8 + r) * kSoPitch)[c];
       l += f * sm_l[w][r];
       o.x += f * x.x;
       o.y += f * x.y;
       o.z += f * x.z;
       o.w += f * x.w;
     }
-    const size_t at = ((size_t)split * a.nkv + kvh) * p.rows + row0 + r;
+    const size_t at = part_row(a, split, kvh, row0 + r);
     if (c == 0) {
       a.pm[at] = mm - kPBits;
       a.pl[at] = l;
     }
-    reinterpret_cast<float4*>(a.po + at * kHeadDim)[c ^ ((row0 + r) & 7)] = o;
+    a.po[part_at(at, c)] = o;
   }
   // launched beside the prefix kernel, whose results it does not need: its end
   // waits for that kernel's, so that the combine, which follows it, finds both
@@ -480,7 +493,7 @@ struct TcSmem {
   uint32_t tmem;
   int err;
   int nv[2][8];  // valid keys of each page of a stage's block
-  float m[128], l[128], m0[128];
+  float m0[256], m1[256];  // each warpgroup's bases and sums at the end
 };
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
@@ -768,67 +781,60 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
       tc_fence_before();
       mbar_arrive(&S.p_full[w]);
     }
-    // ---- the two warpgroups' parts of a row joined, and out: the tile's rows are one run of memory
+    // ---- the two warpgroups' parts of a row joined: each gives half of its pieces, adds up the other half
     const int lastj = nblk - 1 - ((nblk - 1 - w) & 1);  // the warpgroup's last block
-    if (w < nblk && !dead && !tc_wait(&S.o_full[w], (lastj >> 1) & 1, &S.err)) dead = true;
+    const bool has = w < nblk;
+    if (has && !dead && !tc_wait(&S.o_full[w], (lastj >> 1) & 1, &S.err)) dead = true;
     tc_fence_after();
-    float4* ex = reinterpret_cast<float4*>(kvs) + r * 32;  // [row][32 pieces, swizzled]
-    if (w == 1) {
-      S.m[r] = m;
-      S.l[r] = l;
-    } else {
-      S.m0[r] = m;
-    }
+    float* mine = w ? S.m1 : S.m0;
+    mine[r] = m;
+    mine[128 + r] = l;
     asm volatile("bar.sync 2, 256;" ::: "memory");  // both are past their last MMA: K and V are free
-    const float m0 = S.m0[r], m1 = S.m[r], mm = fmaxf(m0, m1);
+    const float mo = (w ? S.m0 : S.m1)[r], lo = (w ? S.m0 : S.m1)[128 + r], mm = fmaxf(m, mo);
     const float f = m == -INFINITY ? 0.f : ex2(m - mm);
-    if (w == 1) {
+    float4* ex = reinterpret_cast<float4*>(kvs) + r;  // [giver][16 pieces][128 rows]
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        uint32_t o[32];
-        if (nblk > 1) {
-          tmem_ld32(base + 128 + 32 * i, o);
-          tmem_wait_ld();
-        }
+    for (int i = 0; i < 2; i++) {
+      uint32_t o[32];
+      if (has) {
+        tmem_ld32(base + 128 + 64 * (w ^ 1) + 32 * i, o);
+        tmem_wait_ld();
+      }
 #pragma unroll
-        for (int d = 0; d < 8; d++) {
-          const float* x = reinterpret_cast<const float*>(o) + 4 * d;
-          ex[(8 * i + d) ^ (r & 7)] = nblk > 1 ? make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+      for (int d = 0; d < 8; d++) {
+        const float* x = reinterpret_cast<const float*>(o) + 4 * d;
+        ex[(16 * w + 8 * i + d) * 128] = has ? make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
     asm volatile("bar.sync 2, 256;" ::: "memory");
-    const int nrow = min(128, p.rows - tile * 128);
-    const size_t at = ((size_t)split * a.nkv + kvh) * p.rows + tile * 128;
-    if (w == 0) {
+    if (tile * 128 + r < p.rows) {
+      const size_t at = part_row(a, split, kvh, tile * 128 + r);
+      if (w == 0) {
+        a.pm[at] = mm - kTcBits;
+        a.pl[at] = l * f + (mo == -INFINITY ? 0.f : lo * ex2(mo - mm));
+      }
+    }
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        uint32_t o[32];
-        tmem_ld32(base + 128 + 32 * i, o);
+    for (int i = 0; i < 2; i++) {
+      uint32_t o[32];
+      if (has) {
+        tmem_ld32(base + 128 + 64 * w + 32 * i, o);
         tmem_wait_ld();
+      }
+      if (tile * 128 + r < p.rows) {
+        const size_t at = part_at(part_row(a, split, kvh, tile * 128 + r), 16 * w + 8 * i);
 #pragma unroll
         for (int d = 0; d < 8; d++) {
           const float* x = reinterpret_cast<const float*>(o) + 4 * d;
-          float4 y = ex[(8 * i + d) ^ (r & 7)];
-          y.x += x[0] * f;
-          y.y += x[1] * f;
-          y.z += x[2] * f;
-          y.w += x[3] * f;
-          ex[(8 * i + d) ^ (r & 7)] = y;
+          float4 y = ex[(16 * (w ^ 1) + 8 * i + d) * 128];
+          if (has) {
+            y.x += x[0] * f;
+            y.y += x[1] * f;
+            y.z += x[2] * f;
+            y.w += x[3] * f;
+          }
+          a.po[at + 8 * d] = y;
         }
-      }
-      if (r < nrow) {
-        a.pm[at + r] = mm - kTcBits;
-        a.pl[at + r] = l * f + (m1 == -INFINITY ? 0.f : S.l[r] * ex2(m1 - mm));
-      }
-      fence_async_smem();
-      asm volatile("bar.sync 3, 128;" ::: "memory");
-      if (tid == 0) {
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.po + at * kHeadDim),
-                     "r"(smem_addr(kvs)), "r"(nrow * kHeadDim * 4)
-                     : "memory");
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       }
     }
     tc_fence_before();
@@ -838,51 +844,65 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
   if (warp == 10) tmem_free(tmem, kTcCols);
 }
 
-// One warp per (sequence, head): lane s first holds split s's maximum and sum
-// (32 splits at a time), then the warp adds the splits' rows, eight loads in
-// flight.
-__global__ void __launch_bounds__(128) attn_shared_combine(const __grid_constant__ SharedArgs a) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+// One CTA per 8 rows of a KV head, a thread per (row, 16-byte piece): 32 splits
+// at a time, their weights by thread (row, split) through shared memory, eight
+// of a row's parts in flight.
+__global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant__ SharedArgs a) {
+  __shared__ float sb[32][8], sl[32][8];
+  const int kvh = blockIdx.x / a.p.groups, row0 = blockIdx.x % a.p.groups * 8;
+  const int rr = threadIdx.x & 7, c = threadIdx.x >> 3, r = row0 + rr, G = a.p.G;
   pdl_wait();
-  if (row >= a.nseq * a.nh) return;
-  const int b = row / a.nh, len = __ldg(a.lens + b);
-  if (len < 0) return;  // a padding sequence: its row stays as it is
-  const size_t n = (size_t)a.nseq * a.nh;  // rows of a split
-  const int G = a.p.G, h = row % a.nh, r = b * G + h % G;
-  const size_t at = (size_t)(h / G) * a.p.rows + r;
-  const int ns = a.p.n_pref + (min(len, a.max_len) + a.p.suf_keys - 1) / a.p.suf_keys;
+  const int b = r / G, len = r < a.p.rows ? __ldg(a.lens + b) : -1;
+  const bool on = len >= 0;  // a padding sequence's row stays as it is
+  const int ns = on ? a.p.n_pref + (min(len, a.max_len) + a.p.suf_keys - 1) / a.p.suf_keys : 0;
+  const size_t row = part_row(a, 0, kvh, r), step = (size_t)a.nkv * a.p.groups * 8;  // rows of a split
+  const float4* po = a.po + part_at(row, c);
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < ns; s0 += 32) {
-    const int s = s0 + lane, cnt = min(32, ns - s0);
-    const float ms = s < ns ? __ldcg(a.pm + s * n + at) : -INFINITY, ls = s < ns ? __ldcg(a.pl + s * n + at) : 0.f;
-    const float nm = fmaxf(m, warp_max(ms));
-    const float f = ms == -INFINITY ? 0.f : exp2f(ms - nm), c = m == -INFINITY ? 0.f : exp2f(m - nm);
+  for (int s0 = 0; __syncthreads_or(s0 < ns); s0 += 32) {
+    const int s = s0 + c;
+    sb[c][rr] = s < ns ? __ldcg(a.pm + row + s * step) : -INFINITY;
+    sl[c][rr] = s < ns ? __ldcg(a.pl + row + s * step) : 0.f;
+    float4 x[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (s0 + j < ns) x[j] = __ldcg(po + (s0 + j) * step * 32);
+    __syncthreads();
+    float nm = m;
+#pragma unroll 8
+    for (int j = 0; j < 32; j++) nm = fmaxf(nm, sb[j][rr]);
+    __syncthreads();
+    const float mine = sb[c][rr];
+    sb[c][rr] = mine == -INFINITY ? 0.f : exp2f(mine - nm);
+    const float f = m == -INFINITY ? 0.f : exp2f(m - nm);
     m = nm;
-    l = l * c + warp_sum(f * ls);
-    o.x *= c;
-    o.y *= c;
-    o.z *= c;
-    o.w *= c;
-    for (int j0 = 0; j0 < cnt; j0 += 8) {
-      float4 x[8];
+    l *= f;
+    o.x *= f;
+    o.y *= f;
+    o.z *= f;
+    o.w *= f;
+    __syncthreads();
+    for (int j0 = 0; j0 < 32 && s0 + j0 < ns; j0 += 8) {
+      if (j0) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (s0 + j0 + j < ns) x[j] = __ldcg(po + (s0 + j0 + j) * step * 32);
+      }
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        if (j0 + j < cnt) x[j] = __ldcg(reinterpret_cast<const float4*>(a.po + ((s0 + j0 + j) * n + at) * kHeadDim) + (lane ^ (r & 7)));
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
-        if (j0 + j < cnt) {
+        if (s0 + j0 + j < ns) {
+          const float w = sb[j0 + j][rr];
+          l += w * sl[j0 + j][rr];
           o.x += w * x[j].x;
           o.y += w * x[j].y;
           o.z += w * x[j].z;
           o.w += w * x[j].w;
         }
-      }
     }
   }
+  if (!on) return;
   const float inv = l != 0.f ? 1.f / l : 0.f;  // no key at all: zeros
-  reinterpret_cast<float4*>(a.out + b * a.ldo + h * kHeadDim)[lane] =
+  reinterpret_cast<float4*>(a.out + b * a.ldo + (kvh * G + r % G) * kHeadDim)[c] =
       make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
@@ -950,16 +970,15 @@ cudaError_t launch_shared(const SharedArgs& a, int kv_f16, long long blocks, cud
                : launch_pdl((const void*)attn_shared_kernel<float>, (unsigned)blocks, 32 * kWarps,
                             kWarps * WarpTile<float>::kStages * WarpTile<float>::kBytes, a.p.tc, args, st);
   if (e == cudaSuccess)
-    e = launch_pdl((const void*)attn_shared_combine, (unsigned)((a.nseq * a.nh + 3) / 4), 128, 0, blocks > 0 || a.p.tc,
+    e = launch_pdl((const void*)attn_shared_combine, (unsigned)(a.nkv * a.p.groups), 256, 0, blocks > 0 || a.p.tc,
                    args, st);
   return e;
 }
 
 bool misaligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) & (to - 1); }
 
-size_t shared_bytes(const SharedPlan& p, int nseq, int nh) {
-  return (size_t)(p.n_pref + p.n_suf) * nseq * nh * (kHeadDim + 2) * sizeof(float);
-}
+size_t shared_rows(const SharedPlan& p, int nkv) { return (size_t)(p.n_pref + p.n_suf) * nkv * p.groups * 8; }
+size_t shared_bytes(const SharedPlan& p, int nkv) { return shared_rows(p, nkv) * (kHeadDim + 2) * sizeof(float); }
 
 const char* shared_dims(int nseq, int nh, int nkv, int prefix_len, int max_len) {
   if (nseq < 1 || nseq > 65536) return "need 1 <= nseq <= 65536";
@@ -1015,7 +1034,7 @@ EG_API eg_status eg_op_attn_shared_prefix_bytes(int nseq, int nh, int nkv, int p
   if (const char* why = shared_dims(nseq, nh, nkv, prefix_len, max_len)) return fail(EG_ERR_ARG, "attn_shared_prefix: %s", why);
   size_t n = 16;  // enough for either cache type
   for (int f16 = 0; f16 < 2; f16++)
-    n = std::max(n, shared_bytes(shared_plan(nseq, nh, nkv, prefix_len, max_len, f16), nseq, nh));
+    n = std::max(n, shared_bytes(shared_plan(nseq, nh, nkv, prefix_len, max_len, f16), nkv));
   *bytes = n;
   return EG_OK;
 }
@@ -1037,7 +1056,7 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
     return fail(EG_ERR_ARG, "attn_shared_prefix: 16-byte aligned buffers required");
   SharedArgs a = {};
   a.p = shared_plan(nseq, nh, nkv, prefix_len, max_len, kv_f16);
-  const size_t need = shared_bytes(a.p, nseq, nh);
+  const size_t need = shared_bytes(a.p, nkv);
   if (ws_bytes < need)
     return fail(EG_ERR_ARG, "attn_shared_prefix: workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes, (unsigned long long)need);
   a.q = q;
@@ -1056,12 +1075,12 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
   a.max_len = max_len;
   a.out = out;
   a.ldo = ldo;
-  const size_t rows = (size_t)(a.p.n_pref + a.p.n_suf) * nseq * nh;
-  a.po = static_cast<float*>(ws);
-  a.pm = a.po + rows * kHeadDim;
+  const size_t rows = shared_rows(a.p, nkv);
+  a.po = static_cast<float4*>(ws);
+  a.pm = reinterpret_cast<float*>(a.po + rows * (kHeadDim / 4));
   a.pl = a.pm + rows;
   a.err = err;
-  const long long blocks = (a.p.tc ? 0 : (long long)a.p.n_pref * a.p.row_groups * nkv) +
+  const long long blocks = (a.p.tc ? 0 : (long long)a.p.n_pref * a.p.groups * nkv) +
                            (long long)a.p.n_suf * nseq * nkv * a.p.gch;
   if (blocks > 0x7fffffffLL) return fail(EG_ERR_ARG, "attn_shared_prefix: too many splits");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
