@@ -522,6 +522,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -552,7 +558,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
   __shared__ TcSmem S;
   unsigned char* qs = tsm;                  // q hi, then q lo
   unsigned char* kvs = tsm + 2 * kTcTile;   // stage s: K at 2 s tiles, V one further
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the warp's number through a shuffle: known to be the same in all lanes, so the
+  // MMA warp's descriptors stay in uniform registers
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const SharedPlan& p = a.p;
   pdl_launch_dependents();
   int blk = blockIdx.x;
@@ -639,17 +647,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
       // ------------------------------------------------ MMA issue
       // D f32, A and B f16, M = N = 128; for P V the B operand (V) is MN-major
       const uint32_t id_s = (1u << 4) | (16u << 17) | (8u << 24), id_o = id_s | (1u << 16);
+      // descriptors of the first MMA of each kind; the others are constants further (units of 16 bytes)
+      const uint64_t q_desc = smem_desc(qs, 2048, 128), k_desc = smem_desc_sw128(kvs, 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(kvs + kTcTile, kTcHalf, 1024);  // all dims of a key-major tile
       if (!tc_wait(&S.q_full, 0, &S.err)) dead = true;
       auto issue_s = [&](int j) {
-        const int w = j & 1;
+        const uint32_t w = j & 1;
         if (!dead && !tc_wait(&S.k_full[w], (j >> 1) & 1, &S.err)) dead = true;
         tc_fence_after();
-        if (lane == 0) {
-          const unsigned char* K = kvs + 2 * w * kTcTile;
+        const uint64_t kd = k_desc + w * (2 * kTcTile >> 4);
+        const uint32_t d = tmem + w * 256;
+        if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < 16; i++)
-            mma_f16_ss(tmem + w * 256, smem_desc(qs + i * 4096, 2048, 128),
-                       smem_desc_sw128(K + ((i >> 2) & 1) * kTcHalf + (i & 3) * 32, 16, 1024), id_s, i > 0);
+          for (int i = 0; i < 16; i++)  // q hi, then q lo, against the same K
+            mma_f16_ss(d, q_desc + i * (4096 >> 4), kd + ((((i >> 2) & 1) * kTcHalf + (i & 3) * 32) >> 4), id_s, i > 0);
           mma_commit(&S.s_full[w]);
           mma_commit(&S.k_empty[w]);
         }
@@ -658,18 +669,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
       issue_s(0);
       if (nblk > 1) issue_s(1);
       for (int j = 0; j < nblk; j++) {
-        const int w = j & 1;
+        const uint32_t w = j & 1;
         if (!dead && !tc_wait(&S.v_full[w], (j >> 1) & 1, &S.err)) dead = true;
         if (!dead && !tc_wait(&S.p_full[w], (j >> 1) & 1, &S.err)) dead = true;
         tc_fence_after();
-        if (lane == 0) {
-          const unsigned char* V = kvs + (2 * w + 1) * kTcTile;
+        const uint64_t vd = v_desc + w * (2 * kTcTile >> 4);
+        const uint32_t pc = tmem + w * 256, d = pc + 128;
+        if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const uint32_t pc = tmem + w * 256 + 32 * (i >> 1) + 8 * (i & 1);
-            const uint64_t vd = smem_desc_sw128(V + i * 2048, kTcHalf, 1024);  // 16 keys of all dims
-            mma_f16_ts(tmem + w * 256 + 128, pc, vd, id_o, i > 0 || j > 1);
-            mma_f16_ts(tmem + w * 256 + 128, pc + 16, vd, id_o, true);
+          for (int i = 0; i < 8; i++) {  // 16 keys a step: P hi and lo against the same V
+            mma_f16_ts(d, pc + 32 * (i >> 1) + 8 * (i & 1), vd + i * (2048 >> 4), id_o, i > 0 || j > 1);
+            mma_f16_ts(d, pc + 32 * (i >> 1) + 8 * (i & 1) + 16, vd + i * (2048 >> 4), id_o, true);
           }
           mma_commit(&S.o_full[w]);
           mma_commit(&S.v_empty[w]);
