@@ -127,6 +127,7 @@ struct SharedPlan {
   int rows, groups;    // nseq * G rows per KV head, in groups of 8
   int pref_keys, n_pref;  // keys per prefix split, splits
   int tc, row_tiles;   // prefix on the tcgen05 tensor cores, in tiles of 128 rows
+  int own;             // prefix in a kernel of its own (tc, or f32 in CTAs of 16 rows)
   int suf_keys, n_suf;                // keys per suffix split, most splits of a sequence
 };
 
@@ -166,29 +167,38 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   p.rows = nseq * p.G;
   p.groups = (p.rows + 7) / 8;
   p.row_tiles = (p.rows + 127) / 128;
-  p.tc = kv_f16 && p.rows > 8 && prefix_len >= 256;
+  // What the prefix's scores number decides its kernel (16 heads, 2 KV heads):
+  // f16 on the tensor cores from 600,000 on (16 sequences x 2048 14.6 us there,
+  // 13.9 by warps; 16 x 4096 15.4 and 18.1; 64 x 1024 14.4 and 17.3); f32 in
+  // CTAs of 16 rows from 250,000 on (16 x 512 11.4 us there, 10.6 in CTAs of 8;
+  // 16 x 2048 19.3 and 24.0); below, the prefix and the suffixes share a launch.
+  const long long scores = (long long)p.rows * nkv * prefix_len;
+  p.tc = kv_f16 && prefix_len >= 256 && scores >= 600000;
+  p.own = p.tc || (!kv_f16 && p.groups > 2 && scores >= 250000);
   if (p.tc) {
-    // one CTA an SM: the number of splits with the shortest rounds, at about 6 us
-    // a CTA and 1.3 us a block
+    // one CTA an SM, about 5.5 us and 1.63 us a block of 128 keys: the number of
+    // splits with the shortest rounds
     const int units = p.row_tiles * nkv;
     double best = 1e300;
     for (int n = (prefix_len + kTcMaxKeys - 1) / kTcMaxKeys; n <= std::max(1, prefix_len / 256); n++) {
       const int keys = round_up((prefix_len + n - 1) / n, 128), got = (prefix_len + keys - 1) / keys;
-      const double t = (double)(((long long)units * got + kSms - 1) / kSms) * (6.0 + 1.3 * (keys / 128)) + 0.05 * got;
+      const double t = (double)(((long long)units * got + kSms - 1) / kSms) * (5.5 + 1.63 * (keys / 128)) + 0.05 * got;
       if (t < best) best = t, p.pref_keys = keys;
-      if ((long long)units * n > 4 * kSms && n > (prefix_len + kTcMaxKeys - 1) / kTcMaxKeys) break;
+      if ((long long)units * n > 4 * kSms) break;
     }
   } else {
-  // about four CTAs an SM, never under 128 keys a split and never above 1024:
-  // the tensor core's f32 sums lose about 2^-25.5 a step, all one way, so a
-  // warp's 16 tiles stay below 2^-20 (256 tiles of a 16384-key split: 1e-5)
-  const long long units = (long long)p.groups * nkv;
-  const long long want = std::max(1LL, 4LL * kSms / units);
-  p.pref_keys = std::min(1024, std::max(128, round_up((int)((prefix_len + want - 1) / want), 64)));
+    // about four CTAs an SM (f32 in its own kernel: two), never under 128 keys a
+    // split and never above 1024: the tensor core's f32 sums lose about 2^-25.5
+    // a step, all one way, so a warp's 16 tiles stay below 2^-20 (256 tiles of a
+    // 16384-key split: 1e-5)
+    const long long units = (long long)(p.own ? (p.groups + 1) / 2 : p.groups) * nkv;
+    const long long want = std::max(1LL, (p.own ? 2LL : 4LL) * kSms / units);
+    p.pref_keys = std::min(1024, std::max(128, round_up((int)((prefix_len + want - 1) / want), 64)));
   }
   p.n_pref = (prefix_len + p.pref_keys - 1) / p.pref_keys;
-  // suffix: two rounds of CTAs (three an SM) or more, 128 keys a split at least
-  const int pairs = nseq * nkv * p.gch, want = std::max(1, 6 * kSms / pairs);
+  // suffix: about four CTAs an SM, 128 keys a split at least (64 sequences x up to
+  // 1024 keys 12.6 us in splits of 256, 14.9 of 128, 20.2 of 1024)
+  const int pairs = nseq * nkv * p.gch, want = std::max(1, 4 * kSms / pairs);
   p.suf_keys = std::max(128, round_up((max_len + want - 1) / want, 64));
   p.n_suf = (max_len + p.suf_keys - 1) / p.suf_keys;
   return p;
@@ -267,35 +277,37 @@ __device__ __forceinline__ void v_frag(const unsigned char* st, int dt, uint32_t
   }
 }
 
-// CTA = one split of the keys for up to 8 rows of one KV head.  Blocks
-// [0, prefix blocks) take the prefix, the others the suffixes.
-template <typename KVT>
-__global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_constant__ SharedArgs a) {
+// CTA = one split of the keys for up to 8 NG rows of one KV head.  Blocks
+// [0, pref) take the prefix, the others the suffixes (8 rows of a sequence
+// each).  NG = 2, for the prefix alone and an f32 cache, halves the reads and
+// the splitting of K and V per row.
+template <typename KVT, int NG>
+__global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_constant__ SharedArgs a, int pref) {
   using W = WarpTile<KVT>;
   constexpr bool F32 = std::is_same<KVT, float>::value;
   extern __shared__ __align__(128) unsigned char sm[];
-  __shared__ float sm_m[kWarps][8], sm_l[kWarps][8];
+  __shared__ float sm_m[kWarps][8 * NG], sm_l[kWarps][8 * NG];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const SharedPlan& p = a.p;
   const int G = p.G;
+  if (NG > 1) pdl_launch_dependents();
 
   // the CTA's rows [row0, row0 + nrow) of KV head kvh and its keys [k0, k1)
-  int kvh, row0, nrow, k0, k1, split;
+  int kvh, row0, nrow, k0, k1, split, kmax;
   const uint32_t* table;
   int blk = blockIdx.x;
-  const int pref_blocks = p.tc ? 0 : p.n_pref * p.groups * a.nkv;
-  if (blk < pref_blocks) {
-    const int rg = blk % p.groups;
-    blk /= p.groups;
+  if (blk < pref) {
+    const int ng = (p.groups + NG - 1) / NG, rg = blk % ng;
+    blk /= ng;
     kvh = blk % a.nkv;
     split = blk / a.nkv;
-    row0 = 8 * rg;
-    nrow = min(8, p.rows - row0);
+    row0 = 8 * NG * rg;
+    nrow = min(8 * NG, p.rows - row0);
     table = a.prefix_pages;
     k0 = split * p.pref_keys;
-    k1 = min(a.prefix_len, k0 + p.pref_keys);
+    k1 = kmax = min(a.prefix_len, k0 + p.pref_keys);
   } else {
-    blk -= pref_blocks;
+    blk -= pref;
     const int gc = blk % p.gch;
     blk /= p.gch;
     kvh = blk % a.nkv;
@@ -305,13 +317,18 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
     row0 = b * G + 8 * gc;
     nrow = min(8, G - 8 * gc);
     table = a.pages + (size_t)b * a.max_pages;
-    const int len = __ldg(a.lens + b);
-    if (len > a.max_len && a.err && threadIdx.x == 0) *a.err = 1;
     k0 = split * p.suf_keys;
-    k1 = min(min(len, a.max_len), k0 + p.suf_keys);
+    kmax = min(a.max_len, k0 + p.suf_keys);  // the table holds that many, whatever the length
+    k1 = a.lens[b];                          // on its way while the first page ids are read
     split += p.n_pref;
+  }
+  auto page_at = [&](int t) -> uint32_t { return k0 + t * kPage < kmax ? __ldg(table + k0 / kPage + t) : 0u; };
+  const uint32_t page0 = page_at(warp), page1 = page_at(warp + kWarps);
+  if ((int)blockIdx.x >= pref) {
+    if (k1 > a.max_len && a.err && threadIdx.x == 0) *a.err = 1;
+    k1 = min(k1, kmax);
     if (k0 >= k1) {
-      if (p.tc) pdl_wait();
+      if (p.own) pdl_wait();
       return;
     }
   }
@@ -319,7 +336,6 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
   unsigned char* st = sm + warp * W::kStages * W::kBytes;
   const int ntile = (k1 - k0 + kPage - 1) / kPage;
   // the warp's tiles: warp, warp + kWarps, ...
-  auto page_of = [&](int t) -> uint32_t { return t < ntile ? __ldg(table + k0 / kPage + t) : 0u; };
   auto issue = [&](int t, uint32_t page, int stage) -> int {
     int nv = t < ntile ? min(kPage, k1 - k0 - t * kPage) : 0;
     if (nv > 0 && page >= a.n_pages) {  // a page outside the pool: its keys are left out
@@ -330,14 +346,15 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
     cp_async_commit();
     return nv;
   };
-  int nv_cur = issue(warp, page_of(warp), 0);
-  uint32_t page_next = page_of(warp + kWarps);
+  int nv_cur = issue(warp, page0, 0);
+  uint32_t page_next = page1;
 
   // q of the rows as B fragments: lane (g, tq) holds row g's dims 2 tq.. of each k-step
-  uint32_t qh[8][2], ql[8][2];
-  {
-    const int r = row0 + g;
-    const bool on = g < nrow;
+  uint32_t qh[NG][8][2], ql[NG][8][2];
+#pragma unroll
+  for (int n = 0; n < NG; n++) {
+    const int r = row0 + 8 * n + g;
+    const bool on = 8 * n + g < nrow;
     const float* q = a.q + (on ? (long long)(r / G) * a.ldq + (kvh * G + r % G) * kHeadDim : 0) + 2 * tq;
     const float c = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
 #pragma unroll
@@ -345,68 +362,89 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         const float2 x = on ? __ldg(reinterpret_cast<const float2*>(q + 16 * ks + 8 * j)) : make_float2(0.f, 0.f);
-        split2(x.x * c, x.y * c, qh[ks][j], ql[ks][j]);
+        split2(x.x * c, x.y * c, qh[n][ks][j], ql[n][ks][j]);
       }
   }
-  float O[8][4];
+  float O[NG][8][4];
+  float m0[NG], m1[NG], l0[NG], l1[NG];  // rows 2 tq and 2 tq + 1
 #pragma unroll
-  for (int j = 0; j < 8; j++) O[j][0] = O[j][1] = O[j][2] = O[j][3] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows 2 tq and 2 tq + 1
+  for (int n = 0; n < NG; n++) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) O[n][j][0] = O[n][j][1] = O[n][j][2] = O[n][j][3] = 0.f;
+    m0[n] = m1[n] = -INFINITY;
+    l0[n] = l1[n] = 0.f;
+  }
 
   int stage = 0;
   for (int t = warp; t < ntile; t += kWarps) {
     const int nv_next = issue(t + kWarps, page_next, stage ^ 1);
-    page_next = page_of(t + 2 * kWarps);
+    page_next = page_at(t + 2 * kWarps);
     cp_async_wait<1>();
     __syncwarp();
     const unsigned char* ks_ = st + stage * W::kBytes;
     const unsigned char* vs_ = ks_ + kPage * W::kRow;
-    float S[4] = {0.f, 0.f, 0.f, 0.f}, S2[4] = {0.f, 0.f, 0.f, 0.f};
+    float S[NG][4], S2[NG][4];
     uint32_t fh[4], fl[4];
+#pragma unroll
+    for (int n = 0; n < NG; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) S[n][j] = S2[n][j] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) {
       k_frag(ks_, ks, fh, fl, KVT());
-      mma16816(S, fh, qh[ks][0], qh[ks][1]);
-      mma16816(S2, fh, ql[ks][0], ql[ks][1]);
-      if (F32) mma16816(S2, fl, qh[ks][0], qh[ks][1]);
-    }
-    // keys g (S[0], S[1]) and g + 8 (S[2], S[3]) for rows 2 tq, 2 tq + 1
-    const bool v0 = g < nv_cur, v1 = g + 8 < nv_cur;
-    const float s0 = v0 ? S[0] + S2[0] : -INFINITY, s1 = v0 ? S[1] + S2[1] : -INFINITY;
-    const float s2 = v1 ? S[2] + S2[2] : -INFINITY, s3 = v1 ? S[3] + S2[3] : -INFINITY;
-    float n0 = fmaxf(s0, s2), n1 = fmaxf(s1, s3);
 #pragma unroll
-    for (int o = 4; o <= 16; o <<= 1) {
-      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
-      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+      for (int n = 0; n < NG; n++) {
+        mma16816(S[n], fh, qh[n][ks][0], qh[n][ks][1]);
+        mma16816(S2[n], fh, ql[n][ks][0], ql[n][ks][1]);
+        if (F32) mma16816(S2[n], fl, qh[n][ks][0], qh[n][ks][1]);
+      }
     }
-    n0 = fmaxf(n0, m0);
-    n1 = fmaxf(n1, m1);
-    // no key so far (or every score -inf): a finite base keeps 2^(-inf - base) = 0
-    const float b0 = n0 == -INFINITY ? 0.f : n0 - kPBits, b1 = n1 == -INFINITY ? 0.f : n1 - kPBits;
-    const float c0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), c1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
-    m0 = n0;
-    m1 = n1;
-    const float p0 = exp2f(s0 - b0), p1 = exp2f(s1 - b1), p2 = exp2f(s2 - b0), p3 = exp2f(s3 - b1);
-    l0 = l0 * c0 + (p0 + p2);
-    l1 = l1 * c1 + (p1 + p3);
-    uint32_t ph0, pl0, ph1, pl1;
-    split2(p0, p1, ph0, pl0);
-    split2(p2, p3, ph1, pl1);
-    ph0 = movmatrix(ph0);
-    ph1 = movmatrix(ph1);
-    pl0 = movmatrix(pl0);
-    pl1 = movmatrix(pl1);
+    uint32_t ph[NG][2], pl[NG][2];
+    float c0[NG], c1[NG];
+    const bool v0 = g < nv_cur, v1 = g + 8 < nv_cur;
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+      // keys g (S[0], S[1]) and g + 8 (S[2], S[3]) for rows 2 tq, 2 tq + 1
+      const float s0 = v0 ? S[n][0] + S2[n][0] : -INFINITY, s1 = v0 ? S[n][1] + S2[n][1] : -INFINITY;
+      const float s2 = v1 ? S[n][2] + S2[n][2] : -INFINITY, s3 = v1 ? S[n][3] + S2[n][3] : -INFINITY;
+      float n0 = fmaxf(s0, s2), n1 = fmaxf(s1, s3);
+#pragma unroll
+      for (int o = 4; o <= 16; o <<= 1) {
+        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+      }
+      n0 = fmaxf(n0, m0[n]);
+      n1 = fmaxf(n1, m1[n]);
+      // no key so far (or every score -inf): a finite base keeps 2^(-inf - base) = 0
+      const float b0 = n0 == -INFINITY ? 0.f : n0 - kPBits, b1 = n1 == -INFINITY ? 0.f : n1 - kPBits;
+      c0[n] = m0[n] == -INFINITY ? 0.f : exp2f(m0[n] - n0);
+      c1[n] = m1[n] == -INFINITY ? 0.f : exp2f(m1[n] - n1);
+      m0[n] = n0;
+      m1[n] = n1;
+      const float p0 = exp2f(s0 - b0), p1 = exp2f(s1 - b1), p2 = exp2f(s2 - b0), p3 = exp2f(s3 - b1);
+      l0[n] = l0[n] * c0[n] + (p0 + p2);
+      l1[n] = l1[n] * c1[n] + (p1 + p3);
+      split2(p0, p1, ph[n][0], pl[n][0]);
+      split2(p2, p3, ph[n][1], pl[n][1]);
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        ph[n][j] = movmatrix(ph[n][j]);
+        pl[n][j] = movmatrix(pl[n][j]);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      O[j][0] *= c0;
-      O[j][1] *= c1;
-      O[j][2] *= c0;
-      O[j][3] *= c1;
       v_frag(vs_, j, fh, fl, KVT());
-      mma16816(O[j], fh, ph0, ph1);
-      mma16816(O[j], fh, pl0, pl1);
-      if (F32) mma16816(O[j], fl, ph0, ph1);
+#pragma unroll
+      for (int n = 0; n < NG; n++) {
+        O[n][j][0] *= c0[n];
+        O[n][j][1] *= c1[n];
+        O[n][j][2] *= c0[n];
+        O[n][j][3] *= c1[n];
+        mma16816(O[n][j], fh, ph[n][0], ph[n][1]);
+        mma16816(O[n][j], fh, pl[n][0], pl[n][1]);
+        if (F32) mma16816(O[n][j], fl, ph[n][0], ph[n][1]);
+      }
     }
     __syncwarp();
     nv_cur = nv_next;
@@ -414,29 +452,34 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
   }
   cp_async_wait<0>();
 #pragma unroll
-  for (int o = 4; o <= 16; o <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+  for (int n = 0; n < NG; n++) {
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) {
+      l0[n] += __shfl_xor_sync(0xffffffffu, l0[n], o);
+      l1[n] += __shfl_xor_sync(0xffffffffu, l1[n], o);
+    }
+    if (g == 0) {
+      sm_m[warp][8 * n + 2 * tq] = m0[n];
+      sm_m[warp][8 * n + 2 * tq + 1] = m1[n];
+      sm_l[warp][8 * n + 2 * tq] = l0[n];
+      sm_l[warp][8 * n + 2 * tq + 1] = l1[n];
+    }
   }
-  if (g == 0) {
-    sm_m[warp][2 * tq] = m0;
-    sm_m[warp][2 * tq + 1] = m1;
-    sm_l[warp][2 * tq] = l0;
-    sm_l[warp][2 * tq + 1] = l1;
-  }
-  __syncthreads();  // every warp's tiles are consumed: the staging becomes [warp][8][kSoPitch] f32
+  __syncthreads();  // every warp's tiles are consumed: the staging becomes [warp][8 NG][kSoPitch] f32
   float* so = reinterpret_cast<float*>(sm);
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    float* d = so + (warp * 8 + 2 * tq) * kSoPitch + 16 * j + g;
-    d[0] = O[j][0];
-    d[kSoPitch] = O[j][1];
-    d[8] = O[j][2];
-    d[kSoPitch + 8] = O[j][3];
-  }
+  for (int n = 0; n < NG; n++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float* d = so + (warp * 8 * NG + 8 * n + 2 * tq) * kSoPitch + 16 * j + g;
+      d[0] = O[n][j][0];
+      d[kSoPitch] = O[n][j][1];
+      d[8] = O[n][j][2];
+      d[kSoPitch + 8] = O[n][j][3];
+    }
   __syncthreads();
-  for (int i = threadIdx.x; i < 8 * 32; i += 32 * kWarps) {
-    const int r = i & 7, c = i >> 3;
+  for (int i = threadIdx.x; i < 8 * NG * 32; i += 32 * kWarps) {
+    const int r = (i & 7) + (i >> 8) * 8, c = (i >> 3) & 31;
     if (r >= nrow) continue;
     float mm = sm_m[0][r];
 #pragma unroll
@@ -446,7 +489,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
 #pragma unroll
     for (int w = 0; w < kWarps; w++) {
       const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2f(sm_m[w][r] - mm);
-      const float4 x = reinterpret_cast<const float4*>(so + (w * 8 + r) * kSoPitch)[c];
+      const float4 x = reinterpret_cast<const float4*>(so + (w * 8 * NG + r) * kSoPitch)[c];
       l += f * sm_l[w][r];
       o.x += f * x.x;
       o.y += f * x.y;
@@ -460,9 +503,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
     }
     a.po[part_at(at, c)] = o;
   }
-  // launched beside the prefix kernel, whose results it does not need: its end
-  // waits for that kernel's, so that the combine, which follows it, finds both
-  if (p.tc) pdl_wait();
+  // the suffixes, launched beside the prefix's own kernel, whose results they do
+  // not need: their end waits for that kernel's, so that the combine, which
+  // follows them, finds both
+  if (NG == 1 && p.own) pdl_wait();
 }
 
 // ======================================================================
@@ -693,32 +737,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------ softmax, one thread a row
-    const int w = warp >> 2, r = tid & 127, G = p.G;
+    const int w = warp >> 2, r = tid & 127;
     {
-      // q times log2(e) / sqrt(128) as f16 hi and lo: 8 rows x 4 float4 a load (full sectors, 8 lines)
+      // q times log2(e) / sqrt(128) as f16 hi and lo: 8 rows x 4 float4 a load (full sectors)
       const float c = 1.4426950408889634f * 0.08838834764831845f;
-      float4 x[16];
+      float4 qx[16];
 #pragma unroll
       for (int g = 0; g < 2; g++) {
-        const int rr = 16 * warp + 8 * g + (lane & 7), gr = tile * 128 + rr;
-        const float* q = a.q + (gr < p.rows ? (long long)(gr / G) * a.ldq + (kvh * G + gr % G) * kHeadDim : 0);
+        const int gr = tile * 128 + 16 * warp + 8 * g + (lane & 7);
+        const float* q = a.q + (gr < p.rows ? (long long)(gr / p.G) * a.ldq + (kvh * p.G + gr % p.G) * kHeadDim : 0);
 #pragma unroll
         for (int i = 0; i < 8; i++)
-          x[8 * g + i] = gr < p.rows ? __ldg(reinterpret_cast<const float4*>(q) + 4 * i + (lane >> 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          qx[8 * g + i] = gr < p.rows ? __ldg(reinterpret_cast<const float4*>(q) + 4 * i + (lane >> 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int g = 0; g < 2; g++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int rr = 16 * warp + 8 * g + (lane & 7), f = 4 * i + (lane >> 3);  // the row's f-th float4: half a chunk
-          const float4 v = x[8 * g + i];
-          uint2 h, l;
-          split2(v.x * c, v.y * c, h.x, l.x);
-          split2(v.z * c, v.w * c, h.y, l.y);
-          const uint32_t at = core_off(rr, f >> 1) + (f & 1) * 8;
-          *reinterpret_cast<uint2*>(qs + at) = h;
-          *reinterpret_cast<uint2*>(qs + kTcTile + at) = l;
-        }
+      for (int i = 0; i < 16; i++) {
+        const int rr = 16 * warp + (i & 8) + (lane & 7), f = 4 * (i & 7) + (lane >> 3);  // half a 16-byte chunk
+        const float4 v = qx[i];
+        uint2 h, l;
+        split2(v.x * c, v.y * c, h.x, l.x);
+        split2(v.z * c, v.w * c, h.y, l.y);
+        const uint32_t at = core_off(rr, f >> 1) + (f & 1) * 8;
+        *reinterpret_cast<uint2*>(qs + at) = h;
+        *reinterpret_cast<uint2*>(qs + kTcTile + at) = l;
+      }
       fence_async_smem();
       mbar_arrive(&S.q_full);
     }
@@ -861,12 +903,12 @@ __global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant
   __shared__ float sb[32][8], sl[32][8];
   const int kvh = blockIdx.x / a.p.groups, row0 = blockIdx.x % a.p.groups * 8;
   const int rr = threadIdx.x & 7, c = threadIdx.x >> 3, r = row0 + rr, G = a.p.G;
-  pdl_wait();
   const int b = r / G, len = r < a.p.rows ? __ldg(a.lens + b) : -1;
   const bool on = len >= 0;  // a padding sequence's row stays as it is
   const int ns = on ? a.p.n_pref + (min(len, a.max_len) + a.p.suf_keys - 1) / a.p.suf_keys : 0;
   const size_t row = part_row(a, 0, kvh, r), step = (size_t)a.nkv * a.p.groups * 8;  // rows of a split
   const float4* po = a.po + part_at(row, c);
+  pdl_wait();
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; __syncthreads_or(s0 < ns); s0 += 32) {
@@ -961,27 +1003,33 @@ cudaError_t page_map(CUtensorMap* map, const void* pool, const SharedArgs& a) {
              : cudaErrorInvalidValue;
 }
 
-cudaError_t launch_shared(const SharedArgs& a, int kv_f16, long long blocks, cudaStream_t st) {
+template <typename KVT, int NG>
+cudaError_t launch_warps(const SharedArgs& a, long long blocks, int pref, bool early, cudaStream_t st) {
+  void* args[2] = {const_cast<SharedArgs*>(&a), &pref};
+  return launch_pdl((const void*)attn_shared_kernel<KVT, NG>, (unsigned)blocks, 32 * kWarps,
+                    kWarps * WarpTile<KVT>::kStages * WarpTile<KVT>::kBytes, early, args, st);
+}
+
+template <typename KVT>
+cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
-  void* args[3] = {const_cast<SharedArgs*>(&a), nullptr, nullptr};
+  const int pref = a.p.n_pref * a.nkv * (a.p.own ? (a.p.groups + 1) / 2 : a.p.groups);
   if (a.p.tc) {
     CUtensorMap km, vm;
     e = page_map(&km, a.kc, a);
     if (e == cudaSuccess) e = page_map(&vm, a.vc, a);
-    args[1] = &km;
-    args[2] = &vm;
+    void* args[3] = {const_cast<SharedArgs*>(&a), &km, &vm};
     if (e == cudaSuccess)
       e = launch_pdl((const void*)attn_prefix_tc_kernel, (unsigned)(a.p.n_pref * a.nkv * a.p.row_tiles), kTcThreads,
                      kTcSmem, false, args, st);
+  } else if constexpr (std::is_same<KVT, float>::value) {
+    if (a.p.own) e = launch_warps<KVT, 2>(a, pref, pref, false, st);
   }
-  if (e == cudaSuccess && blocks > 0)
-    e = kv_f16 ? launch_pdl((const void*)attn_shared_kernel<__half>, (unsigned)blocks, 32 * kWarps,
-                            kWarps * WarpTile<__half>::kStages * WarpTile<__half>::kBytes, a.p.tc, args, st)
-               : launch_pdl((const void*)attn_shared_kernel<float>, (unsigned)blocks, 32 * kWarps,
-                            kWarps * WarpTile<float>::kStages * WarpTile<float>::kBytes, a.p.tc, args, st);
+  const long long blocks = (a.p.own ? 0 : pref) + (long long)a.p.n_suf * a.nseq * a.nkv * a.p.gch;
+  if (e == cudaSuccess && blocks > 0) e = launch_warps<KVT, 1>(a, blocks, a.p.own ? 0 : pref, a.p.own, st);
+  void* args[1] = {const_cast<SharedArgs*>(&a)};
   if (e == cudaSuccess)
-    e = launch_pdl((const void*)attn_shared_combine, (unsigned)(a.nkv * a.p.groups), 256, 0, blocks > 0 || a.p.tc,
-                   args, st);
+    e = launch_pdl((const void*)attn_shared_combine, (unsigned)(a.nkv * a.p.groups), 256, 0, blocks > 0 || a.p.own, args, st);
   return e;
 }
 
@@ -1090,11 +1138,10 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
   a.pm = reinterpret_cast<float*>(a.po + rows * (kHeadDim / 4));
   a.pl = a.pm + rows;
   a.err = err;
-  const long long blocks = (a.p.tc ? 0 : (long long)a.p.n_pref * a.p.groups * nkv) +
-                           (long long)a.p.n_suf * nseq * nkv * a.p.gch;
-  if (blocks > 0x7fffffffLL) return fail(EG_ERR_ARG, "attn_shared_prefix: too many splits");
+  if (((long long)a.p.n_pref * a.p.groups + (long long)a.p.n_suf * nseq * a.p.gch) * nkv > 0x7fffffffLL)
+    return fail(EG_ERR_ARG, "attn_shared_prefix: too many splits");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const cudaError_t e = launch_shared(a, kv_f16, blocks, st);
+  const cudaError_t e = kv_f16 ? launch_shared<__half>(a, st) : launch_shared<float>(a, st);
   if (e != cudaSuccess) return fail(EG_ERR_CUDA, "attn_shared_prefix: %s", cudaGetErrorString(e));
   return EG_OK;
 }
