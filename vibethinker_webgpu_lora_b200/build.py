@@ -4,7 +4,8 @@ nvcc compiles the CUDA sources for `-gencode arch=compute_100a,code=sm_100a`
 (cross-compiles without a GPU); g++ compiles the host quantiser/generator
 with -ffp-contract=off so its arithmetic matches the reference's JS doubles
 operation by operation.  Objects go to _build/ beside this file, the shared
-library next to the package so it ships with the source tree.
+library next to the package so it ships with the source tree, and beside it the
+Python binding of the ops on torch tensors (_ops, against the installed torch).
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libemberglass_cuda.so")
+OPS = os.path.join(HERE, "_ops.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -66,7 +68,26 @@ def build(verbose: bool = False, extra_nvflags: list[str] | None = None) -> str:
     if _stale(LIB, objs):
         _run([NVCC, *ARCH, "-shared", "-ccbin", CXX, "-o", LIB, *objs, "-Xcompiler", "-fopenmp",
               "-lgomp", "-Xlinker", "--no-undefined"], verbose)
+    build_ops(verbose)
     return LIB
+
+
+def build_ops(verbose: bool = False) -> str:
+    """_ops.so: csrc/eg_torch.cpp against torch's headers and libraries and the
+    library above (found beside it at run time)."""
+    src = os.path.join(CSRC, "eg_torch.cpp")
+    if _stale(OPS, [src, __file__, os.path.join(INCLUDE, "emberglass.h")]):
+        import sysconfig
+
+        import torch
+        from torch.utils.cpp_extension import include_paths, library_paths
+        inc = [f for p in include_paths() + ["/usr/local/cuda/include"] for f in ("-isystem", p)]
+        libs = [f for p in library_paths() for f in ("-L", p, f"-Wl,-rpath,{p}")]
+        _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+              "-I", INCLUDE, *inc, "-isystem", sysconfig.get_paths()["include"], src, "-o", OPS, "-L", HERE,
+              "-l:" + os.path.basename(LIB), *libs, "-lc10",
+              "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], verbose)
+    return OPS
 
 
 if __name__ == "__main__":

@@ -7,7 +7,6 @@
 // lengths live on the device, so a captured graph serves every step.
 #include <cuda.h>
 #include <math.h>
-#include <string.h>
 #include <algorithm>
 #include <type_traits>
 
@@ -120,7 +119,7 @@ constexpr float kPBits = 14.f;
 constexpr int kWarps = 4;       // warps of a CTA, each with its own 16-key tiles
 constexpr int kSoPitch = kHeadDim + 4;  // floats a row of the warps' outputs in shared memory
 constexpr int kSms = 148;       // plans are made for the B200's SM count
-constexpr int kTcMaxKeys = 2048;  // keys of a prefix split on the tensor cores
+constexpr int kTcMaxKeys = 1536;  // keys of a prefix split on the tensor cores
 
 struct SharedPlan {
   int G, gch;          // query heads per KV head; chunks of 8 of them
@@ -168,12 +167,12 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   p.groups = (p.rows + 7) / 8;
   p.row_tiles = (p.rows + 127) / 128;
   // What the prefix's scores number decides its kernel (16 heads, 2 KV heads):
-  // f16 on the tensor cores from 600,000 on (16 sequences x 2048 14.6 us there,
-  // 13.9 by warps; 16 x 4096 15.4 and 18.1; 64 x 1024 14.4 and 17.3); f32 in
+  // f16 on the tensor cores from 900,000 on (16 sequences x 2048 14.6 us there,
+  // 11.2 by warps; 16 x 4096 15.4 and 18.1; 64 x 1024 14.4 and 17.3); f32 in
   // CTAs of 16 rows from 250,000 on (16 x 512 11.4 us there, 10.6 in CTAs of 8;
   // 16 x 2048 19.3 and 24.0); below, the prefix and the suffixes share a launch.
   const long long scores = (long long)p.rows * nkv * prefix_len;
-  p.tc = kv_f16 && prefix_len >= 256 && scores >= 600000;
+  p.tc = kv_f16 && prefix_len >= 256 && scores >= 900000;
   p.own = p.tc || (!kv_f16 && p.groups > 2 && scores >= 250000);
   if (p.tc) {
     // one CTA an SM, about 5.5 us and 1.63 us a block of 128 keys: the number of
@@ -187,12 +186,13 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
       if ((long long)units * n > 4 * kSms) break;
     }
   } else {
-    // about four CTAs an SM (f32 in its own kernel: two), never under 128 keys a
-    // split and never above 1024: the tensor core's f32 sums lose about 2^-25.5
-    // a step, all one way, so a warp's 16 tiles stay below 2^-20 (256 tiles of a
-    // 16384-key split: 1e-5)
+    // two CTAs an SM (f32: one, 128 KB each): what is resident at once beside the
+    // suffixes (16 x 2048 f16 11.2 us so, 13.9 with four an SM); never under 128
+    // keys a split and never above 1024: the tensor core's f32 sums lose about
+    // 2^-24.5 a step, all one way, so a warp's 16 tiles stay below 2^-20 (256
+    // tiles of a 16384-key split: 1e-5)
     const long long units = (long long)(p.own ? (p.groups + 1) / 2 : p.groups) * nkv;
-    const long long want = std::max(1LL, (p.own ? 2LL : 4LL) * kSms / units);
+    const long long want = std::max(1LL, (kv_f16 ? 2LL : 1LL) * kSms / units);
     p.pref_keys = std::min(1024, std::max(128, round_up((int)((prefix_len + want - 1) / want), 64)));
   }
   p.n_pref = (prefix_len + p.pref_keys - 1) / p.pref_keys;
@@ -520,8 +520,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
 // turn, so one's softmax runs under the other's products.  O stays in TMEM: a
 // row's base b moves (and its O is scaled) only when the maximum passes b by
 // kTcBits + kTcSlack bits, which after the first block is rare.  The tensor
-// core's sums lose about 2^-25.5 a step, all one way: a split's 2048 keys are
-// 128 steps a warpgroup, 2.5e-6 at most.
+// core's sums lose about 2^-24.5 a step, all one way: a split of 1536 keys is
+// 96 steps a warpgroup, 2e-6 of the output on average.
 // Warps: 0-3 and 4-7 softmax, 8 copies K, 9 copies V (TMA: a page of one KV
 // head is two boxes of 16 rows x 64 dims, 128-byte swizzle), 10 issues MMAs and
 // owns TMEM.
@@ -960,12 +960,15 @@ __global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant
 
 // The launches of one call: the prefix kernel (tcgen05), the suffix kernel
 // beside it, the combine after both.
-cudaError_t launch_pdl(const void* fn, unsigned blocks, int threads, int smem, bool early, void** args,
+cudaError_t launch_pdl(const void* fn, OncePerDevice& once, unsigned blocks, int threads, int smem, bool early, void** args,
                        cudaStream_t st) {
-  if (smem > 48 << 10) {
-    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
+  int dev = 0;
+  cudaError_t e = smem > 48 << 10 ? cudaGetDevice(&dev) : cudaSuccess;
+  if (e == cudaSuccess && smem > 48 << 10 && once.first(dev)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) once.done(dev);
   }
+  if (e != cudaSuccess) return e;
   cudaLaunchAttribute at = {};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
@@ -1005,13 +1008,15 @@ cudaError_t page_map(CUtensorMap* map, const void* pool, const SharedArgs& a) {
 
 template <typename KVT, int NG>
 cudaError_t launch_warps(const SharedArgs& a, long long blocks, int pref, bool early, cudaStream_t st) {
+  static OncePerDevice once;
   void* args[2] = {const_cast<SharedArgs*>(&a), &pref};
-  return launch_pdl((const void*)attn_shared_kernel<KVT, NG>, (unsigned)blocks, 32 * kWarps,
+  return launch_pdl((const void*)attn_shared_kernel<KVT, NG>, once, (unsigned)blocks, 32 * kWarps,
                     kWarps * WarpTile<KVT>::kStages * WarpTile<KVT>::kBytes, early, args, st);
 }
 
 template <typename KVT>
 cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
+  static OncePerDevice tc_once, no_smem;
   cudaError_t e = cudaSuccess;
   const int pref = a.p.n_pref * a.nkv * (a.p.own ? (a.p.groups + 1) / 2 : a.p.groups);
   if (a.p.tc) {
@@ -1020,7 +1025,7 @@ cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
     if (e == cudaSuccess) e = page_map(&vm, a.vc, a);
     void* args[3] = {const_cast<SharedArgs*>(&a), &km, &vm};
     if (e == cudaSuccess)
-      e = launch_pdl((const void*)attn_prefix_tc_kernel, (unsigned)(a.p.n_pref * a.nkv * a.p.row_tiles), kTcThreads,
+      e = launch_pdl((const void*)attn_prefix_tc_kernel, tc_once, (unsigned)(a.p.n_pref * a.nkv * a.p.row_tiles), kTcThreads,
                      kTcSmem, false, args, st);
   } else if constexpr (std::is_same<KVT, float>::value) {
     if (a.p.own) e = launch_warps<KVT, 2>(a, pref, pref, false, st);
@@ -1029,7 +1034,7 @@ cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
   if (e == cudaSuccess && blocks > 0) e = launch_warps<KVT, 1>(a, blocks, a.p.own ? 0 : pref, a.p.own, st);
   void* args[1] = {const_cast<SharedArgs*>(&a)};
   if (e == cudaSuccess)
-    e = launch_pdl((const void*)attn_shared_combine, (unsigned)(a.nkv * a.p.groups), 256, 0, blocks > 0 || a.p.own, args, st);
+    e = launch_pdl((const void*)attn_shared_combine, no_smem, (unsigned)(a.nkv * a.p.groups), 256, 0, blocks > 0 || a.p.own, args, st);
   return e;
 }
 
@@ -1144,26 +1149,6 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
   const cudaError_t e = kv_f16 ? launch_shared<__half>(a, st) : launch_shared<float>(a, st);
   if (e != cudaSuccess) return fail(EG_ERR_CUDA, "attn_shared_prefix: %s", cudaGetErrorString(e));
   return EG_OK;
-}
-
-// The same calls with their arguments as a block of 64-bit values, in order
-// (the Python wrappers').
-EG_API eg_status eg_packed_kv_append_paged(const char* block) {
-  int64_t a[22];
-  memcpy(a, block, sizeof a);
-  return eg_op_kv_append_paged((const float*)a[0], a[1], (int)a[2], (const int*)a[3], (const int*)a[4],
-                               (const uint32_t*)a[5], (int)a[6], (int)a[7], (int)a[8], (int)a[9], (void*)a[10],
-                               (void*)a[11], (const float*)a[12], (const float*)a[13], (int)a[14], (int)a[15],
-                               (int)a[16], (int)a[17], (float*)a[18], a[19], (int*)a[20], (void*)a[21]);
-}
-
-EG_API eg_status eg_packed_attn_shared_prefix(const char* block) {
-  int64_t a[21];
-  memcpy(a, block, sizeof a);
-  return eg_op_attn_shared_prefix((const float*)a[0], a[1], (int)a[2], (const void*)a[3], (const void*)a[4],
-                                  (int)a[5], (const uint32_t*)a[6], (int)a[7], (const uint32_t*)a[8], (int)a[9],
-                                  (const int*)a[10], (int)a[11], (int)a[12], (int)a[13], (int)a[14], (float*)a[15],
-                                  a[16], (void*)a[17], (uint64_t)a[18], (int*)a[19], (void*)a[20]);
 }
 
 }  // extern "C"

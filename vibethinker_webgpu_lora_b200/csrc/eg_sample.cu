@@ -13,7 +13,6 @@
 // changes a result.
 #include <cooperative_groups.h>
 #include <math.h>
-#include <string.h>
 #include <algorithm>
 
 #include "eg_common.cuh"
@@ -950,7 +949,13 @@ cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
   const int per = ((a.n + c - 1) / c + 3) & ~3, staged = per <= kSlice;
   const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 + kStagedHits * 4 : kHits * 4, kList * 12);
   static_assert(sizeof(FastSmem) + kSlice * 4 + kStagedHits * 4 <= 113 << 10, "two CTAs an SM");
-  const cudaError_t e = cudaFuncSetAttribute(sample_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 << 10);
+  static OncePerDevice once;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && once.first(dev)) {
+    e = cudaFuncSetAttribute(sample_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 << 10);
+    if (e == cudaSuccess) once.done(dev);
+  }
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at = {};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -993,16 +998,6 @@ EG_API eg_status eg_op_sample_filtered(const float* logits, int64_t ld, int rows
   const cudaError_t e = launch_sample(a, reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(EG_ERR_CUDA, "sample_filtered: %s", cudaGetErrorString(e));
   return EG_OK;
-}
-
-// The same call with its arguments as a block of 64-bit values, in order (the
-// Python wrapper's).
-EG_API eg_status eg_packed_sample_filtered(const char* block) {
-  int64_t a[12];
-  memcpy(a, block, sizeof a);
-  return eg_op_sample_filtered((const float*)a[0], a[1], (int)a[2], (int)a[3], (const float*)a[4], (const int*)a[5],
-                               (const float*)a[6], (const float*)a[7], (const float*)a[8], (uint32_t*)a[9],
-                               (float*)a[10], (void*)a[11]);
 }
 
 }  // extern "C"
