@@ -47,7 +47,7 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 
 struct RowParams {
-  double t, p, minp, r;
+  double t, p, minp, cut, r;  // cut: how far below the maximum min_p reaches, in x / t
   int k;  // 0: off
 };
 __device__ __forceinline__ RowParams row_params(const SampleArgs& a, int row) {
@@ -57,6 +57,7 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs& a, int row) {
   q.t = t > 0.f ? (double)t : 1.0;        // NaN too
   q.p = p < 1.f ? fmax((double)p, 0.0) : 1.0;
   q.minp = m > 0.f ? (double)m : 0.0;
+  q.cut = m > 0.f ? -log((double)m) : INFINITY;
   q.r = r > 0.f ? fmin((double)r, 1.0) : 0.0;
   q.k = a.top_k ? max(__ldg(a.top_k + row), 0) : 0;
   return q;
@@ -274,6 +275,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kBins = 2048;        // the last one: past the range
 constexpr int kList = 1024;        // gathered tokens
+constexpr int kCountMost = 256;    // of them put in order by counting
 constexpr int kSlice = 19200;      // most tokens that a CTA stages (75 KB: two CTAs an SM)
 constexpr int kHits = 8192, kStagedHits = 1024;  // ids that a pass may pick before they are checked
 constexpr int kQBits = 26;
@@ -439,7 +441,7 @@ __device__ __forceinline__ void bitonic_falling(unsigned long long* list, int np
 // for the 64-bit form.
 template <int kThreads>
 __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl, const Bins& B, const RowParams& P, int C,
-                                              bool wide, double e4) {
+                                              bool wide, double e4, double cut_pos) {
   constexpr int kPer = kBins / kThreads;  // consecutive bins of a thread: 2 or 4
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned long long q[kPer];
@@ -547,10 +549,9 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
     hi = fmin(hi, mass_above(p_hi + 1));
   }
   if (P.minp > 0.0) {
-    const double pos = -log(P.minp) / B.step;
-    if (pos < kBins - 2) {
-      m_lo = max(0, (int)rint(pos - 0.01));
-      m_hi = max(0, min(kBins - 2, (int)rint(pos + 0.01)));
+    if (cut_pos < kBins - 2) {
+      m_lo = max(0, (int)rint(cut_pos - 0.01));
+      m_hi = max(0, min(kBins - 2, (int)rint(cut_pos + 0.01)));
       lo = fmin(lo, mass_above(m_lo));
       hi = fmin(hi, mass_above(m_hi + 1));
     }
@@ -597,6 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     const int len = e1 - e0, quads = (reinterpret_cast<uintptr_t>(x) & 15) == 0 ? len / 4 : 0;
     for (int i = tid; i < quads; i += kThreads) cp_async16g(xs + 4 * i, x + e0 + 4 * i);
     for (int i = 4 * quads + tid; i < len; i += kThreads) cp_async4(xs + i, x + e0 + i);
+    if (tid < (-len & 3)) xs[len + tid] = -INFINITY;
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   for (int i = tid; i < kBins; i += kThreads) S.hist[i] = 0;
@@ -605,55 +607,51 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
   }
-  // f(value, id) over the slice, the whole warp at a time (-inf past its end)
+  // f(four values, id of the first) over the slice, the whole warp at a time (-inf past its end)
   const bool vec = !staged && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   auto each = [&](auto f) {
+    const float4 none4 = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     if (staged) {
-#pragma unroll 4
-      for (int i0 = e0; i0 < e1; i0 += kThreads) {
-        const int i = i0 + tid;
-        f(i < e1 ? xs[i - e0] : -INFINITY, i);
+#pragma unroll 2
+      for (int i0 = e0; i0 < e1; i0 += 4 * kThreads) {
+        const int i = i0 + 4 * tid;
+        f(i < e1 ? *reinterpret_cast<const float4*>(xs + (i - e0)) : none4, i);
       }
     } else if (vec) {
       // eight tokens a thread, the next eight already on their way
-      auto load = [&](int i) {
-        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (i + 3 < e1) {
-          v = __ldg(reinterpret_cast<const float4*>(x + i));
-        } else if (i < e1) {
-          v.x = __ldg(x + i);
-          if (i + 1 < e1) v.y = __ldg(x + i + 1);
-          if (i + 2 < e1) v.z = __ldg(x + i + 2);
-        }
-        return v;
-      };
-      auto give = [&](float4 v, int i) {
-        f(v.x, i);
-        f(v.y, i + 1);
-        f(v.z, i + 2);
-        f(v.w, i + 3);
-      };
-      int i = e0 + 4 * tid;
+      const int last = (e1 - e0) & ~3;  // up to here four at a time lie in the row
+      const float4* x4 = reinterpret_cast<const float4*>(x + e0);
+      auto load = [&](int i) { return i < last ? __ldg(x4 + i / 4) : none4; };
+      int i = 4 * tid;
       float4 v0 = load(i), v1 = load(i + 4 * kThreads);
-      for (int i0 = e0; i0 < e1; i0 += 8 * kThreads, i += 8 * kThreads) {
+      for (int i0 = 0; i0 < last; i0 += 8 * kThreads, i += 8 * kThreads) {
         const float4 n0 = load(i + 8 * kThreads), n1 = load(i + 12 * kThreads);
-        give(v0, i);
-        give(v1, i + 4 * kThreads);
+        f(v0, e0 + i);
+        f(v1, e0 + i + 4 * kThreads);
         v0 = n0;
         v1 = n1;
+      }
+      if (e0 + last < e1 && warp == 0) {  // and the one to three beyond
+        const int k = e0 + last + lane;
+        f(make_float4(k < e1 ? __ldg(x + k) : -INFINITY, -INFINITY, -INFINITY, -INFINITY), k);
       }
     } else {
 #pragma unroll 4
       for (int i0 = e0; i0 < e1; i0 += kThreads) {
         const int i = i0 + tid;
-        f(i < e1 ? __ldg(x + i) : -INFINITY, i);
+        f(make_float4(i < e1 ? __ldg(x + i) : -INFINITY, -INFINITY, -INFINITY, -INFINITY), i);
       }
     }
   };
   // ---- the slice's largest and smallest candidate
   float mx = -INFINITY, mn = INFINITY;
-  each([&](float v, int) {
-    if (v >= -1e30f) mx = fmaxf(mx, v), mn = fminf(mn, v);
+  each([&](float4 v, int) {
+    const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      mx = fmaxf(mx, w[j] >= -1e30f ? w[j] : -INFINITY);
+      mn = fminf(mn, w[j] >= -1e30f ? w[j] : INFINITY);
+    }
   });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -699,17 +697,22 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   if (!none && !slow0) {
     if (tid < 4) S.unit[tid] = exp(-(double)tid * B.step) * (1.0 / (1 << kQBits));
     if (!wide)
-      each([&](float v, int) {
-        const float p = bin_place(B, v), pr = p + kRound;
-        if (in_range(p)) {
-          const int b = __float_as_int(pr) - __float_as_int(kRound);
-          atomicAdd(&S.sum[b], (uint32_t)((1 << 22) - q_short(bin_rest(B, v, pr - kRound))));
-          atomicAdd(&S.cnt[b], 1u);
+      each([&](float4 v, int) {
+        const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float p = bin_place(B, w[j]), pr = p + kRound;
+          if (in_range(p)) {
+            const int b = __float_as_int(pr) - __float_as_int(kRound);
+            atomicAdd(&S.sum[b], (uint32_t)((1 << 22) - q_short(bin_rest(B, w[j], pr - kRound))));
+            atomicAdd(&S.cnt[b], 1u);
+          }
         }
       });
   }
   // bin_unit's factor for the leader's bins, while other CTAs count
   const double e4 = rank == 0 && !none && !slow0 ? exp(-(double)((tid * (kBins / kThreads)) & ~3) * B.step) : 0.0;
+  const double cut_pos = rank == 0 && !none && !slow0 ? P.cut / B.step : 0.0;
   cl.sync();
   if (none || slow0) {  // the same in every CTA of the cluster
     if (rank == 0) {
@@ -726,16 +729,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   }
   for (;;) {
     if (wide) {
-      each([&](float v, int) {
-        if (in_range(bin_place(B, v))) {
-          uint32_t q;
-          const int b = bin_of(B, v, q);
-          atomicAdd(&S.hist[b], kCountOne + q);
-        }
+      each([&](float4 v, int) {
+        const float w[4] = {v.x, v.y, v.z, v.w};
+        for (int j = 0; j < 4; j++)
+          if (in_range(bin_place(B, w[j]))) {
+            uint32_t q;
+            const int b = bin_of(B, w[j], q);
+            atomicAdd(&S.hist[b], kCountOne + q);
+          }
       });
       cl.sync();
     }
-    if (rank == 0) leader_ranges<kThreads>(S, cl, B, P, C, wide, e4);
+    if (rank == 0) leader_ranges<kThreads>(S, cl, B, P, C, wide, e4, cut_pos);
     cl.sync();
     if (!L->rg.redo) break;
     wide = true;  // a bin holds too many tokens for the 32-bit sums: once more
@@ -756,14 +761,21 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     uint32_t* hits = reinterpret_cast<uint32_t*>(dsm + sizeof(FastSmem) + (staged ? per * 4 : 0)) + warp * room;
     const uint32_t below = (1u << lane) - 1;
     uint32_t nh = 0;
-    each([&](float v, int i) {
+    auto inside = [&](float v) {
       bool hit = ((v >= from0) & (v <= to0)) | ((v >= from1) & (v <= to1));
       if (more) hit |= ((v >= from2) & (v <= to2)) | ((v >= from3) & (v <= to3));
-      const uint32_t vote = __ballot_sync(0xffffffffu, hit);
-      if (vote) {
-        const uint32_t to = nh + __popc(vote & below);
-        if (hit && to < room) hits[to] = (uint32_t)i;
-        nh += __popc(vote);
+      return hit;
+    };
+    each([&](float4 v, int i) {
+      const bool hit[4] = {inside(v.x), inside(v.y), inside(v.z), inside(v.w)};
+      if (__any_sync(0xffffffffu, hit[0] | hit[1] | hit[2] | hit[3])) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint32_t vote = __ballot_sync(0xffffffffu, hit[j]);
+          const uint32_t to = nh + __popc(vote & below);
+          if (hit[j] && to < room) hits[to] = (uint32_t)(i + j);
+          nh += __popc(vote);
+        }
       }
     });
     __syncwarp();
@@ -810,11 +822,28 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   }
   // ---- the gathered tokens in order (a bitonic sort, falling), then the place
   // and running mass of each: sums from the first token of its bin on
-  int np = 64;
-  while (np < nl) np *= 2;
-  for (int i = nl + tid; i < np; i += kThreads) S.list[i] = 0;
-  __syncthreads();
-  bitonic_falling<kThreads>(S.list, np);
+  unsigned long long* list = S.list;
+  if (nl <= kCountMost) {
+    // a few: each is compared with all, eight threads a token
+    list = reinterpret_cast<unsigned long long*>(xs) + kList * 3 / 2;  // behind the two arrays below
+    constexpr int kPart = 8;
+    const int part = tid & (kPart - 1);
+    for (int e = tid / kPart; e < (nl + 31) / 32 * 32; e += kThreads / kPart) {
+      const unsigned long long me = e < nl ? S.list[e] : 0;
+      int place = 0;
+      for (int f = part; f < nl; f += kPart) place += S.list[f] > me;
+#pragma unroll
+      for (int o = 1; o < kPart; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+      if (part == 0 && e < nl) list[place] = me;
+    }
+    __syncthreads();
+  } else {
+    int np = 64;
+    while (np < nl) np *= 2;
+    for (int i = nl + tid; i < np; i += kThreads) S.list[i] = 0;
+    __syncthreads();
+    bitonic_falling<kThreads>(S.list, np);
+  }
   constexpr int kMine = kList / kThreads;  // consecutive tokens of a thread
   unsigned long long* before = reinterpret_cast<unsigned long long*>(xs);  // sum of q before each; the slice is done with
   int* bins = reinterpret_cast<int*>(before + kList);
@@ -824,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   for (int j = 0; j < kMine; j++) {
     const int i = tid * kMine + j;
     uint32_t v = 0;
-    lb[j] = i < nl ? bin_of(B, key_value((uint32_t)(S.list[i] >> 32)), v) : kBins;
+    lb[j] = i < nl ? bin_of(B, key_value((uint32_t)(list[i] >> 32)), v) : kBins;
     bins[i] = lb[j];
     q[j] = v;
     sum += v;
@@ -884,7 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     if (i >= nl) continue;
     if (P.p < 1.0 && cum[j] >= P.p * z) atomicMin(&S.n_p, num[j]);
     if (R.lo[2] <= R.hi[2] && lb[j] >= R.lo[2] && lb[j] <= R.hi[2] &&
-        weight(key_value((uint32_t)(S.list[i] >> 32)), B.xmax, P.t) >= P.minp)
+        weight(key_value((uint32_t)(list[i] >> 32)), B.xmax, P.t) >= P.minp)
       atomicMin(&S.n_m, ~num[j]);  // the largest place
   }
   __syncthreads();
@@ -927,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   for (int j = 0; j < kMine; j++) {
     const int i = tid * kMine + j;
     if (i < nl && num[j] == (uint32_t)S.best) {
-      const unsigned long long me = S.list[i];
+      const unsigned long long me = list[i];
       a.ids[row] = ~(uint32_t)me;
       if (a.probs) a.probs[row] = (float)(weight(key_value((uint32_t)(me >> 32)), B.xmax, P.t) / mass);
     }
@@ -947,7 +976,7 @@ int cluster_size(int rows, int n) {
 template <int kThreads>
 cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
   const int per = ((a.n + c - 1) / c + 3) & ~3, staged = per <= kSlice;
-  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 + kStagedHits * 4 : kHits * 4, kList * 12);
+  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 + kStagedHits * 4 : kHits * 4, kList * 12 + kCountMost * 8);
   static_assert(sizeof(FastSmem) + kSlice * 4 + kStagedHits * 4 <= 113 << 10, "two CTAs an SM");
   static OncePerDevice once;
   int dev = 0;
