@@ -464,7 +464,7 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
 #pragma unroll
     for (int c = 0; c < 8; c++) {  // all remote loads in flight
       if (c >= C) break;
-      const FastSmem* R = cl.map_shared_rank(&S, c);
+      const FastSmem* R = c == 0 ? &S : cl.map_shared_rank(&S, c);  // the leader is rank 0
 #pragma unroll
       for (int j = 0; j < kPer; j += 2) {
         const uint2 n = *reinterpret_cast<const uint2*>(R->cnt + tid * kPer + j);
@@ -963,13 +963,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   }
 }
 
-// CTAs of a row's cluster: as many as all rows' CTAs can be resident at once
-// (two an SM) with slices of 2048 tokens or longer.  A slice is staged in
-// shared memory where it fits; few CTAs a row read it from L2 in each pass
-// instead (256 rows of 151936: one unstaged CTA a row 120 us, eight staged 276).
+// CTAs of a row's cluster: as many as leave every CTA an SM of its own, with
+// slices of 4096 tokens or longer (32 rows of 151936: 4 CTAs a row 34 us, 8 39;
+// 64 rows: 2 51, 8 71; 256 rows: 1 133, 8 243); clusters of 8, which do not fill
+// the GPCs' SMs, for up to 8 rows.
 int cluster_size(int rows, int n) {
   int c = 1;
-  while (c < 8 && 2LL * rows * c <= 2 * 148 && n / (2 * c) >= 2048) c *= 2;
+  while (c < 8 && 2LL * rows * c <= (c == 4 ? 64 : 128) && n / (2 * c) >= 4096) c *= 2;
   return c;
 }
 
@@ -1000,12 +1000,11 @@ cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, sample_kernel<kThreads>, a, staged);
 }
 
-// 1024 threads while every cluster finds SMs of its own (clusters of 8 do not
-// fill the GPCs' SMs: 16 rows took two rounds, 49 us against 37), else two CTAs
-// of 512 an SM.
+// 1024 threads for the few rows that take clusters of 8 (27 us against 29), else
+// 512, two CTAs an SM.
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
   const int c = cluster_size(a.rows, a.n);
-  return (long long)a.rows * c <= 64 && a.n / c >= 4096 ? launch_sample<1024>(a, c, st) : launch_sample<512>(a, c, st);
+  return c == 8 ? launch_sample<1024>(a, c, st) : launch_sample<512>(a, c, st);
 }
 
 }  // namespace
