@@ -97,13 +97,20 @@ __device__ Cut generic_cut(const float* x, int n, float xmax, double t, double s
     const int shift = 24 - 8 * level;
     for (int i = threadIdx.x; i < 256; i += kThreads) S.mass[i] = 0, S.cnt[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const float v = __ldg(x + i);
+    for (int i0 = 0; i0 < n; i0 += kThreads) {
+      const int i = i0 + threadIdx.x;
+      const float v = i < n ? __ldg(x + i) : -INFINITY;
       const uint32_t key = order_key(v);
-      if (!key || (level && (key >> (shift + 8)) != prefix)) continue;
-      const uint32_t b = (key >> shift) & 255;
-      atomicAdd(&S.cnt[b], 1u);
-      if (by_mass) atomicAdd(&S.mass[b], (unsigned long long)__double2ll_rn(weight(v, xmax, t) * scale));
+      const bool in = key && (!level || (key >> (shift + 8)) == prefix);
+      const uint32_t vote = __ballot_sync(0xffffffffu, in), one = vote & (0u - vote);
+      if (!vote) continue;
+      // many equal logits: one atomic for the warp
+      const uint32_t key1 = __shfl_sync(0xffffffffu, key, __ffs(vote) - 1);
+      const bool same = __all_sync(0xffffffffu, !in || key == key1);
+      if (!in || (same && !((one >> (threadIdx.x & 31)) & 1))) continue;
+      const uint32_t b = (key >> shift) & 255, many = same ? __popc(vote) : 1;
+      atomicAdd(&S.cnt[b], many);
+      if (by_mass) atomicAdd(&S.mass[b], many * (unsigned long long)__double2ll_rn(weight(v, xmax, t) * scale));
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -274,10 +281,11 @@ __device__ __noinline__ void sample_generic(const SampleArgs& a, int row, Generi
 namespace cg = cooperative_groups;
 
 constexpr int kBins = 2048;        // the last one: past the range
-constexpr int kList = 1024;        // gathered tokens
+constexpr int kList = 2048;        // gathered tokens
 constexpr int kCountMost = 256;    // of them put in order by counting
-constexpr int kSlice = 19200;      // most tokens that a CTA stages (75 KB: two CTAs an SM)
-constexpr int kHits = 8192, kStagedHits = 1024;  // ids that a pass may pick before they are checked
+// Most tokens that a CTA stages: with an SM to itself, or as one of two.
+constexpr int kSliceAlone = 38912, kSlice = 15872;
+constexpr int kHits = 8192, kStagedHits = 2048;  // ids that a pass may pick before they are checked
 constexpr int kQBits = 26;
 constexpr uint32_t kQBase = (1u << kQBits) - (1u << 22);
 constexpr uint32_t kDense = 512;   // tokens of a CTA in one bin, at most, in the usual form
@@ -384,18 +392,15 @@ __device__ __forceinline__ void cp_async16g(void* dst, const void* src) {
                : "memory");
 }
 
-// list[0 .. np) (np a power of two from 64 to 1024) into falling order: 32
+// list[0 .. np) (np a power of two from 64 to kList) into falling order: 32
 // pairs a warp in registers and shuffles, shared memory where a step spans
 // more than a warp's 64 values.
 template <int kThreads>
 __device__ __forceinline__ void bitonic_falling(unsigned long long* list, int np) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int base = 64 * warp;
-  const bool on = base < np;
   auto inside = [&](int size, int dmax) {  // the steps of distances dmax <= 32 .. 1 of one size
-    if (on) {
+    for (int base = 64 * warp; base < np; base += 2 * kThreads) {
       unsigned long long x = list[base + lane], y = list[base + 32 + lane];
-      // values base + lane and base + 32 + lane
       for (int d = dmax; d > 0; d /= 2) {
         if (d == 32) {
           const bool fall = ((base + lane) & size) == 0;
@@ -582,6 +587,130 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
   }
 }
 
+// The leader's last part: place and running mass of each gathered token (kMine
+// consecutive ones a thread), the cuts of the filters, the sample.
+template <int kThreads, int kMine>
+__device__ __forceinline__ void finish_row(const SampleArgs& a, int row, FastSmem& S, const Bins& B, const RowParams& P,
+                                           const unsigned long long* list, int nl, float* xs) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  unsigned long long* before = reinterpret_cast<unsigned long long*>(xs);  // sum of q before each; the slice is done with
+  int* bins = reinterpret_cast<int*>(before + kList);
+  int lb[kMine], start[kMine];
+  unsigned long long q[kMine], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid * kMine + j;
+    uint32_t v = 0;
+    lb[j] = i < nl ? bin_of(B, key_value((uint32_t)(list[i] >> 32)), v) : kBins;
+    bins[i] = lb[j];
+    q[j] = v;
+    sum += v;
+  }
+  unsigned long long incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) S.lsum[warp] = incl;
+  __syncthreads();
+  unsigned long long pre, all;
+  warp_sums<kThreads>(S.lsum, pre, all);
+  pre += incl - sum;
+  int first = 0;
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid * kMine + j;
+    before[i] = pre;
+    pre += q[j];
+    if (i > 0 && bins[i - 1] != lb[j]) first = i;
+    start[j] = first;
+  }
+  int most = first;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, most, o);
+    if (lane >= o) most = max(most, v);
+  }
+  int prev = __shfl_up_sync(0xffffffffu, most, 1);
+  if (lane == 0) prev = 0;
+  if (lane == 31) S.wcnt[warp] = (uint32_t)most;
+  __syncthreads();
+  prev = max(prev, __reduce_max_sync(0xffffffffu, lane < warp ? (int)S.wcnt[lane] : 0));
+  uint32_t num[kMine];
+  double cum[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid * kMine + j;
+    num[j] = 0xffffffffu;
+    cum[j] = 0.0;
+    if (i < nl) {
+      const int s0 = max(start[j], prev);
+      num[j] = S.count_above[lb[j]] + (uint32_t)(i - s0) + 1;
+      cum[j] = S.above[lb[j]] + (double)(before[i] - before[s0] + q[j]) * bin_unit(B, S.unit, lb[j]);
+      if (P.k > 0 && (uint32_t)P.k == num[j]) S.z = cum[j];
+    }
+  }
+  __syncthreads();
+  const Ranges R = S.rg;
+  const bool k_in = R.lo[0] <= R.hi[0];
+  const double z = S.z;
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid * kMine + j;
+    if (i >= nl) continue;
+    if (P.p < 1.0 && cum[j] >= P.p * z) atomicMin(&S.n_p, num[j]);
+    if (R.lo[2] <= R.hi[2] && lb[j] >= R.lo[2] && lb[j] <= R.hi[2] &&
+        weight(key_value((uint32_t)(list[i] >> 32)), B.xmax, P.t) >= P.minp)
+      atomicMin(&S.n_m, ~num[j]);  // the largest place
+  }
+  __syncthreads();
+  uint32_t n_keep = k_in ? (uint32_t)P.k : 0xffffffffu;  // 0xffffffff: everything that weighs
+  double mass = z;
+  const uint32_t n_p = S.n_p;
+  uint32_t n_m = 0xffffffffu;
+  if (R.lo[2] <= R.hi[2]) n_m = S.n_m == 0xffffffffu ? S.count_above[R.lo[2]] : ~S.n_m;
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    if (num[j] == n_p && n_p != 0xffffffffu) S.mass_p = cum[j];
+    if (num[j] == n_m) S.mass_m = cum[j];
+  }
+  if (tid == 0 && R.lo[2] <= R.hi[2] && S.n_m == 0xffffffffu) S.mass_m = S.above[R.lo[2]];
+  __syncthreads();
+  if (n_p < n_keep) n_keep = n_p, mass = S.mass_p;
+  if (n_m < n_keep) n_keep = n_m, mass = S.mass_m;
+  if (n_keep == 0) n_keep = 1, mass = 1.0;  // min_p above 1: the best token stays
+  const double target = P.r * mass;
+#pragma unroll
+  for (int j = 0; j < kMine; j++)
+    if (num[j] <= n_keep && num[j] != 0xffffffffu && (cum[j] >= target || num[j] == n_keep))
+      atomicMin(&S.best, (unsigned long long)num[j]);
+  __syncthreads();
+  if (S.best == ~0ull) {  // the target lies past the gathered tokens by a rounding: the last of them
+    uint32_t end = 0;
+#pragma unroll
+    for (int j = 0; j < kMine; j++)
+      if (num[j] != 0xffffffffu && num[j] <= n_keep) end = max(end, num[j]);
+    end = __reduce_max_sync(0xffffffffu, end);
+    if (lane == 0) S.wcnt[warp] = end;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < kThreads / 32; w++) end = max(end, S.wcnt[w]);
+      S.best = end;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < kMine; j++) {
+    const int i = tid * kMine + j;
+    if (i < nl && num[j] == (uint32_t)S.best) {
+      const unsigned long long me = list[i];
+      a.ids[row] = ~(uint32_t)me;
+      if (a.probs) a.probs[row] = (float)(weight(key_value((uint32_t)(me >> 32)), B.xmax, P.t) / mass);
+    }
+  }
+}
+
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const __grid_constant__ SampleArgs a, int staged) {
   extern __shared__ __align__(16) unsigned char dsm[];
@@ -731,12 +860,19 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     if (wide) {
       each([&](float4 v, int) {
         const float w[4] = {v.x, v.y, v.z, v.w};
-        for (int j = 0; j < 4; j++)
-          if (in_range(bin_place(B, w[j]))) {
-            uint32_t q;
-            const int b = bin_of(B, w[j], q);
-            atomicAdd(&S.hist[b], kCountOne + q);
-          }
+        for (int j = 0; j < 4; j++) {
+          const bool in = in_range(bin_place(B, w[j]));
+          uint32_t q;
+          const int b = bin_of(B, w[j], q);
+          const uint32_t vote = __ballot_sync(0xffffffffu, in);
+          if (!vote) continue;
+          // many equal logits: one atomic for the warp
+          const int one = __ffs(vote) - 1;
+          const int b1 = __shfl_sync(0xffffffffu, b, one);
+          const uint32_t q1 = __shfl_sync(0xffffffffu, q, one);
+          const bool same = __all_sync(0xffffffffu, !in || (b == b1 && q == q1));
+          if (in && (!same || lane == one)) atomicAdd(&S.hist[b], (kCountOne + q) * (same ? __popc(vote) : 1));
+        }
       });
       cl.sync();
     }
@@ -820,8 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     sample_generic<kThreads>(a, row, *reinterpret_cast<GenericSmem*>(dsm));
     return;
   }
-  // ---- the gathered tokens in order (a bitonic sort, falling), then the place
-  // and running mass of each: sums from the first token of its bin on
+  // ---- the gathered tokens in falling order
   unsigned long long* list = S.list;
   if (nl <= kCountMost) {
     // a few: each is compared with all, eight threads a token
@@ -844,123 +979,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     __syncthreads();
     bitonic_falling<kThreads>(S.list, np);
   }
-  constexpr int kMine = kList / kThreads;  // consecutive tokens of a thread
-  unsigned long long* before = reinterpret_cast<unsigned long long*>(xs);  // sum of q before each; the slice is done with
-  int* bins = reinterpret_cast<int*>(before + kList);
-  int lb[kMine], start[kMine];
-  unsigned long long q[kMine], sum = 0;
-#pragma unroll
-  for (int j = 0; j < kMine; j++) {
-    const int i = tid * kMine + j;
-    uint32_t v = 0;
-    lb[j] = i < nl ? bin_of(B, key_value((uint32_t)(list[i] >> 32)), v) : kBins;
-    bins[i] = lb[j];
-    q[j] = v;
-    sum += v;
-  }
-  unsigned long long incl = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) S.lsum[warp] = incl;
-  __syncthreads();
-  unsigned long long pre, all;
-  warp_sums<kThreads>(S.lsum, pre, all);
-  pre += incl - sum;
-  int first = 0;
-#pragma unroll
-  for (int j = 0; j < kMine; j++) {
-    const int i = tid * kMine + j;
-    before[i] = pre;
-    pre += q[j];
-    if (i > 0 && bins[i - 1] != lb[j]) first = i;
-    start[j] = first;
-  }
-  int most = first;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, most, o);
-    if (lane >= o) most = max(most, v);
-  }
-  int prev = __shfl_up_sync(0xffffffffu, most, 1);
-  if (lane == 0) prev = 0;
-  if (lane == 31) S.wcnt[warp] = (uint32_t)most;
-  __syncthreads();
-  prev = max(prev, __reduce_max_sync(0xffffffffu, lane < warp ? (int)S.wcnt[lane] : 0));
-  uint32_t num[kMine];
-  double cum[kMine];
-#pragma unroll
-  for (int j = 0; j < kMine; j++) {
-    const int i = tid * kMine + j;
-    num[j] = 0xffffffffu;
-    cum[j] = 0.0;
-    if (i < nl) {
-      const int s0 = max(start[j], prev);
-      num[j] = S.count_above[lb[j]] + (uint32_t)(i - s0) + 1;
-      cum[j] = S.above[lb[j]] + (double)(before[i] - before[s0] + q[j]) * bin_unit(B, S.unit, lb[j]);
-      if (P.k > 0 && (uint32_t)P.k == num[j]) S.z = cum[j];
-    }
-  }
-  __syncthreads();
-  const Ranges R = S.rg;
-  const bool k_in = R.lo[0] <= R.hi[0];
-  const double z = S.z;
-#pragma unroll
-  for (int j = 0; j < kMine; j++) {
-    const int i = tid * kMine + j;
-    if (i >= nl) continue;
-    if (P.p < 1.0 && cum[j] >= P.p * z) atomicMin(&S.n_p, num[j]);
-    if (R.lo[2] <= R.hi[2] && lb[j] >= R.lo[2] && lb[j] <= R.hi[2] &&
-        weight(key_value((uint32_t)(list[i] >> 32)), B.xmax, P.t) >= P.minp)
-      atomicMin(&S.n_m, ~num[j]);  // the largest place
-  }
-  __syncthreads();
-  uint32_t n_keep = k_in ? (uint32_t)P.k : 0xffffffffu;  // 0xffffffff: everything that weighs
-  double mass = z;
-  const uint32_t n_p = S.n_p;
-  uint32_t n_m = 0xffffffffu;
-  if (R.lo[2] <= R.hi[2]) n_m = S.n_m == 0xffffffffu ? S.count_above[R.lo[2]] : ~S.n_m;
-#pragma unroll
-  for (int j = 0; j < kMine; j++) {
-    if (num[j] == n_p && n_p != 0xffffffffu) S.mass_p = cum[j];
-    if (num[j] == n_m) S.mass_m = cum[j];
-  }
-  if (tid == 0 && R.lo[2] <= R.hi[2] && S.n_m == 0xffffffffu) S.mass_m = S.above[R.lo[2]];
-  __syncthreads();
-  if (n_p < n_keep) n_keep = n_p, mass = S.mass_p;
-  if (n_m < n_keep) n_keep = n_m, mass = S.mass_m;
-  if (n_keep == 0) n_keep = 1, mass = 1.0;  // min_p above 1: the best token stays
-  const double target = P.r * mass;
-#pragma unroll
-  for (int j = 0; j < kMine; j++)
-    if (num[j] <= n_keep && num[j] != 0xffffffffu && (cum[j] >= target || num[j] == n_keep))
-      atomicMin(&S.best, (unsigned long long)num[j]);
-  __syncthreads();
-  if (S.best == ~0ull) {  // the target lies past the gathered tokens by a rounding: the last of them
-    uint32_t end = 0;
-#pragma unroll
-    for (int j = 0; j < kMine; j++)
-      if (num[j] != 0xffffffffu && num[j] <= n_keep) end = max(end, num[j]);
-    end = __reduce_max_sync(0xffffffffu, end);
-    if (lane == 0) S.wcnt[warp] = end;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 0; w < kThreads / 32; w++) end = max(end, S.wcnt[w]);
-      S.best = end;
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int j = 0; j < kMine; j++) {
-    const int i = tid * kMine + j;
-    if (i < nl && num[j] == (uint32_t)S.best) {
-      const unsigned long long me = list[i];
-      a.ids[row] = ~(uint32_t)me;
-      if (a.probs) a.probs[row] = (float)(weight(key_value((uint32_t)(me >> 32)), B.xmax, P.t) / mass);
-    }
-  }
+  // one token a thread where that holds them all
+  if (nl <= kThreads) finish_row<kThreads, 1>(a, row, S, B, P, list, nl, xs);
+  else finish_row<kThreads, kList / kThreads>(a, row, S, B, P, list, nl, xs);
 }
 
 // CTAs of a row's cluster: as many as leave every CTA an SM of its own, with
@@ -975,14 +996,16 @@ int cluster_size(int rows, int n) {
 
 template <int kThreads>
 cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
-  const int per = ((a.n + c - 1) / c + 3) & ~3, staged = per <= kSlice;
+  const int per = ((a.n + c - 1) / c + 3) & ~3;
+  const int staged = per <= ((long long)a.rows * c <= 148 ? kSliceAlone : kSlice);
   const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 + kStagedHits * 4 : kHits * 4, kList * 12 + kCountMost * 8);
   static_assert(sizeof(FastSmem) + kSlice * 4 + kStagedHits * 4 <= 113 << 10, "two CTAs an SM");
+  static_assert(sizeof(FastSmem) + kSliceAlone * 4 + kStagedHits * 4 <= 227 << 10, "a CTA's shared memory");
   static OncePerDevice once;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && once.first(dev)) {
-    e = cudaFuncSetAttribute(sample_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 << 10);
+    e = cudaFuncSetAttribute(sample_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 << 10);
     if (e == cudaSuccess) once.done(dev);
   }
   if (e != cudaSuccess) return e;
