@@ -57,48 +57,70 @@ __device__ __forceinline__ void store4<__half>(__half* d, float4 v) {
       make_uint2(h2_bits(__floats2half2_rn(v.x, v.y)), h2_bits(__floats2half2_rn(v.z, v.w)));
 }
 
-template <typename KVT>
+// The bound is bytes, 512 read and 256 or 512 written a head.  U heads a half-
+// warp, their loads issued first: at 16384 tokens of 48 heads (743 MB) U = 2
+// runs at the copy rate (113 us, U = 1 120), at 512 tokens of 20 the launch and
+// three dependent loads are the time (U = 1 3.1 us, U = 2 3.5).
+template <typename KVT, int U>
 __global__ void __launch_bounds__(256) kv_append_paged_kernel(AppendArgs a) {
   const int H = a.nh + 2 * a.nkv, l = threadIdx.x & 15;
-  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
-  if (item >= (long long)a.T * H) return;
-  const int t = (int)(item / H), h = (int)(item - (long long)t * H);
-  if (h < a.nh && !a.q_out) return;
-  const float* src = a.qkv + t * a.ld + h * kHeadDim + 4 * l;
-  float4 lo = __ldcs(reinterpret_cast<const float4*>(src));
-  float4 hi = __ldcs(reinterpret_cast<const float4*>(src + kHeadDim / 2));
-  const int pos = __ldg(a.pos + t), s = __ldg(a.slot + t);
-  if (pos < 0) return;  // a padding row
-  const int row = pos - a.prefix_len;
-  bool ok = pos < a.table_len && row >= 0 && s >= 0 && s < a.n_slots && row / kPage < a.max_pages;
-  uint32_t page = 0;
-  if (ok) {
-    page = __ldg(a.pages + (size_t)s * a.max_pages + row / kPage);
-    ok = page < (uint32_t)a.n_pages;
+  const long long first = (long long)blockIdx.x * 16 * U + (threadIdx.x >> 4), n = (long long)a.T * H;
+  float4 lo[U], hi[U];
+  int t[U], h[U], pos[U], s[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const long long item = first + 16 * u;
+    t[u] = item < n ? (int)(item / H) : 0;
+    h[u] = (int)(item - (long long)t[u] * H);
+    pos[u] = -1;
+    if (item < n && (h[u] >= a.nh || a.q_out)) {
+      const float* src = a.qkv + t[u] * a.ld + h[u] * kHeadDim + 4 * l;
+      lo[u] = __ldg(reinterpret_cast<const float4*>(src));
+      hi[u] = __ldg(reinterpret_cast<const float4*>(src + kHeadDim / 2));
+      pos[u] = __ldg(a.pos + t[u]);
+      s[u] = __ldg(a.slot + t[u]);
+    }
   }
-  if (!ok) {
-    if (a.err && l == 0) *a.err = 1;
-    return;
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    if (pos[u] < 0) continue;  // a padding row
+    const int row = pos[u] - a.prefix_len;
+    bool ok = pos[u] < a.table_len && row >= 0 && s[u] >= 0 && s[u] < a.n_slots && row / kPage < a.max_pages;
+    uint32_t page = 0;
+    if (ok) {
+      page = __ldg(a.pages + (size_t)s[u] * a.max_pages + row / kPage);
+      ok = page < (uint32_t)a.n_pages;
+    }
+    if (!ok) {
+      if (a.err && l == 0) *a.err = 1;
+      continue;
+    }
+    if (h[u] < a.nh + a.nkv) {
+      const float4 c = __ldg(reinterpret_cast<const float4*>(a.cosT + (size_t)pos[u] * kHeadDim + 4 * l));
+      const float4 d = __ldg(reinterpret_cast<const float4*>(a.sinT + (size_t)pos[u] * kHeadDim + 4 * l));
+      rope_pair(lo[u].x, hi[u].x, c.x, d.x, 0);
+      rope_pair(lo[u].y, hi[u].y, c.y, d.y, 0);
+      rope_pair(lo[u].z, hi[u].z, c.z, d.z, 0);
+      rope_pair(lo[u].w, hi[u].w, c.w, d.w, 0);
+    }
+    if (h[u] < a.nh) {
+      float* d = a.q_out + t[u] * a.ldq + h[u] * kHeadDim + 4 * l;
+      store4(d, lo[u]);
+      store4(d + kHeadDim / 2, hi[u]);
+      continue;
+    }
+    const bool is_k = h[u] < a.nh + a.nkv;
+    const int kvh = h[u] - a.nh - (is_k ? 0 : a.nkv);
+    KVT* d = static_cast<KVT*>(is_k ? a.kc : a.vc) + (((size_t)page * kPage + row % kPage) * a.nkv + kvh) * kHeadDim + 4 * l;
+    store4(d, lo[u]);
+    store4(d + kHeadDim / 2, hi[u]);
   }
-  if (h < a.nh + a.nkv) {
-    const float4 c = __ldg(reinterpret_cast<const float4*>(a.cosT + (size_t)pos * kHeadDim + 4 * l));
-    const float4 n = __ldg(reinterpret_cast<const float4*>(a.sinT + (size_t)pos * kHeadDim + 4 * l));
-    rope_pair(lo.x, hi.x, c.x, n.x, 0);
-    rope_pair(lo.y, hi.y, c.y, n.y, 0);
-    rope_pair(lo.z, hi.z, c.z, n.z, 0);
-    rope_pair(lo.w, hi.w, c.w, n.w, 0);
-  }
-  if (h < a.nh) {
-    float* d = a.q_out + t * a.ldq + h * kHeadDim + 4 * l;
-    store4(d, lo);
-    store4(d + kHeadDim / 2, hi);
-    return;
-  }
-  const int kvh = h < a.nh + a.nkv ? h - a.nh : h - a.nh - a.nkv;
-  KVT* d = static_cast<KVT*>(h < a.nh + a.nkv ? a.kc : a.vc) +
-           (((size_t)page * kPage + row % kPage) * a.nkv + kvh) * kHeadDim + 4 * l;
-  store4(d, lo);
-  store4(d + kHeadDim / 2, hi);
+}
+
+template <typename KVT>
+void launch_append(const AppendArgs& a, long long heads, cudaStream_t st) {
+  if (heads >= 131072) kv_append_paged_kernel<KVT, 2><<<(unsigned)((heads + 31) / 32), 256, 0, st>>>(a);
+  else kv_append_paged_kernel<KVT, 1><<<(unsigned)((heads + 15) / 16), 256, 0, st>>>(a);
 }
 
 // ======================================================================
@@ -1079,13 +1101,11 @@ EG_API eg_status eg_op_kv_append_paged(const float* qkv, int64_t ld, int T, cons
     return fail(EG_ERR_ARG, "kv_append_paged: 16-byte aligned buffers required");
   AppendArgs a = {qkv, ld, T, pos, slot, pages, n_slots, max_pages, n_pages, prefix_len, k_cache, v_cache,
                   cos_t, sin_t, table_len, nh, nkv, q_out, ldq, err};
-  const long long blocks = ((long long)T * H + 15) / 16;
-  if (blocks > 0x7fffffffLL) return fail(EG_ERR_ARG, "kv_append_paged: too many rows");
+  const long long heads = (long long)T * H;
+  if (heads / 16 >= 0x7fffffffLL) return fail(EG_ERR_ARG, "kv_append_paged: too many rows");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (kv_f16)
-    kv_append_paged_kernel<__half><<<(unsigned)blocks, 256, 0, st>>>(a);
-  else
-    kv_append_paged_kernel<float><<<(unsigned)blocks, 256, 0, st>>>(a);
+  if (kv_f16) launch_append<__half>(a, heads, st);
+  else launch_append<float>(a, heads, st);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(EG_ERR_CUDA, "kv_append_paged: %s", cudaGetErrorString(e));
   return EG_OK;
