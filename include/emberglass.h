@@ -420,7 +420,8 @@ EG_API eg_status eg_op_sample_topk(const uint32_t* ids, const float* vals, int k
  * by its position and v go to row pos[t] - prefix_len of the slot's pages
  * (pages [n_slots][max_pages]; a slot that continues a shared prefix holds
  * only what follows it), each rounded once to the cache's type; q turned goes
- * to q_out (rows ldq floats apart; NULL: q is not wanted; not qkv itself).
+ * to q_out (rows ldq floats apart; NULL: q is not wanted; qkv with ldq = ld:
+ * in place).
  * The rotation is f32 in both cache types.  cos_t / sin_t: [table_len][128].
  * pos[t] < 0: a padding row, nothing of it is read on or written.  A position
  * outside the table or the slot's pages, a slot outside n_slots or a page

@@ -155,6 +155,26 @@ def test_append_far_rows(cuda):
             assert torch.equal(far[p, :n], near.d[c][int(near.pages[0, i]), :n])
 
 
+def test_append_turns_q_in_place(cuda):
+    """q_out may be qkv's own q heads, as attn_prefill turns them."""
+    for runs in ([(0, 20), (7, 9)], [(0, 7000)]):
+        a = Append(cuda, runs, 16, 2, "f16")
+        a.d["q_out"] = a.d["qkv"][:, :16 * HD]
+        K.kv_append_paged(**a.d)
+        a.check()
+
+
+def test_append_many_tokens(cuda):
+    """More heads than the small form takes."""
+    a = Append(cuda, [(5, 5003), (0, 1800)], 16, 2, "f16", prefix=3, pad=(17, 6802))
+    K.kv_append_paged(**a.d)
+    a.check()
+    b = Append(cuda, [(0, 3700)], 28, 4, "f32")
+    b.d["q_out"] = None
+    K.kv_append_paged(**b.d)
+    b.check()
+
+
 # ---------------------------------------------------------------- attention over a shared prefix
 class Shared:
     def __init__(self, cuda, prefix, lens, nh, nkv, kv, seed=0, max_len=None, extra=0, spike=0.0, fill=np.nan):
@@ -316,6 +336,73 @@ def test_shared_prefix_two_streams_two_workspaces(cuda):
     b.check(range(0, 11, 5))
 
 
+@pytest.mark.parametrize("kv,n,prefix,longest", [("f16", 40, 4000, 100), ("f16", 9, 300, 40), ("f32", 30, 1100, 50)])
+def test_shared_prefix_captured(cuda, kv, n, prefix, longest):
+    """One capture, replayed over other lengths, pages and queries, gives the
+    bits of eager calls (each kernel choice: tensor cores, one launch, f32)."""
+    lens = [(i * 13) % (longest + 1) for i in range(n)]
+    s = Shared(cuda, prefix, lens, 16, 2, kv, seed=3, max_len=longest)
+    K.attn_shared_prefix(**s.d)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        K.attn_shared_prefix(**s.d)
+        K.attn_shared_prefix(**s.d)  # the same workspace, one after the other
+    for seed in (11, 12):
+        o = Shared(cuda, prefix, lens[::-1] if seed == 12 else lens, 16, 2, kv, seed=seed, max_len=longest)
+        for k in ("q", "k_cache", "v_cache", "prefix_pages", "pages", "lens"):
+            s.d[k].copy_(o.d[k])
+        s.d["out"].fill_(5.0)
+        g.replay()
+        K.attn_shared_prefix(**o.d)
+        torch.cuda.synchronize()
+        assert torch.equal(s.d["out"], o.d["out"])
+        o.check(range(0, n, 5))
+
+
+def test_shared_prefix_workspace_of_another_size(cuda):
+    """Calls of different shapes in turn through one workspace."""
+    shapes = [(40, 4000, 60), (3, 100, 20), (12, 1000, 300), (70, 2500, 5)]
+    cases = [Shared(cuda, p, [(i * 7) % (m + 1) for i in range(n)], 16, 2, "f16", seed=n, max_len=m) for n, p, m in shapes]
+    ws = max((c.d["ws"] for c in cases), key=lambda t: t.numel())
+    for _ in range(2):
+        for c in cases:
+            c.d["out"].fill_(5.0)
+            K.attn_shared_prefix(**{**c.d, "ws": ws})
+    for c in cases:
+        c.check(range(0, len(c.lens), 9))
+
+
+@pytest.mark.parametrize("prefix", [256, 257, 1535, 1537, 2999, 4097])
+def test_shared_prefix_block_ends(cuda, prefix):
+    """Prefixes that end at, before and behind the blocks and splits of the tensor-core form, and one bad page in it."""
+    n = 65 if prefix > 1000 else 300
+    s = Shared(cuda, prefix, [i % 3 for i in range(n)], 16, 2, "f16", seed=prefix)
+    K.attn_shared_prefix(**s.d)
+    s.check(range(0, n, n // 8))
+    assert s.d["err"].item() == 0
+    last = (prefix - 1) // PAGE
+    s.d["prefix_pages"][last] = 1 << 24
+    K.attn_shared_prefix(**s.d)
+    s.prefix = last * PAGE
+    s.check(range(0, n, n // 8))
+    assert s.d["err"].item() == 1
+
+
+def test_shared_prefix_rising_scores(cuda):
+    """Scores that rise along the prefix: the tensor-core form moves its base again and again."""
+    n, prefix = 64, 3000
+    s = Shared(cuda, prefix, [4] * n, 16, 2, "f16", seed=8)
+    rows = R.rows_of(s.ppages, prefix)
+    d = np.sign(np.random.default_rng(1).standard_normal(HD)).astype(np.float32)
+    s.kc[rows] = (s.kc[rows].astype(np.float32) * 0.3 + np.linspace(0, 4, prefix)[:, None, None] * d / 8).astype(np.float16)
+    s.q[:, :16 * HD] = np.tile(d * 12, 16) + s.q[:, :16 * HD] * 0.1
+    s.d["k_cache"].copy_(torch.from_numpy(s.kc.reshape(s.d["k_cache"].shape)))
+    s.d["q"].copy_(torch.from_numpy(s.q[:, :16 * HD]))
+    K.attn_shared_prefix(**s.d)
+    s.check(range(0, n, 7))
+
+
 # ---------------------------------------------------------------- sampling
 def rows_for(n, rows, seed, kind):
     rng = np.random.default_rng(seed)
@@ -446,6 +533,79 @@ def test_sample_agrees_with_topk_and_sample_topk(cuda):
         torch.cuda.synchronize()
         near = {R.sample(x[i], 0.8, 40, r=float(r[i]) + e)[0] for e in (-1e-5, 0, 1e-5)}
         assert one.item() in near and int(got[i]) in near
+
+
+@pytest.mark.parametrize("order", ["falling", "rising", "blocks"])
+def test_sample_neighbours_in_the_vocabulary(cuda, order):
+    """The deciding tokens side by side in the row, or a whole row of a few values."""
+    n = 100000
+    x = np.sort(rows_for(n, 4, 6, "flat"), 1)
+    x = {"falling": x[:, ::-1], "rising": x, "blocks": np.round(x * 4) / 4}[order].astype(np.float32).copy()
+    r = np.array([0.1, 0.5, 0.9, 0.99], np.float32)
+    for t, k, p, m in [(1, 0, 0.9, 0), (0.7, 3000, 1, 0.01), (1, 0, 1, 0)]:
+        got, probs = run_sample(cuda, x, t, k, p, m, r)
+        check_sample(x, got, probs, t, k, p, m, r)
+
+
+def test_sample_extreme_temperatures(cuda):
+    x = rows_for(3001, 5, 14, "flat")
+    for t in (1e-40, 1e-30, 1e-25, 1e-6, 1e-3, 1e4, 1e28, 1e38, float("inf")):
+        r = np.array([0.0, 0.3, 0.6, 0.9, 0.999], np.float32)
+        got, probs = run_sample(cuda, x, t, 0, 1.0, 0.0, r)
+        if t < 1e-4:
+            assert got.tolist() == x.argmax(1).tolist() and (probs > 0.999).all()
+        else:
+            check_sample(x, got, probs, t, 0, 1.0, 0.0, r)
+
+
+def test_sample_extreme_values(cuda):
+    big = np.finfo(np.float32).max
+    x = np.zeros((6, 500), np.float32)
+    x[0, 3] = big
+    x[1] = -1e30  # the lowest that is taken
+    x[2] = 1e-42  # below f32's normal range, with one above
+    x[2, 77] = 1e-38
+    x[3, ::2] = -0.0  # equal to +0: ties to the lower id
+    x[4] = -5e29
+    x[4, 9] = -4e29
+    x[5, :499] = np.float32(-1.0000001e30)  # never taken
+    r = np.float32(0.5)
+    got, probs = run_sample(cuda, x, 1.0, 0, 1.0, 0.0, r)
+    assert got[0] == 3 and probs[0] == 1.0
+    assert got[4] == 9 and probs[4] == 1.0
+    assert got[5] == 499 and probs[5] == 1.0
+    for i in (1, 2, 3):
+        assert got[i] in (249, 250) and abs(probs[i] - 1 / 500) < 1e-9, (i, got[i], probs[i])
+    got, _ = run_sample(cuda, x, 1.0, 7, 1.0, 0.0, np.float32(0.99))
+    assert got[3] == 6 and got[1] == 6
+
+
+def test_sample_two_streams_and_capture(cuda):
+    """Two calls at once, and one capture replayed over other inputs (nothing is kept between calls)."""
+    n = 30000
+    xa, xb = rows_for(n, 7, 1, "flat"), rows_for(n, 40, 2, "peaked")
+    f = lambda v, k: torch.full((k,), v, device=cuda)  # noqa: E731
+    a = dict(logits=torch.from_numpy(xa).to(cuda), r=f(0.4, 7), ids=i32(np.zeros(7), cuda), top_p=f(0.9, 7))
+    b = dict(logits=torch.from_numpy(xb).to(cuda), r=f(0.7, 40), ids=i32(np.zeros(40), cuda), min_p=f(0.02, 40))
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        K.sample_filtered(**a, stream=s1)
+        K.sample_filtered(**b, stream=s2)
+    torch.cuda.synchronize()
+    for x, c, kw in ((xa, a, dict(p=float(np.float32(0.9)), r=float(np.float32(0.4)))),
+                     (xb, b, dict(minp=float(np.float32(0.02)), r=float(np.float32(0.7))))):
+        assert all(R.sample_near(x[i], int(g), **kw) for i, g in enumerate(c["ids"].tolist()))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        K.sample_filtered(**a)
+    for seed in (5, 6):
+        x = rows_for(n, 7, seed, "peaked")
+        a["logits"].copy_(torch.from_numpy(x))
+        a["ids"].fill_(-7)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(R.sample_near(x[i], int(v), p=float(np.float32(0.9)), r=float(np.float32(0.4))) for i, v in enumerate(a["ids"].tolist()))
 
 
 def test_sample_same_bits_every_time(cuda):

@@ -75,8 +75,8 @@ __global__ void __launch_bounds__(256) kv_append_paged_kernel(AppendArgs a) {
     pos[u] = -1;
     if (item < n && (h[u] >= a.nh || a.q_out)) {
       const float* src = a.qkv + t[u] * a.ld + h[u] * kHeadDim + 4 * l;
-      lo[u] = __ldg(reinterpret_cast<const float4*>(src));
-      hi[u] = __ldg(reinterpret_cast<const float4*>(src + kHeadDim / 2));
+      lo[u] = __ldcg(reinterpret_cast<const float4*>(src));  // q_out may be these very words
+      hi[u] = __ldcg(reinterpret_cast<const float4*>(src + kHeadDim / 2));
       pos[u] = __ldg(a.pos + t[u]);
       s[u] = __ldg(a.slot + t[u]);
     }

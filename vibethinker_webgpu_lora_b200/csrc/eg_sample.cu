@@ -285,7 +285,7 @@ constexpr int kList = 2048;        // gathered tokens
 constexpr int kCountMost = 256;    // of them put in order by counting
 // Most tokens that a CTA stages: with an SM to itself, or as one of two.
 constexpr int kSliceAlone = 38912, kSlice = 15872;
-constexpr int kHits = 8192, kStagedHits = 2048;  // ids that a pass may pick before they are checked
+constexpr int kHits = 8192, kStagedHits = 4096;  // ids that a pass may pick before they are checked
 constexpr int kQBits = 26;
 constexpr uint32_t kQBase = (1u << kQBits) - (1u << 22);
 constexpr uint32_t kDense = 512;   // tokens of a CTA in one bin, at most, in the usual form
@@ -805,9 +805,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     mx = warp_max(R->mx);
     mn = -warp_max(-R->mn);
   }
-  // rows of values near -1e30, or of steps that reach there, are left to the byte-wise form:
-  // below, what lies in the bins' range is a candidate
-  const bool none = mx == -INFINITY, slow0 = mx == INFINITY || (!none && (mx < -9e29f || P.t > 1e27));
+  // rows of values near -1e30, or of steps that reach there, are left to the byte-wise form
+  // (below, what lies in the bins' range is a candidate), and so are temperatures that f32 cannot divide by
+  const bool none = mx == -INFINITY, slow0 = mx == INFINITY || (!none && (mx < -9e29f || P.t > 1e27 || P.t < 1e-28));
   Bins B;
   if (!none && !slow0) {
     // the range: all candidates, but at most 64 in x and 64 in x / t (whichever is more, steps of at most 2)
@@ -893,8 +893,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     const float from2 = S.rg.from[2], to2 = S.rg.to[2], from3 = S.rg.from[3], to3 = S.rg.to[3];
     const bool more = from2 <= to2 || from3 <= to3;
     // a warp's hits go to its own part of a list of ids: no atomics in the pass
+    // (staged: 16-bit offsets; either way a run of kList neighbours finds room)
     const uint32_t room = (staged ? kStagedHits : kHits) / (kThreads / 32);
-    uint32_t* hits = reinterpret_cast<uint32_t*>(dsm + sizeof(FastSmem) + (staged ? per * 4 : 0)) + warp * room;
+    unsigned char* hits = dsm + sizeof(FastSmem) + (staged ? per * 4 : 0);
+    uint16_t* hits16 = reinterpret_cast<uint16_t*>(hits) + warp * room;
+    uint32_t* hits32 = reinterpret_cast<uint32_t*>(hits) + warp * room;
     const uint32_t below = (1u << lane) - 1;
     uint32_t nh = 0;
     auto inside = [&](float v) {
@@ -909,7 +912,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         for (int j = 0; j < 4; j++) {
           const uint32_t vote = __ballot_sync(0xffffffffu, hit[j]);
           const uint32_t to = nh + __popc(vote & below);
-          if (hit[j] && to < room) hits[to] = (uint32_t)(i + j);
+          if (hit[j] && to < room) {
+            if (staged) hits16[to] = (uint16_t)(i + j - e0);
+            else hits32[to] = (uint32_t)(i + j);
+          }
           nh += __popc(vote);
         }
       }
@@ -921,7 +927,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       uint32_t id = 0;
       float v = 0.f;
       if (k0 + lane < min(nh, room)) {
-        id = hits[k0 + lane];
+        id = staged ? e0 + hits16[k0 + lane] : hits32[k0 + lane];
         v = staged ? xs[id - e0] : __ldg(x + id);
         const float p = bin_place(B, v);
         const int b = __float_as_int(p + kRound) - __float_as_int(kRound);  // as bin_of, where in_range
@@ -998,9 +1004,9 @@ template <int kThreads>
 cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
   const int per = ((a.n + c - 1) / c + 3) & ~3;
   const int staged = per <= ((long long)a.rows * c <= 148 ? kSliceAlone : kSlice);
-  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 + kStagedHits * 4 : kHits * 4, kList * 12 + kCountMost * 8);
-  static_assert(sizeof(FastSmem) + kSlice * 4 + kStagedHits * 4 <= 113 << 10, "two CTAs an SM");
-  static_assert(sizeof(FastSmem) + kSliceAlone * 4 + kStagedHits * 4 <= 227 << 10, "a CTA's shared memory");
+  const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 + kStagedHits * 2 : kHits * 4, kList * 12 + kCountMost * 8);
+  static_assert(sizeof(FastSmem) + kSlice * 4 + kStagedHits * 2 <= 113 << 10, "two CTAs an SM");
+  static_assert(sizeof(FastSmem) + kSliceAlone * 4 + kStagedHits * 2 <= 227 << 10, "a CTA's shared memory");
   static OncePerDevice once;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
