@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const SharedPlan& p = a.p;
   const int G = p.G;
-  if (NG > 1) pdl_launch_dependents();
+  pdl_launch_dependents();  // what follows waits for the end of this kernel before it reads its results
 
   // the CTA's rows [row0, row0 + nrow) of KV head kvh and its keys [k0, k1)
   int kvh, row0, nrow, k0, k1, split, kmax;
