@@ -141,7 +141,6 @@ constexpr float kPBits = 14.f;
 constexpr int kWarps = 4;       // warps of a CTA, each with its own 16-key tiles
 constexpr int kSoPitch = kHeadDim + 4;  // floats a row of the warps' outputs in shared memory
 constexpr int kSms = 148;       // plans are made for the B200's SM count
-constexpr int kTcMaxKeys = 1536;  // keys of a prefix split on the tensor cores
 
 struct SharedPlan {
   int G, gch;          // query heads per KV head; chunks of 8 of them
@@ -197,13 +196,13 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   p.tc = kv_f16 && prefix_len >= 256 && scores >= 900000;
   p.own = p.tc || (!kv_f16 && p.groups > 2 && scores >= 250000);
   if (p.tc) {
-    // one CTA an SM, about 5.5 us and 1.63 us a block of 128 keys: the number of
+    // one CTA an SM, about 5.5 us and 1.8 us a block of 128 keys: the number of
     // splits with the shortest rounds
     const int units = p.row_tiles * nkv;
     double best = 1e300;
-    for (int n = (prefix_len + kTcMaxKeys - 1) / kTcMaxKeys; n <= std::max(1, prefix_len / 256); n++) {
+    for (int n = 1; n <= std::max(1, prefix_len / 256); n++) {
       const int keys = round_up((prefix_len + n - 1) / n, 128), got = (prefix_len + keys - 1) / keys;
-      const double t = (double)(((long long)units * got + kSms - 1) / kSms) * (5.5 + 1.63 * (keys / 128)) + 0.05 * got;
+      const double t = (double)(((long long)units * got + kSms - 1) / kSms) * (5.5 + 1.8 * (keys / 128)) + 0.1 * got;
       if (t < best) best = t, p.pref_keys = keys;
       if ((long long)units * n > 4 * kSms) break;
     }
@@ -537,13 +536,12 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
 // A CTA takes 128 rows of one KV head over one split of the prefix, in blocks
 // of 128 keys: S = q K^T (M = rows, N = keys; q as f16 hi + lo stacked on the
 // same K: 16 MMAs of K = 16), softmax by one thread a row from TMEM, P back to
-// TMEM as f16 hi + lo over S's own columns, O += P V (A from TMEM, V^T as the
+// TMEM as f16 hi + lo over S's own columns, O = P V (A from TMEM, V^T as the
 // key-major tile read MN-major; 16 MMAs).  Two warpgroups take the blocks in
-// turn, so one's softmax runs under the other's products.  O stays in TMEM: a
-// row's base b moves (and its O is scaled) only when the maximum passes b by
-// kTcBits + kTcSlack bits, which after the first block is rare.  The tensor
-// core's sums lose about 2^-24.5 a step, all one way: a split of 1536 keys is
-// 96 steps a warpgroup, 2e-6 of the output on average.
+// turn, so one's softmax runs under the other's products.  A block's O is a
+// fresh accumulator, added to the row's f32 registers while the next scores are
+// made: kept in TMEM over a split it loses about 2^-24.5 a step, all one way
+// (2048 keys: 4e-6 of the output, against 1e-6 here).
 // Warps: 0-3 and 4-7 softmax, 8 copies K, 9 copies V (TMA: a page of one KV
 // head is two boxes of 16 rows x 64 dims, 128-byte swizzle), 10 issues MMAs and
 // owns TMEM.
@@ -552,7 +550,6 @@ constexpr uint32_t kTcTile = 128 * kHeadDim * 2;  // 32 KB: 128 rows or keys of 
 constexpr uint32_t kTcHalf = kTcTile / 2;         // 128 keys x 64 dims, 128-byte rows
 constexpr int kTcSmem = 6 * kTcTile;              // q hi, q lo, 2 x (K, V)
 constexpr uint32_t kTcCols = 512;                 // per warpgroup 128 of S / P and 128 of O
-constexpr float kTcBits = 7.f, kTcSlack = 8.f;    // p up to 2^15 (f16: 65504), 2^7 at the block's maximum where b was set
 
 struct TcSmem {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], v_raw;
@@ -659,7 +656,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
   bool dead = false;
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp < 10) {
       // ------------------------------------------------ K (warp 8) and V (warp 9) of every block
       const bool is_v = warp == 9;
@@ -744,7 +741,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < 8; i++) {  // 16 keys a step: P hi and lo against the same V
-            mma_f16_ts(d, pc + 32 * (i >> 1) + 8 * (i & 1), vd + i * (2048 >> 4), id_o, i > 0 || j > 1);
+            mma_f16_ts(d, pc + 32 * (i >> 1) + 8 * (i & 1), vd + i * (2048 >> 4), id_o, i > 0);
             mma_f16_ts(d, pc + 32 * (i >> 1) + 8 * (i & 1) + 16, vd + i * (2048 >> 4), id_o, true);
           }
           mma_commit(&S.o_full[w]);
@@ -757,7 +754,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
       for (int j = max(0, nblk - 2); j < nblk; j++) tc_wait_bounded(&S.o_full[j & 1], (j >> 1) & 1);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ------------------------------------------------ softmax, one thread a row
     const int w = warp >> 2, r = tid & 127;
     {
@@ -787,79 +784,80 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
       mbar_arrive(&S.q_full);
     }
     const uint32_t base = tmem + w * 256 + ((uint32_t)(32 * (warp & 3)) << 16);
-    float m = -INFINITY, l = 0.f;  // the base b is m - kTcBits
+    float O[kHeadDim];
+#pragma unroll
+    for (int i = 0; i < kHeadDim; i++) O[i] = 0.f;
+    float m = -INFINITY, l = 0.f;  // the base b is m - kPBits
     for (int j = w; j < nblk; j += 2) {
-      const int nkey = k1 - k0 - j * kTcBlock;
-      // S is there, and with it the warpgroup's last O (the commit covers what was issued before)
       if (!dead && !tc_wait(&S.s_full[w], (j >> 1) & 1, &S.err)) dead = true;
       // the block's valid keys: every page whole, but at the end of the prefix (or beside a bad page)
       if (!dead && !tc_wait(&S.v_full[w], (j >> 1) & 1, &S.err)) dead = true;
-      bool whole = nkey >= kTcBlock;
+      bool whole = true;
 #pragma unroll
       for (int g = 0; g < 8; g++) whole &= S.nv[w][g] == kPage;
       tc_fence_after();
-      uint32_t v[4][32];
+      // scores 64 at a time, twice: the maximum, then the weights
+      auto scores = [&](int half, uint32_t (&v)[2][32]) {
+        tmem_ld32(base + 64 * half, v[0]);
+        tmem_ld32(base + 64 * half + 32, v[1]);
+        tmem_wait_ld();
+        if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) tmem_ld32(base + 32 * i, v[i]);
-      tmem_wait_ld();
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int d = 0; d < 32; d++)
-            if (d % kPage >= S.nv[w][2 * i + d / kPage]) v[i][d] = __float_as_uint(-INFINITY);
-      }
-      float mx[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        mx[i] = __uint_as_float(v[i][0]);
-#pragma unroll
-        for (int d = 1; d < 32; d++) mx[i] = fmaxf(mx[i], __uint_as_float(v[i][d]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (j < 2) {
-        m = top;
-      } else {
-        const bool up = top > m + kTcSlack;
-        if (__any_sync(0xffffffffu, up)) {
-          const float f = up && m != -INFINITY ? ex2(m - top) : 1.f;
-          l *= f;
-          if (up) m = top;
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            uint32_t o[32];
-            tmem_ld32(base + 128 + 32 * i, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int d = 0; d < 32; d++) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
-            tmem_st32(base + 128 + 32 * i, o);
-          }
+          for (int i = 0; i < 64; i++)
+            if (i % kPage >= S.nv[w][4 * half + i / kPage]) v[i / 32][i % 32] = __float_as_uint(-INFINITY);
         }
+      };
+      float top = m;
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        uint32_t v[2][32];
+        scores(half, v);
+        float mx[2] = {__uint_as_float(v[0][0]), __uint_as_float(v[1][0])};
+#pragma unroll
+        for (int d = 1; d < 32; d++) {
+          mx[0] = fmaxf(mx[0], __uint_as_float(v[0][d]));
+          mx[1] = fmaxf(mx[1], __uint_as_float(v[1][d]));
+        }
+        top = fmaxf(top, fmaxf(mx[0], mx[1]));
       }
-      const float b = m == -INFINITY ? 0.f : m - kTcBits;
+      const float corr = m == -INFINITY ? 0.f : ex2(m - top), b = top == -INFINITY ? 0.f : top - kPBits;
+      m = top;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        uint32_t o[32];
+      for (int half = 0; half < 2; half++) {
+        uint32_t v[2][32];
+        scores(half, v);
 #pragma unroll
-        for (int d = 0; d < 16; d++) {
-          const float x = ex2(__uint_as_float(v[i][2 * d]) - b), y = ex2(__uint_as_float(v[i][2 * d + 1]) - b);
-          s0 += x;
-          s1 += y;
-          split2(x, y, o[d], o[16 + d]);
+        for (int i = 0; i < 2; i++) {
+          uint32_t o[32];
+#pragma unroll
+          for (int d = 0; d < 16; d++) {
+            const float x = ex2(__uint_as_float(v[i][2 * d]) - b), y = ex2(__uint_as_float(v[i][2 * d + 1]) - b);
+            s0 += x;
+            s1 += y;
+            split2(x, y, o[d], o[16 + d]);
+          }
+          tmem_st32(base + 64 * half + 32 * i, o);
         }
-        tmem_st32(base + 32 * i, o);
       }
-      l += s0 + s1;
+      l = l * corr + (s0 + s1);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&S.p_full[w]);
+      // the block's O, while the next scores are made (p_full of the next block lets O be overwritten)
+      if (!dead && !tc_wait(&S.o_full[w], (j >> 1) & 1, &S.err)) dead = true;
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        uint32_t v[2][32];
+        tmem_ld32(base + 128 + 64 * i, v[0]);
+        tmem_ld32(base + 128 + 64 * i + 32, v[1]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int d = 0; d < 64; d++) O[64 * i + d] = fmaf(O[64 * i + d], corr, __uint_as_float(v[d / 32][d % 32]));
+      }
     }
     // ---- the two warpgroups' parts of a row joined: each gives half of its pieces, adds up the other half
-    const int lastj = nblk - 1 - ((nblk - 1 - w) & 1);  // the warpgroup's last block
-    const bool has = w < nblk;
-    if (has && !dead && !tc_wait(&S.o_full[w], (lastj >> 1) & 1, &S.err)) dead = true;
-    tc_fence_after();
     float* mine = w ? S.m1 : S.m0;
     mine[r] = m;
     mine[128 + r] = l;
@@ -868,47 +866,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
     const float f = m == -INFINITY ? 0.f : ex2(m - mm);
     float4* ex = reinterpret_cast<float4*>(kvs) + r;  // [giver][16 pieces][128 rows]
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      uint32_t o[32];
-      if (has) {
-        tmem_ld32(base + 128 + 64 * (w ^ 1) + 32 * i, o);
-        tmem_wait_ld();
-      }
-#pragma unroll
-      for (int d = 0; d < 8; d++) {
-        const float* x = reinterpret_cast<const float*>(o) + 4 * d;
-        ex[(16 * w + 8 * i + d) * 128] = has ? make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+    for (int i = 0; i < 16; i++) {
+      float4 y;
+      if (w) y = make_float4(O[4 * i] * f, O[4 * i + 1] * f, O[4 * i + 2] * f, O[4 * i + 3] * f);
+      else y = make_float4(O[64 + 4 * i] * f, O[65 + 4 * i] * f, O[66 + 4 * i] * f, O[67 + 4 * i] * f);
+      ex[(16 * w + i) * 128] = y;
     }
     asm volatile("bar.sync 2, 256;" ::: "memory");
     if (tile * 128 + r < p.rows) {
       const size_t at = part_row(a, split, kvh, tile * 128 + r);
       if (w == 0) {
-        a.pm[at] = mm - kTcBits;
+        a.pm[at] = mm - kPBits;
         a.pl[at] = l * f + (mo == -INFINITY ? 0.f : lo * ex2(mo - mm));
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      uint32_t o[32];
-      if (has) {
-        tmem_ld32(base + 128 + 64 * w + 32 * i, o);
-        tmem_wait_ld();
-      }
-      if (tile * 128 + r < p.rows) {
-        const size_t at = part_at(part_row(a, split, kvh, tile * 128 + r), 16 * w + 8 * i);
-#pragma unroll
-        for (int d = 0; d < 8; d++) {
-          const float* x = reinterpret_cast<const float*>(o) + 4 * d;
-          float4 y = ex[(16 * (w ^ 1) + 8 * i + d) * 128];
-          if (has) {
-            y.x += x[0] * f;
-            y.y += x[1] * f;
-            y.z += x[2] * f;
-            y.w += x[3] * f;
-          }
-          a.po[at + 8 * d] = y;
+      for (int i = 0; i < 16; i++) {
+        float4 y = ex[(16 * (w ^ 1) + i) * 128];
+        if (w) {
+          y.x += O[64 + 4 * i] * f;
+          y.y += O[65 + 4 * i] * f;
+          y.z += O[66 + 4 * i] * f;
+          y.w += O[67 + 4 * i] * f;
+        } else {
+          y.x += O[4 * i] * f;
+          y.y += O[4 * i + 1] * f;
+          y.z += O[4 * i + 2] * f;
+          y.w += O[4 * i + 3] * f;
         }
+        a.po[part_at(at, 16 * w + i)] = y;
       }
     }
     tc_fence_before();
