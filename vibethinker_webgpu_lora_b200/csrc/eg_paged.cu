@@ -138,7 +138,6 @@ void launch_append(const AppendArgs& a, long long heads, cudaStream_t st) {
 // [16-byte piece][row % 8]: a thread a row writes whole sectors, and so does a
 // group of 8 rows.
 constexpr float kPBits = 14.f;
-constexpr int kWarps = 4;       // warps of a CTA, each with its own 16-key tiles
 constexpr int kSoPitch = kHeadDim + 4;  // floats a row of the warps' outputs in shared memory
 constexpr int kSms = 148;       // plans are made for the B200's SM count
 
@@ -240,7 +239,11 @@ template <typename KVT>
 struct WarpTile {
   static constexpr int kRow = kHeadDim * (int)sizeof(KVT);  // bytes of a staged row
   static constexpr int kBytes = 2 * kPage * kRow;           // K and V of one tile
-  static constexpr int kStages = 2;
+  // warps of a CTA, each with its own tiles, and how many a warp stages: 64 KB for
+  // f16 (three CTAs an SM); 128 KB for f32, whose warps compute longer, so twice
+  // the warps hide more than a second stage (17 x 1001: 18.7 us, 4 warps of 2 stages 20.5)
+  static constexpr bool kF32 = std::is_same<KVT, float>::value;
+  static constexpr int kWarps = kF32 ? 8 : 4, kStages = kF32 ? 1 : 2;
   static constexpr int kChunks = kRow / 16;
 };
 
@@ -303,9 +306,10 @@ __device__ __forceinline__ void v_frag(const unsigned char* st, int dt, uint32_t
 // each).  NG = 2, for the prefix alone and an f32 cache, halves the reads and
 // the splitting of K and V per row.
 template <typename KVT, int NG>
-__global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_constant__ SharedArgs a, int pref) {
+__global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel(const __grid_constant__ SharedArgs a, int pref) {
   using W = WarpTile<KVT>;
-  constexpr bool F32 = std::is_same<KVT, float>::value;
+  constexpr bool F32 = W::kF32;
+  constexpr int kWarps = W::kWarps;
   extern __shared__ __align__(128) unsigned char sm[];
   __shared__ float sm_m[kWarps][8 * NG], sm_l[kWarps][8 * NG];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
@@ -398,9 +402,12 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
 
   int stage = 0;
   for (int t = warp; t < ntile; t += kWarps) {
-    const int nv_next = issue(t + kWarps, page_next, stage ^ 1);
-    page_next = page_at(t + 2 * kWarps);
-    cp_async_wait<1>();
+    int nv_next = 0;
+    if (W::kStages == 2) {
+      nv_next = issue(t + kWarps, page_next, stage ^ 1);
+      page_next = page_at(t + 2 * kWarps);
+    }
+    cp_async_wait<W::kStages - 1>();
     __syncwarp();
     const unsigned char* ks_ = st + stage * W::kBytes;
     const unsigned char* vs_ = ks_ + kPage * W::kRow;
@@ -468,8 +475,12 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
       }
     }
     __syncwarp();
+    if (W::kStages == 1) {
+      nv_next = issue(t + kWarps, page_next, stage);
+      page_next = page_at(t + 2 * kWarps);
+    }
     nv_cur = nv_next;
-    stage ^= 1;
+    stage ^= W::kStages - 1;
   }
   cp_async_wait<0>();
 #pragma unroll
@@ -1017,8 +1028,9 @@ template <typename KVT, int NG>
 cudaError_t launch_warps(const SharedArgs& a, long long blocks, int pref, bool early, cudaStream_t st) {
   static OncePerDevice once;
   void* args[2] = {const_cast<SharedArgs*>(&a), &pref};
-  return launch_pdl((const void*)attn_shared_kernel<KVT, NG>, once, (unsigned)blocks, 32 * kWarps,
-                    kWarps * WarpTile<KVT>::kStages * WarpTile<KVT>::kBytes, early, args, st);
+  using W = WarpTile<KVT>;
+  return launch_pdl((const void*)attn_shared_kernel<KVT, NG>, once, (unsigned)blocks, 32 * W::kWarps,
+                    W::kWarps * W::kStages * W::kBytes, early, args, st);
 }
 
 template <typename KVT>
