@@ -336,6 +336,60 @@ def test_shared_prefix_two_streams_two_workspaces(cuda):
     b.check(range(0, 11, 5))
 
 
+def relative(s, seqs):
+    torch.cuda.synchronize()
+    got = s.d["out"].cpu().numpy().astype(np.float64).reshape(len(s.lens), s.nh, HD)
+    want = np.stack([s.want(b)[0] for b in seqs])
+    return np.linalg.norm(got[list(seqs)] - want) / np.linalg.norm(want)
+
+
+def test_shared_prefix_long_suffixes_of_many(cuda):
+    """A few long sequences among many: the parts stay short (a running sum on
+    the tensor cores loses 2^-24.5 a step; 1024 keys over 4 warps are 32 steps,
+    a score 16: together below 8e-6 of the output, where one part of 32768 keys
+    would lose 2e-5)."""
+    n, longest = 300, 32768
+    lens = [longest if i in (17, 170) else i % 40 for i in range(n)]
+    s = Shared(cuda, 20, lens[:2] + [longest], 16, 2, "f16", seed=5)  # one long run of pages, used by both
+    pages = np.tile(s.pages[2], (n, 1))
+    s.pages, s.lens = pages, lens
+    rng = np.random.default_rng(6)
+    s.q = rng.standard_normal((n, 16 * HD)).astype(np.float32)
+    s.d.update(q=torch.from_numpy(s.q).to(cuda), pages=i32(pages, cuda), lens=i32(lens, cuda),
+               out=torch.zeros(n, 16 * HD, device=cuda),
+               ws=torch.empty(K.attn_shared_prefix_bytes(n, 16, 2, 20, longest), dtype=torch.uint8, device=cuda))
+    K.attn_shared_prefix(**s.d)
+    err = relative(s, [17, 170])
+    print("relative error", err)
+    assert err < 8e-6
+    s.check([0, 16, 17, 18, 299])
+
+
+@pytest.mark.parametrize("size", [1e-4, 30.0])
+@pytest.mark.parametrize("n", [2, 40])
+def test_shared_prefix_keys_of_any_size(cuda, n, size):
+    """Keys of an f32 cache far below 1 under queries as far above it, and the other way round."""
+    s = Shared(cuda, 800, [60] * n, 16, 2, "f32", seed=17)
+    s.kc *= np.float32(size)
+    s.q /= np.float32(size)
+    s.d["k_cache"].copy_(torch.from_numpy(s.kc.reshape(s.d["k_cache"].shape)))
+    s.d["q"].copy_(torch.from_numpy(s.q[:, :16 * HD]))
+    K.attn_shared_prefix(**s.d)
+    assert relative(s, range(0, n, max(1, n // 5))) < 8e-6
+
+
+@pytest.mark.parametrize("n", [2, 40])
+@pytest.mark.parametrize("size", [1e-6, 1e-3, 300.0])
+def test_shared_prefix_values_of_any_size(cuda, n, size):
+    """An f32 cache's small or large values keep their precision: hi and lo
+    parts to 2^-22, or 2^-36 where that is more; the scores' part as above."""
+    s = Shared(cuda, 800, [60] * n, 16, 2, "f32", seed=7)
+    s.vc *= np.float32(size)
+    s.d["v_cache"].copy_(torch.from_numpy(s.vc.reshape(s.d["v_cache"].shape)))
+    K.attn_shared_prefix(**s.d)
+    assert relative(s, range(0, n, max(1, n // 5))) < 8e-6 + 2.0 ** -36 / size * 2
+
+
 @pytest.mark.parametrize("kv,n,prefix,longest", [("f16", 40, 4000, 100), ("f16", 9, 300, 40), ("f32", 30, 1100, 50)])
 def test_shared_prefix_captured(cuda, kv, n, prefix, longest):
     """One capture, replayed over other lengths, pages and queries, gives the

@@ -217,9 +217,10 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   }
   p.n_pref = (prefix_len + p.pref_keys - 1) / p.pref_keys;
   // suffix: about four CTAs an SM, 128 keys a split at least (64 sequences x up to
-  // 1024 keys 12.6 us in splits of 256, 14.9 of 128, 20.2 of 1024)
+  // 1024 keys 12.6 us in splits of 256, 14.9 of 128, 20.2 of 1024), 1024 at most
+  // as above
   const int pairs = nseq * nkv * p.gch, want = std::max(1, 4 * kSms / pairs);
-  p.suf_keys = std::max(128, round_up((max_len + want - 1) / want, 64));
+  p.suf_keys = std::min(1024, std::max(128, round_up((max_len + want - 1) / want, 64)));
   p.n_suf = (max_len + p.suf_keys - 1) / p.suf_keys;
   return p;
 }
@@ -234,7 +235,10 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 // S^T = K q^T and O^T = V^T p^T as mma.sync m16n8k16 (16 keys or dims x 8
 // rows), so the 8 query heads of a group fill the n side exactly.  q and p are
 // f16 hi + lo pairs (two products); with an f32 cache K and V are split too
-// (three products, the lo.lo one left out: 2^-22 of the product).
+// (three products, the lo.lo one left out: 2^-22 of the product).  lo parts of
+// q, K and V are lifted by 2^11 (split_lifted): an f16 holds them to 2^-36 then,
+// not 2^-25, which small values would feel.  The scores sum theirs apart; V's
+// meets p hi lowered by 2^-11.
 template <typename KVT>
 struct WarpTile {
   static constexpr int kRow = kHeadDim * (int)sizeof(KVT);  // bytes of a staged row
@@ -271,6 +275,15 @@ __device__ __forceinline__ void tile_load(unsigned char* st, const SharedArgs& a
   }
 }
 
+// (x, y) = hi + 2^-11 lo, each an f16 pair
+constexpr float kLift = 2048.f;
+__device__ __forceinline__ void split_lifted(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = h2_bits(h);
+  lo = h2_bits(__floats2half2_rn((x - f.x) * kLift, (y - f.y) * kLift));
+}
+
 // (16 keys x 16 dims at dim 16 ks) as A fragments, hi and (f32 cache) lo
 __device__ __forceinline__ void k_frag(const unsigned char* st, int ks, uint32_t (&h)[4], uint32_t (&)[4], __half) {
   const int lane = threadIdx.x & 31, i = lane >> 3, r = (lane & 7) + 8 * (i & 1);
@@ -282,7 +295,7 @@ __device__ __forceinline__ void k_frag(const unsigned char* st, int ks, uint32_t
   for (int i = 0; i < 4; i++) {
     const int r = g + 8 * (i & 1), d = 16 * ks + 8 * (i >> 1) + 2 * tq;
     const float2 x = *reinterpret_cast<const float2*>(st + tile_off<float>(r, d >> 2) + (d & 3) * 4);
-    split2(x.x, x.y, h[i], l[i]);
+    split_lifted(x.x, x.y, h[i], l[i]);
   }
 }
 // (16 dims at 16 dt x 16 keys) of V^T as A fragments
@@ -297,7 +310,7 @@ __device__ __forceinline__ void v_frag(const unsigned char* st, int dt, uint32_t
     const int d = 16 * dt + g + 8 * (i & 1), r = 8 * (i >> 1) + 2 * tq;
     const float x = *reinterpret_cast<const float*>(st + tile_off<float>(r, d >> 2) + (d & 3) * 4);
     const float y = *reinterpret_cast<const float*>(st + tile_off<float>(r + 1, d >> 2) + (d & 3) * 4);
-    split2(x, y, h[i], l[i]);
+    split_lifted(x, y, h[i], l[i]);
   }
 }
 
@@ -387,7 +400,7 @@ __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         const float2 x = on ? __ldg(reinterpret_cast<const float2*>(q + 16 * ks + 8 * j)) : make_float2(0.f, 0.f);
-        split2(x.x * c, x.y * c, qh[n][ks][j], ql[n][ks][j]);
+        split_lifted(x.x * c, x.y * c, qh[n][ks][j], ql[n][ks][j]);
       }
   }
   float O[NG][8][4];
@@ -427,14 +440,14 @@ __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel
         if (F32) mma16816(S2[n], fl, qh[n][ks][0], qh[n][ks][1]);
       }
     }
-    uint32_t ph[NG][2], pl[NG][2];
+    uint32_t ph[NG][2], pl[NG][2], pd[NG][2];  // p hi, p lo, p hi 2^-11
     float c0[NG], c1[NG];
     const bool v0 = g < nv_cur, v1 = g + 8 < nv_cur;
 #pragma unroll
     for (int n = 0; n < NG; n++) {
       // keys g (S[0], S[1]) and g + 8 (S[2], S[3]) for rows 2 tq, 2 tq + 1
-      const float s0 = v0 ? S[n][0] + S2[n][0] : -INFINITY, s1 = v0 ? S[n][1] + S2[n][1] : -INFINITY;
-      const float s2 = v1 ? S[n][2] + S2[n][2] : -INFINITY, s3 = v1 ? S[n][3] + S2[n][3] : -INFINITY;
+      const float s0 = v0 ? fmaf(S2[n][0], 1.f / kLift, S[n][0]) : -INFINITY, s1 = v0 ? fmaf(S2[n][1], 1.f / kLift, S[n][1]) : -INFINITY;
+      const float s2 = v1 ? fmaf(S2[n][2], 1.f / kLift, S[n][2]) : -INFINITY, s3 = v1 ? fmaf(S2[n][3], 1.f / kLift, S[n][3]) : -INFINITY;
       float n0 = fmaxf(s0, s2), n1 = fmaxf(s1, s3);
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1) {
@@ -458,6 +471,7 @@ __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel
       for (int j = 0; j < 2; j++) {
         ph[n][j] = movmatrix(ph[n][j]);
         pl[n][j] = movmatrix(pl[n][j]);
+        if (F32) pd[n][j] = h2_bits(__hmul2(*reinterpret_cast<const __half2*>(&ph[n][j]), __float2half2_rn(1.f / kLift)));
       }
     }
 #pragma unroll
@@ -471,7 +485,7 @@ __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel
         O[n][j][3] *= c1[n];
         mma16816(O[n][j], fh, ph[n][0], ph[n][1]);
         mma16816(O[n][j], fh, pl[n][0], pl[n][1]);
-        if (F32) mma16816(O[n][j], fl, ph[n][0], ph[n][1]);
+        if (F32) mma16816(O[n][j], fl, pd[n][0], pd[n][1]);
       }
     }
     __syncwarp();

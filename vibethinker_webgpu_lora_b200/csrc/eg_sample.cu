@@ -325,7 +325,7 @@ struct __align__(16) FastSmem {
 struct Bins {
   float xmax, width, inv_width, inv_t;  // width has 12 significant bits: r * width is exact for every bin r
   bool poly;                            // steps of x / t up to 1/16: e^-u by its series
-  double step;                          // width / t
+  double step, inv_td;                  // width / t, 1 / t
 };
 
 // A candidate's place (xmax - x) / width; its bin is the nearest integer.
@@ -356,8 +356,12 @@ __device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
     return kBins - 1;
   }
   const float r = (p + kRound) - kRound;
-  const float u = bin_rest(B, x, r);
-  q = B.poly ? (1u << kQBits) - q_short(u) : (uint32_t)__double2ll_rn(exp(-(double)u) * (double)(1 << kQBits));
+  if (B.poly) {
+    q = (1u << kQBits) - q_short(bin_rest(B, x, r));
+  } else {  // u up to 1: in 64 bits, f32 would leave 2^-23 of the weight
+    const double u = ((double)B.xmax - (double)x - (double)r * B.width) * B.inv_td;
+    q = (uint32_t)__double2ll_rn(exp(-u) * (double)(1 << kQBits));
+  }
   return (int)r;
 }
 
@@ -824,7 +828,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     B.width = __uint_as_float((__float_as_uint(w) + 0xfff) & ~0xfffu);
     B.inv_width = 1.f / B.width;
     B.inv_t = (float)(1.0 / P.t);
-    B.step = (double)B.width / P.t;
+    B.inv_td = 1.0 / P.t;
+    B.step = (double)B.width * B.inv_td;
     B.poly = B.step <= 0.0625;
   }
   FastSmem* L = cl.map_shared_rank(&S, 0);
