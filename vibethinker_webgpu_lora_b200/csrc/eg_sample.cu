@@ -63,9 +63,13 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs& a, int row) {
   return q;
 }
 
+// One copy of the 64-bit exponential: inlined at each use it crowds the
+// registers of the passes and the instruction cache.
+__device__ __noinline__ double exp64(double x) { return exp(x); }
+
 // w of a candidate; an infinite maximum takes all the mass
 __device__ __forceinline__ double weight(float x, float xmax, double t) {
-  return x == xmax ? 1.0 : exp(((double)x - (double)xmax) / t);
+  return x == xmax ? 1.0 : exp64(((double)x - (double)xmax) / t);
 }
 
 struct Cut {  // a leading part of the order: its size, its mass, its last token's key and place among equal keys
@@ -325,7 +329,7 @@ struct __align__(16) FastSmem {
 struct Bins {
   float xmax, width, inv_width, inv_t;  // width has 12 significant bits: r * width is exact for every bin r
   bool poly;                            // steps of x / t up to 1/16: e^-u by its series
-  double step, inv_td;                  // width / t, 1 / t
+  double step;                          // width / t
 };
 
 // A candidate's place (xmax - x) / width; its bin is the nearest integer.
@@ -359,15 +363,15 @@ __device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
   if (B.poly) {
     q = (1u << kQBits) - q_short(bin_rest(B, x, r));
   } else {  // u up to 1: in 64 bits, f32 would leave 2^-23 of the weight
-    const double u = ((double)B.xmax - (double)x - (double)r * B.width) * B.inv_td;
-    q = (uint32_t)__double2ll_rn(exp(-u) * (double)(1 << kQBits));
+    const double u = ((double)B.xmax - (double)x - (double)r * B.width) * (B.step / B.width);
+    q = (uint32_t)__double2ll_rn(exp64(-u) * (double)(1 << kQBits));
   }
   return (int)r;
 }
 
 // The weight of q = 1 in bin b; units[j]: of bin j (4 of them).
 __device__ __forceinline__ double bin_unit(const Bins& B, const double* units, int b) {
-  return exp(-(double)(b & ~3) * B.step) * units[b & 3];
+  return exp64(-(double)(b & ~3) * B.step) * units[b & 3];
 }
 // sums over the warps before this one and over all, of one value a warp in shared memory
 template <int kThreads, typename T>
@@ -828,14 +832,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     B.width = __uint_as_float((__float_as_uint(w) + 0xfff) & ~0xfffu);
     B.inv_width = 1.f / B.width;
     B.inv_t = (float)(1.0 / P.t);
-    B.inv_td = 1.0 / P.t;
-    B.step = (double)B.width * B.inv_td;
+    B.step = (double)B.width / P.t;
     B.poly = B.step <= 0.0625;
   }
   FastSmem* L = cl.map_shared_rank(&S, 0);
   bool wide = !none && !slow0 && !B.poly;  // the 64-bit form
   if (!none && !slow0) {
-    if (tid < 4) S.unit[tid] = exp(-(double)tid * B.step) * (1.0 / (1 << kQBits));
+    if (tid < 4) S.unit[tid] = exp64(-(double)tid * B.step) * (1.0 / (1 << kQBits));
     if (!wide)
       each([&](float4 v, int) {
         const float w[4] = {v.x, v.y, v.z, v.w};
@@ -851,7 +854,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       });
   }
   // bin_unit's factor for the leader's bins, while other CTAs count
-  const double e4 = rank == 0 && !none && !slow0 ? exp(-(double)((tid * (kBins / kThreads)) & ~3) * B.step) : 0.0;
+  const double e4 = rank == 0 && !none && !slow0 ? exp64(-(double)((tid * (kBins / kThreads)) & ~3) * B.step) : 0.0;
   const double cut_pos = rank == 0 && !none && !slow0 ? P.cut / B.step : 0.0;
   sync_row(cl, C);
   if (none || slow0) {  // the same in every CTA of the cluster
