@@ -288,6 +288,42 @@ def test_shared_prefix_bounds_read_on_the_device(cuda):
         assert s.d["err"].item() == 1
 
 
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("nh,nkv,n", [(8, 1, 3), (12, 1, 2), (2, 2, 5), (40, 8, 6)])
+@pytest.mark.parametrize("prefix,longest", [(0, 1), (0, 128), (129, 0), (0, 1000), (512, 512), (515, 513), (640, 130), (1024, 100)])
+def test_shared_prefix_of_few_splits(cuda, kv, nh, nkv, n, prefix, longest):
+    """1 to 9 splits: joined within a cluster up to 8, by a launch of their own from 9 on."""
+    lens = [longest, -1, 0, longest // 2, longest, min(3, longest)][:n]
+    s = Shared(cuda, prefix, lens, nh, nkv, kv, seed=nh + prefix, max_len=longest, extra=8)
+    K.attn_shared_prefix(**s.d)
+    s.check()
+    assert s.d["err"].item() == 0
+
+
+def test_shared_prefix_few_splits_of_both_streams_and_no_keys(cuda):
+    """Sequences that hold nothing get zeros; replays beside an eager call agree."""
+    s = Shared(cuda, 0, [0, 0, 40], 16, 2, "f16", max_len=300)
+    K.attn_shared_prefix(**s.d)
+    torch.cuda.synchronize()
+    assert (s.d["out"][:2] == 0).all()
+    s.check()
+    g = torch.cuda.CUDAGraph()
+    first = s.d["out"].clone()
+    with torch.cuda.graph(g):
+        K.attn_shared_prefix(**s.d)
+    side = torch.cuda.Stream()
+    b = Shared(cuda, 300, [17] * 9, 16, 2, "f32", seed=3)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        K.attn_shared_prefix(**b.d)
+    for _ in range(5):
+        s.d["out"].fill_(1)
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(first, s.d["out"])
+    b.check()
+
+
 def test_shared_prefix_nan_and_inf_stay_in_their_row(cuda):
     s = Shared(cuda, 100, [20] * 12, 16, 2, "f16")
     s.d["q"][3, 5] = float("nan")

@@ -5,6 +5,7 @@
 // kernels.js:1657-1911): pools [n_pages][16][nkv][128] of f16 or f32, row t of
 // a sequence at physical row pages[t / 16] * 16 + t % 16.  Page ids and
 // lengths live on the device, so a captured graph serves every step.
+#include <cooperative_groups.h>
 #include <cuda.h>
 #include <math.h>
 #include <algorithm>
@@ -146,6 +147,7 @@ struct SharedPlan {
   int rows, groups;    // nseq * G rows per KV head, in groups of 8
   int pref_keys, n_pref;  // keys per prefix split, splits
   int tc, row_tiles;   // prefix on the tcgen05 tensor cores, in tiles of 128 rows
+  int fused;           // everything in one launch, a cluster of all splits for each 8 rows of a sequence
   int own;             // prefix in a kernel of its own (tc, or f32 in CTAs of 16 rows)
   int suf_keys, n_suf;                // keys per suffix split, most splits of a sequence
 };
@@ -222,6 +224,16 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   const int pairs = nseq * nkv * p.gch, want = std::max(1, 4 * kSms / pairs);
   p.suf_keys = std::min(1024, std::max(128, round_up((max_len + want - 1) / want, 64)));
   p.n_suf = (max_len + p.suf_keys - 1) / p.suf_keys;
+  // up to 8 splits, few rows: one launch that joins them within a cluster, each
+  // sequence reading the prefix for itself (2 sequences x 256 keys 5.6 us, 6.8 with
+  // the combine's launch; 16 x (512 + 512) 7.4 and 8.2).  At most as many CTAs as
+  // find room at once in clusters of 8: two an SM in f16 (512 CTAs 13.3 us, 7.8 in
+  // two launches), three SMs of four in f32 (128 CTAs 13.9 and 8.4).  A single split
+  // without a prefix has nothing to join and reads nothing twice: any number (32
+  // sequences x 16 heads of their own x 128 keys 9.4 and 11.3).
+  const int splits = p.n_pref + p.n_suf;
+  p.fused = !p.own && splits >= 1 && splits <= 8 &&
+            ((splits == 1 && prefix_len == 0) || pairs * splits <= (kv_f16 ? 2 * kSms : kSms * 3 / 4));
   return p;
 }
 
@@ -245,7 +257,7 @@ struct WarpTile {
   static constexpr int kBytes = 2 * kPage * kRow;           // K and V of one tile
   // warps of a CTA, each with its own tiles, and how many a warp stages: 64 KB for
   // f16 (three CTAs an SM); 128 KB for f32, whose warps compute longer, so twice
-  // the warps hide more than a second stage (17 x 1001: 18.7 us, 4 warps of 2 stages 20.5)
+  // the warps hide more than a second stage (17 x 1001: 19.2 us, 4 warps of 2 stages 1.8 more)
   static constexpr bool kF32 = std::is_same<KVT, float>::value;
   static constexpr int kWarps = kF32 ? 8 : 4, kStages = kF32 ? 1 : 2;
   static constexpr int kChunks = kRow / 16;
@@ -317,14 +329,18 @@ __device__ __forceinline__ void v_frag(const unsigned char* st, int dt, uint32_t
 // CTA = one split of the keys for up to 8 NG rows of one KV head.  Blocks
 // [0, pref) take the prefix, the others the suffixes (8 rows of a sequence
 // each).  NG = 2, for the prefix alone and an f32 cache, halves the reads and
-// the splitting of K and V per row.
-template <typename KVT, int NG>
+// the splitting of K and V per row.  FUSED: a cluster's CTAs are all splits of 8
+// rows of one sequence, the prefix's first, and join their parts through each
+// other's shared memory: one launch, for few splits.  Every CTA of a cluster
+// reaches both of its barriers; none leaves before the others have read its parts.
+template <typename KVT, int NG, bool FUSED>
 __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel(const __grid_constant__ SharedArgs a, int pref) {
   using W = WarpTile<KVT>;
   constexpr bool F32 = W::kF32;
   constexpr int kWarps = W::kWarps;
   extern __shared__ __align__(128) unsigned char sm[];
   __shared__ float sm_m[kWarps][8 * NG], sm_l[kWarps][8 * NG];
+  __shared__ float part_m[FUSED ? 8 : 1], part_l[FUSED ? 8 : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const SharedPlan& p = a.p;
   const int G = p.G;
@@ -334,7 +350,27 @@ __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel
   int kvh, row0, nrow, k0, k1, split, kmax;
   const uint32_t* table;
   int blk = blockIdx.x;
-  if (blk < pref) {
+  if (FUSED) {
+    const int c = p.n_pref + p.n_suf;
+    split = blk % c;
+    blk /= c;
+    const int gc = blk % p.gch;
+    blk /= p.gch;
+    kvh = blk % a.nkv;
+    const int b = blk / a.nkv;
+    row0 = b * G + 8 * gc;
+    nrow = min(8, G - 8 * gc);
+    k1 = a.lens[b];
+    if (split < p.n_pref) {
+      table = a.prefix_pages;
+      k0 = split * p.pref_keys;
+      kmax = min(a.prefix_len, k0 + p.pref_keys);
+    } else {
+      table = a.pages + (size_t)b * a.max_pages;
+      k0 = (split - p.n_pref) * p.suf_keys;
+      kmax = min(a.max_len, k0 + p.suf_keys);
+    }
+  } else if (blk < pref) {
     const int ng = (p.groups + NG - 1) / NG, rg = blk % ng;
     blk /= ng;
     kvh = blk % a.nkv;
@@ -362,7 +398,11 @@ __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel
   }
   auto page_at = [&](int t) -> uint32_t { return k0 + t * kPage < kmax ? __ldg(table + k0 / kPage + t) : 0u; };
   const uint32_t page0 = page_at(warp), page1 = page_at(warp + kWarps);
-  if ((int)blockIdx.x >= pref) {
+  const int len = k1;  // suffixes: the sequence's own keys
+  if (FUSED) {
+    if (k1 > a.max_len && a.err && threadIdx.x == 0) *a.err = 1;
+    k1 = split < p.n_pref ? kmax : max(k0, min(k1, kmax));
+  } else if ((int)blockIdx.x >= pref) {
     if (k1 > a.max_len && a.err && threadIdx.x == 0) *a.err = 1;
     k1 = min(k1, kmax);
     if (k0 >= k1) {
@@ -526,7 +566,7 @@ __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel
   __syncthreads();
   for (int i = threadIdx.x; i < 8 * NG * 32; i += 32 * kWarps) {
     const int r = (i & 7) + (i >> 8) * 8, c = (i >> 3) & 31;
-    if (r >= nrow) continue;
+    if (r >= nrow) continue;  // FUSED: piece c of row r is read and written by this thread alone
     float mm = sm_m[0][r];
 #pragma unroll
     for (int w = 1; w < kWarps; w++) mm = fmaxf(mm, sm_m[w][r]);
@@ -542,12 +582,58 @@ __global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel
       o.z += f * x.z;
       o.w += f * x.w;
     }
+    if (FUSED) {
+      reinterpret_cast<float4*>(so + r * kSoPitch)[c] = o;
+      if (c == 0) part_m[r] = mm, part_l[r] = l;
+      continue;
+    }
     const size_t at = part_row(a, split, kvh, row0 + r);
     if (c == 0) {
       a.pm[at] = mm - kPBits;
       a.pl[at] = l;
     }
     a.po[part_at(at, c)] = o;
+  }
+  if (FUSED) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    // rows of this CTA: rank, rank + C, ...; 4 rows x 32 pieces at a time
+    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), c = threadIdx.x & 31;
+    for (int r = rank + C * warp; r < nrow && len >= 0; r += C * kWarps) {
+      float mm[8], ls[8];
+      float4 x[8];
+#pragma unroll
+      for (int s = 0; s < 8; s++) {
+        mm[s] = -INFINITY;
+        if (s < C) {
+          mm[s] = *cl.map_shared_rank(&part_m[r], s);
+          ls[s] = *cl.map_shared_rank(&part_l[r], s);
+          x[s] = *cl.map_shared_rank(reinterpret_cast<float4*>(so + r * kSoPitch) + c, s);
+        }
+      }
+      float m = mm[0];
+#pragma unroll
+      for (int s = 1; s < 8; s++) m = fmaxf(m, mm[s]);
+      float l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < 8; s++)
+        if (s < C) {
+          const float f = mm[s] == -INFINITY ? 0.f : exp2f(mm[s] - m);
+          l += f * ls[s];
+          o.x += f * x[s].x;
+          o.y += f * x[s].y;
+          o.z += f * x[s].z;
+          o.w += f * x[s].w;
+        }
+      const float inv = l != 0.f ? 1.f / l : 0.f;  // no key at all: zeros
+      const int rr = row0 + r;
+      reinterpret_cast<float4*>(a.out + (long long)(rr / G) * a.ldo + (kvh * G + rr % G) * kHeadDim)[c] =
+          make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
+    cl.sync();  // the parts are read
+    return;
   }
   // the suffixes, launched beside the prefix's own kernel, whose results they do
   // not need: their end waits for that kernel's, so that the combine, which
@@ -993,7 +1079,7 @@ __global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant
 // The launches of one call: the prefix kernel (tcgen05), the suffix kernel
 // beside it, the combine after both.
 cudaError_t launch_pdl(const void* fn, OncePerDevice& once, unsigned blocks, int threads, int smem, bool early, void** args,
-                       cudaStream_t st) {
+                       cudaStream_t st, int cluster = 1) {
   int dev = 0;
   cudaError_t e = smem > 48 << 10 ? cudaGetDevice(&dev) : cudaSuccess;
   if (e == cudaSuccess && smem > 48 << 10 && once.first(dev)) {
@@ -1002,15 +1088,21 @@ cudaError_t launch_pdl(const void* fn, OncePerDevice& once, unsigned blocks, int
   }
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at = {};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
+  if (cluster > 1) {
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  } else {
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = &at;
-  cfg.numAttrs = early ? 1 : 0;
+  cfg.numAttrs = early || cluster > 1 ? 1 : 0;
   return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
@@ -1038,19 +1130,21 @@ cudaError_t page_map(CUtensorMap* map, const void* pool, const SharedArgs& a) {
              : cudaErrorInvalidValue;
 }
 
-template <typename KVT, int NG>
+template <typename KVT, int NG, bool FUSED = false>
 cudaError_t launch_warps(const SharedArgs& a, long long blocks, int pref, bool early, cudaStream_t st) {
   static OncePerDevice once;
   void* args[2] = {const_cast<SharedArgs*>(&a), &pref};
   using W = WarpTile<KVT>;
-  return launch_pdl((const void*)attn_shared_kernel<KVT, NG>, once, (unsigned)blocks, 32 * W::kWarps,
-                    W::kWarps * W::kStages * W::kBytes, early, args, st);
+  return launch_pdl((const void*)attn_shared_kernel<KVT, NG, FUSED>, once, (unsigned)blocks, 32 * W::kWarps,
+                    W::kWarps * W::kStages * W::kBytes, early, args, st, FUSED ? a.p.n_pref + a.p.n_suf : 1);
 }
 
 template <typename KVT>
 cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
   static OncePerDevice tc_once, no_smem;
   cudaError_t e = cudaSuccess;
+  if (a.p.fused)
+    return launch_warps<KVT, 1, true>(a, (long long)a.nseq * a.nkv * a.p.gch * (a.p.n_pref + a.p.n_suf), 0, false, st);
   const int pref = a.p.n_pref * a.nkv * (a.p.own ? (a.p.groups + 1) / 2 : a.p.groups);
   if (a.p.tc) {
     CUtensorMap km, vm;
