@@ -648,6 +648,21 @@ def test_sample_extreme_temperatures(cuda):
             check_sample(x, got, probs, t, 0, 1.0, 0.0, r)
 
 
+@pytest.mark.parametrize("spread", [1e-3, 0.3, 4.0, 50.0])
+@pytest.mark.parametrize("offset", [0.0, -0.49, 0.02, 100.0, -1e4, 3e5, -2.0 ** 24])
+def test_sample_offsets_of_the_logits(cuda, spread, offset):
+    """Maxima below, above and near 0, and far above the spread, where neighbouring
+    logits are few or one f32 step apart; a bin's middle must not round."""
+    rng = np.random.default_rng(31)
+    x = (rng.standard_normal((6, 20011)) * spread + offset).astype(np.float32)
+    x[3, ::3] = -np.inf
+    x[4, 1:] = np.minimum(x[4, 1:], np.float32(offset))
+    r = np.array([0.01, 0.3, 0.5, 0.8, 0.97, 0.9999], np.float32)
+    for t, k, p, m in [(1.0, 0, 1.0, 0.0), (spread, 0, 0.9, 0.0), (0.25 * spread, 300, 0.95, 0.02), (3 * spread, 0, 1.0, 0.3)]:
+        got, probs = run_sample(cuda, x, t, k, p, m, r)
+        check_sample(x, got, probs, t, k, p, m, r)
+
+
 def test_sample_extreme_values(cuda):
     big = np.finfo(np.float32).max
     x = np.zeros((6, 500), np.float32)

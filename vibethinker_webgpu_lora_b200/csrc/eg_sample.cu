@@ -274,10 +274,13 @@ __device__ __noinline__ void sample_generic(const SampleArgs& a, int row, Generi
 // 2^-26 q e^(-b step): b its bin, q = 2^26 e^-u an integer, u its distance from
 // the bin's middle.  The histogram holds each bin's count and sum of q; in the
 // usual form q stays within 2^26 +- 2^22 and two 32-bit shared-memory atomics
-// take the count and the part of q above 2^26 - 2^22 (below 2^23: 512 tokens of
-// a CTA in one bin cannot overflow it; rows with more, or with steps of x / t
-// above 1/16, are counted again with 64-bit atomics, which cost three times as
-// much).  The leader CTA turns the merged bins into running counts and masses,
+// take the count and, modulo 2^32, the bits of kRound + q - 2^26: with the count
+// they give the sum of q above 2^26 - 2^22 (below 2^23 each: 512 tokens of a CTA
+// in one bin cannot overflow it; rows with more, or with steps of x / t above
+// 1/16, are counted again with 64-bit atomics, which cost three times as much).
+// The two atomics, 4 cycles of an SM each for a warp, bound the pass (38,000
+// tokens a CTA: 5.2 us).  The leader CTA turns the merged bins into running
+// counts and masses,
 // which fix each filter's and the sample's bin; only the tokens of those few
 // bins are gathered and put in order, in the same integers.
 // Tokens past the last bin (64 below the maximum in x / t or more) weigh
@@ -295,10 +298,13 @@ constexpr uint32_t kQBase = (1u << kQBits) - (1u << 22);
 constexpr uint32_t kDense = 512;   // tokens of a CTA in one bin, at most, in the usual form
 constexpr unsigned long long kCountOne = 1ull << 46;
 constexpr float kRound = 12582912.f;  // 1.5 2^23: x + kRound rounds |x| < 2^22 to an integer in the low bits
+constexpr uint32_t kRoundBits = 0x4B400000u;
+constexpr uint32_t kPartBase = kRoundBits - (1u << 22);  // of a token's part of a sum, what q - kQBase does not hold
 
 struct Ranges {  // bins [lo, hi] of: top-k, top-p, min-p, the sample (lo > hi: none)
   int lo[4], hi[4], redo;
-  float from[4], to[4];  // the same as windows of values, a little wide: the sample, top-p, top-k, min-p
+  int n;                // the same as n windows |x - mid| <= half of values, a little wide
+  float mid[4], half[4];
 };
 
 struct __align__(16) FastSmem {
@@ -326,32 +332,31 @@ struct __align__(16) FastSmem {
   uint32_t n_p, n_m;
 };
 
+// Bin r's middle is top - r width.  In the usual form top (the maximum, rounded
+// up) and width are multiples of 2^-24 of a power of two above every middle, so
+// each middle is an f32 without rounding.
 struct Bins {
-  float xmax, width, inv_width, inv_t;  // width has 12 significant bits: r * width is exact for every bin r
-  bool poly;                            // steps of x / t up to 1/16: e^-u by its series
-  double step;                          // width / t
+  float xmax, top, width, inv_width, inv_t;
+  bool poly;          // steps of x / t up to 1/16: e^z by its series
+  double step, lead;  // width / t, (top - xmax) / t
 };
 
-// A candidate's place (xmax - x) / width; its bin is the nearest integer.
-__device__ __forceinline__ float bin_place(const Bins& B, float x) { return __fmul_rn(B.xmax - x, B.inv_width); }
-__device__ __forceinline__ bool in_range(float p) { return p < (float)(kBins - 2) + 0.5f; }
-// u of a candidate in bin r: d + dl = xmax - x exactly (two-term sum), d - r
-// width exactly, then one rounding of each operation: right to 2^-23 of u.
-__device__ __forceinline__ float bin_rest(const Bins& B, float x, float r) {
-  const float d = B.xmax - x;
-  const float bb = d - B.xmax;
-  const float dl = (B.xmax - (d - bb)) - (x + bb);
-  return __fmul_rn(__fadd_rn(fmaf(-r, B.width, d), dl), B.inv_t);  // |u| <= step / 2 (a little more by place's rounding)
-}
-// 2^26 (1 - e^-u), rounded, for |u| <= 1/32: u (1 - u (1/2 - u (1/6 - u (1/24
-// - u / 120)))), the next term below 2^-39; fused as written, so that every
-// caller gets the same integer
-__device__ __forceinline__ int q_short(float u) {
-  float y = fmaf(-u, 1.f / 120.f, 1.f / 24.f);
-  y = fmaf(-u, y, 1.f / 6.f);
-  y = fmaf(-u, y, 0.5f);
-  y = fmaf(-u, y, 1.f);
-  return __float_as_int(fmaf(__fmul_rn(u, (float)(1 << kQBits)), y, kRound)) - __float_as_int(kRound);
+// kRound + a candidate's bin, the integer nearest (top - x) / width
+__device__ __forceinline__ float bin_place(const Bins& B, float x) { return fmaf(B.top - x, B.inv_width, kRound); }
+__device__ __forceinline__ bool in_range(float place) { return place <= kRound + (kBins - 2); }
+__device__ __forceinline__ int bin_index(float place) { return __float_as_int(place) - (int)kRoundBits; }
+// kRound + 2^26 (e^z - 1), rounded, of a candidate: z = (x - middle) / t, |z| <=
+// 1/32 (a little more by place's rounding).  x - middle and z are rounded once
+// each, so z is right to 2^-23; z (1 + z (1/2 + z (1/6 + z / 24))) leaves z^5 /
+// 120, 0.02 of 2^-26; fused as written, so that every caller gets the same
+// integer.
+__device__ __forceinline__ float bin_part(const Bins& B, float x, float place) {
+  constexpr float kOne = (float)(1 << kQBits);
+  const float z = __fmul_rn(__fsub_rn(x, fmaf(kRound - place, B.width, B.top)), B.inv_t);
+  float y = fmaf(z, kOne / 24.f, kOne / 6.f);
+  y = fmaf(z, y, kOne / 2.f);
+  y = fmaf(z, y, kOne);
+  return fmaf(z, y, kRound);
 }
 __device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
   const float p = bin_place(B, x);
@@ -359,14 +364,13 @@ __device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
     q = 0;
     return kBins - 1;
   }
-  const float r = (p + kRound) - kRound;
   if (B.poly) {
-    q = (1u << kQBits) - q_short(bin_rest(B, x, r));
+    q = (1u << kQBits) + __float_as_int(bin_part(B, x, p)) - (int)kRoundBits;
   } else {  // u up to 1: in 64 bits, f32 would leave 2^-23 of the weight
-    const double u = ((double)B.xmax - (double)x - (double)r * B.width) * (B.step / B.width);
+    const double u = ((double)B.top - (double)x - (double)(p - kRound) * B.width) * (B.step / B.width);
     q = (uint32_t)__double2ll_rn(exp64(-u) * (double)(1 << kQBits));
   }
-  return (int)r;
+  return bin_index(p);
 }
 
 // The weight of q = 1 in bin b; units[j]: of bin j (4 of them).
@@ -490,8 +494,8 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
         const uint2 v = *reinterpret_cast<const uint2*>(R->sum + tid * kPer + j);
         cnt[j] += n.x;
         cnt[j + 1] += n.y;
-        q[j] += (unsigned long long)n.x * kQBase + v.x;
-        q[j + 1] += (unsigned long long)n.y * kQBase + v.y;
+        q[j] += (unsigned long long)n.x * kQBase + (v.x - n.x * kPartBase);
+        q[j + 1] += (unsigned long long)n.y * kQBase + (v.y - n.y * kPartBase);
         most = max(most, max(n.x, n.y));
       }
     }
@@ -584,9 +588,17 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
     const int wl = tid == 0 ? min(S.cross[3], last) : tid == 1 ? p_lo : tid == 2 ? (k_on ? kb : 1) : m_lo;
     const int wh = tid == 0 ? min(S.cross[4], last) : tid == 1 ? p_hi : tid == 2 ? (k_on ? kb : 0) : m_hi;
     const double slack = 0.01 * B.width + 0x1p-21 * (fabs((double)B.xmax) + (wh + 1.0) * B.width);
-    const bool some = wl <= wh;
-    S.rg.from[tid] = some ? __double2float_rd((double)B.xmax - (wh + 0.5) * B.width - slack) : INFINITY;
-    S.rg.to[tid] = some ? __double2float_ru((double)B.xmax - (wl - 0.5) * B.width + slack) : -INFINITY;
+    const uint32_t vote = __ballot_sync(0xfu, wl <= wh);
+    const int at = __popc(vote & ((1u << tid) - 1));
+    if (wl <= wh) {
+      // x - mid is rounded in the pass: so are the ends here, and rounding keeps their order
+      const float from = __double2float_rd((double)B.top - (wh + 0.5) * B.width - slack);
+      const float to = __double2float_ru((double)B.top - (wl - 0.5) * B.width + slack);
+      const float mid = 0.5f * from + 0.5f * to;
+      S.rg.mid[at] = mid;
+      S.rg.half[at] = fmaxf(mid - from, to - mid);
+    }
+    if (tid == 0) S.rg.n = __popc(vote);
   }
   if (tid == 32) {
     Ranges& R = S.rg;
@@ -761,10 +773,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         f(i < e1 ? *reinterpret_cast<const float4*>(xs + (i - e0)) : none4, i);
       }
     } else if (vec) {
-      // eight tokens a thread, the next eight already on their way
+      // eight tokens a thread, the next eight already on their way; they pass L1 by
+      // (256 rows: 132 us, 137 through it)
       const int last = (e1 - e0) & ~3;  // up to here four at a time lie in the row
       const float4* x4 = reinterpret_cast<const float4*>(x + e0);
-      auto load = [&](int i) { return i < last ? __ldg(x4 + i / 4) : none4; };
+      auto load = [&](int i) {
+        float4 v = none4;
+        if (i < last)
+          asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                       : "l"(x4 + i / 4));
+        return v;
+      };
       int i = 4 * tid;
       float4 v0 = load(i), v1 = load(i + 4 * kThreads);
       for (int i0 = 0; i0 < last; i0 += 8 * kThreads, i += 8 * kThreads) {
@@ -790,10 +810,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   float mx = -INFINITY, mn = INFINITY;
   each([&](float4 v, int) {
     const float w[4] = {v.x, v.y, v.z, v.w};
+    const float least = fminf(fminf(v.x, v.y), fminf(v.z, v.w));
+    if (staged && least >= -1e30f) {  // no masked value among them
+      mx = fmaxf(fmaxf(fmaxf(mx, v.x), fmaxf(v.y, v.z)), v.w);
+      mn = fminf(mn, least);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      mx = fmaxf(mx, w[j] >= -1e30f ? w[j] : -INFINITY);
-      mn = fminf(mn, w[j] >= -1e30f ? w[j] : INFINITY);
+      for (int j = 0; j < 4; j++) {
+        mx = fmaxf(mx, w[j] >= -1e30f ? w[j] : -INFINITY);
+        mn = fminf(mn, w[j] >= -1e30f ? w[j] : INFINITY);
+      }
     }
   });
 #pragma unroll
@@ -827,35 +853,41 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     // the range: all candidates, but at most 64 in x and 64 in x / t (whichever is more, steps of at most 2)
     const double cap = fmax(64.0 * P.t, fmin(64.0, 2.0 * (kBins - 2) * P.t));
     const double range = fmin((double)mx - (double)mn, cap);
-    const float w = (float)fmax(range / (kBins - 2), 1e-30);  // equal logits: one bin
+    const float w = (float)fmax(range / (kBins - 4), 1e-30);  // equal logits: one bin
+    // 2^-24 of the power of two above |mx| + 2044 w and what rounding adds: 2046 width
+    // is at most 1.001 of 2044 w and 2^-13 of that power
+    const float all = (float)((fabs((double)mx) + (kBins - 4.0) * w) * 1.002);
+    const float grid = __uint_as_float((__float_as_uint(all) & 0x7f800000u) - (23u << 23));
     B.xmax = mx;
-    B.width = __uint_as_float((__float_as_uint(w) + 0xfff) & ~0xfffu);
+    B.width = ceilf(w / grid) * grid;
     B.inv_width = 1.f / B.width;
     B.inv_t = (float)(1.0 / P.t);
     B.step = (double)B.width / P.t;
     B.poly = B.step <= 0.0625;
+    B.top = B.poly ? ceilf(mx / grid) * grid : mx;  // at most grid <= width above: t / 16
+    B.lead = ((double)B.top - (double)mx) / P.t;
   }
   FastSmem* L = cl.map_shared_rank(&S, 0);
   bool wide = !none && !slow0 && !B.poly;  // the 64-bit form
   if (!none && !slow0) {
-    if (tid < 4) S.unit[tid] = exp64(-(double)tid * B.step) * (1.0 / (1 << kQBits));
+    if (tid < 4) S.unit[tid] = exp64(B.lead - (double)tid * B.step) * (1.0 / (1 << kQBits));
+    const uint32_t bins0 = (uint32_t)__cvta_generic_to_shared(S.cnt) - kRoundBits * 4;
     if (!wide)
       each([&](float4 v, int) {
         const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float p = bin_place(B, w[j]), pr = p + kRound;
-          if (in_range(p)) {
-            const int b = __float_as_int(pr) - __float_as_int(kRound);
-            atomicAdd(&S.sum[b], (uint32_t)((1 << 22) - q_short(bin_rest(B, w[j], pr - kRound))));
-            atomicAdd(&S.cnt[b], 1u);
-          }
+          const float p = bin_place(B, w[j]);
+          if (in_range(p))
+            asm volatile("red.shared.add.u32 [%0], 1;\n\tred.shared.add.u32 [%0 + %2], %1;"
+                         ::"r"(bins0 + __float_as_uint(p) * 4), "r"(__float_as_uint(bin_part(B, w[j], p))), "n"(4 * kBins)
+                         : "memory");  // cnt and sum of the bin
         }
       });
   }
   // bin_unit's factor for the leader's bins, while other CTAs count
   const double e4 = rank == 0 && !none && !slow0 ? exp64(-(double)((tid * (kBins / kThreads)) & ~3) * B.step) : 0.0;
-  const double cut_pos = rank == 0 && !none && !slow0 ? P.cut / B.step : 0.0;
+  const double cut_pos = rank == 0 && !none && !slow0 ? (P.cut + B.lead) / B.step : 0.0;
   sync_row(cl, C);
   if (none || slow0) {  // the same in every CTA of the cluster
     if (rank == 0) {
@@ -903,9 +935,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       if (tid == 0) S.rg = L->rg;
       __syncthreads();
     }
-    const float from0 = S.rg.from[0], to0 = S.rg.to[0], from1 = S.rg.from[1], to1 = S.rg.to[1];
-    const float from2 = S.rg.from[2], to2 = S.rg.to[2], from3 = S.rg.from[3], to3 = S.rg.to[3];
-    const bool more = from2 <= to2 || from3 <= to3;
+    const int windows = S.rg.n;
+    float mid[4], half[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) mid[j] = j < windows ? S.rg.mid[j] : 0.f, half[j] = j < windows ? S.rg.half[j] : -1.f;
     // a warp's hits go to its own part of a list of ids: no atomics in the pass
     // (staged: 16-bit offsets; either way a run of kList neighbours finds room)
     const uint32_t room = (staged ? kStagedHits : kHits) / (kThreads / 32);
@@ -914,13 +947,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     uint32_t* hits32 = reinterpret_cast<uint32_t*>(hits) + warp * room;
     const uint32_t below = (1u << lane) - 1;
     uint32_t nh = 0;
-    auto inside = [&](float v) {
-      bool hit = ((v >= from0) & (v <= to0)) | ((v >= from1) & (v <= to1));
-      if (more) hit |= ((v >= from2) & (v <= to2)) | ((v >= from3) & (v <= to3));
-      return hit;
-    };
     each([&](float4 v, int i) {
-      const bool hit[4] = {inside(v.x), inside(v.y), inside(v.z), inside(v.w)};
+      const float w[4] = {v.x, v.y, v.z, v.w};
+      bool hit[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) hit[j] = (fabsf(w[j] - mid[0]) <= half[0]) | (fabsf(w[j] - mid[1]) <= half[1]);
+      if (windows > 2)
+#pragma unroll
+        for (int j = 0; j < 4; j++) hit[j] = hit[j] | (fabsf(w[j] - mid[2]) <= half[2]) | (fabsf(w[j] - mid[3]) <= half[3]);
       if (__any_sync(0xffffffffu, hit[0] | hit[1] | hit[2] | hit[3])) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -944,7 +978,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         id = staged ? e0 + hits16[k0 + lane] : hits32[k0 + lane];
         v = staged ? xs[id - e0] : __ldg(x + id);
         const float p = bin_place(B, v);
-        const int b = __float_as_int(p + kRound) - __float_as_int(kRound);  // as bin_of, where in_range
+        const int b = bin_index(p);  // as bin_of, where in_range
 #pragma unroll
         for (int j = 0; j < 4; j++) in |= b >= S.rg.lo[j] && b <= S.rg.hi[j];
         in &= in_range(p);
@@ -979,17 +1013,26 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   // ---- the gathered tokens in falling order
   unsigned long long* list = S.list;
   if (nl <= kCountMost) {
-    // a few: each is compared with all, eight threads a token
+    // a few: each is compared with all, eight threads for every two tokens (a key
+    // loaded is compared twice: the loads' bytes bound this)
     list = reinterpret_cast<unsigned long long*>(xs) + kList * 3 / 2;  // behind the two arrays below
-    constexpr int kPart = 8;
+    constexpr int kPart = 8, kApart = kThreads / kPart;
     const int part = tid & (kPart - 1);
-    for (int e = tid / kPart; e < (nl + 31) / 32 * 32; e += kThreads / kPart) {
-      const unsigned long long me = e < nl ? S.list[e] : 0;
-      int place = 0;
-      for (int f = part; f < nl; f += kPart) place += S.list[f] > me;
+    for (int e = tid / kPart; e < (nl + 31) / 32 * 32; e += 2 * kApart) {
+      const unsigned long long me0 = e < nl ? S.list[e] : 0, me1 = e + kApart < nl ? S.list[e + kApart] : 0;
+      int at0 = 0, at1 = 0;
+      for (int f = part; f < nl; f += kPart) {
+        const unsigned long long u = S.list[f];
+        at0 += u > me0;
+        at1 += u > me1;
+      }
 #pragma unroll
-      for (int o = 1; o < kPart; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
-      if (part == 0 && e < nl) list[place] = me;
+      for (int o = 1; o < kPart; o <<= 1) {
+        at0 += __shfl_xor_sync(0xffffffffu, at0, o);
+        at1 += __shfl_xor_sync(0xffffffffu, at1, o);
+      }
+      if (part == 0 && e < nl) list[at0] = me0;
+      if (part == 0 && e + kApart < nl) list[at1] = me1;
     }
     __syncthreads();
   } else {
@@ -1005,12 +1048,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 }
 
 // CTAs of a row's cluster: as many as leave every CTA an SM of its own, with
-// slices of 4096 tokens or longer (32 rows of 151936: 4 CTAs a row 34 us, 8 39;
-// 64 rows: 2 51, 8 71; 256 rows: 1 133, 8 243); clusters of 8, which do not fill
-// the GPCs' SMs, for up to 8 rows.
+// slices of 4096 tokens or longer (32 rows of 151936, top-p: 4 CTAs a row 38 us, 2
+// 45, 8 62; 64 rows: 2 45, 4 49; 256 rows: 1 114, 2 134); clusters of 8, which do
+// not fill the GPCs' SMs, for up to 12 rows (12 rows: 8 CTAs a row 28 us, 4 33; 16
+// rows: 44 and 37).
 int cluster_size(int rows, int n) {
   int c = 1;
-  while (c < 8 && 2LL * rows * c <= (c == 4 ? 64 : 128) && n / (2 * c) >= 4096) c *= 2;
+  while (c < 8 && 2LL * rows * c <= (c == 4 ? 96 : 128) && n / (2 * c) >= 4096) c *= 2;
   return c;
 }
 
