@@ -290,7 +290,7 @@ def test_shared_prefix_bounds_read_on_the_device(cuda):
 
 @pytest.mark.parametrize("kv", ["f16", "f32"])
 @pytest.mark.parametrize("nh,nkv,n", [(8, 1, 3), (12, 1, 2), (2, 2, 5), (40, 8, 6)])
-@pytest.mark.parametrize("prefix,longest", [(0, 1), (0, 128), (129, 0), (0, 1000), (512, 512), (515, 513), (640, 130), (1024, 100)])
+@pytest.mark.parametrize("prefix,longest", [(0, 1), (0, 128), (129, 0), (0, 1000), (512, 512), (515, 513), (640, 130), (1024, 100), (2048, 640), (30, 2048), (2000, 1900)])
 def test_shared_prefix_of_few_splits(cuda, kv, nh, nkv, n, prefix, longest):
     """1 to 9 splits: joined within a cluster up to 8, by a launch of their own from 9 on."""
     lens = [longest, -1, 0, longest // 2, longest, min(3, longest)][:n]

@@ -231,9 +231,23 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   // two launches), three SMs of four in f32 (128 CTAs 13.9 and 8.4).  A single split
   // without a prefix has nothing to join and reads nothing twice: any number (32
   // sequences x 16 heads of their own x 128 keys 9.4 and 11.3).
+  const int limit = kv_f16 ? 2 * kSms : kSms * 3 / 4;
+  // f16: longer splits where that makes 8 of them (16 x 2048 + 640 in 384 keys 10.3
+  // us, 12.0 in 8 of 256 and 5 of 128 with the combine; few pairs, which leave SMs
+  // to more splits, gain up to 384: 2 x 2048 + 2048 in 512 9.9 and 9.3; f32 loses:
+  // 2 x 1024 + 1024 in 256 9.8 and 9.0)
+  if (kv_f16 && !p.own && p.n_pref + p.n_suf > 8 && pairs * 8 <= limit)
+    for (int keys = 64; keys <= (pairs >= 8 ? 512 : 384); keys += 64) {
+      const int np = (prefix_len + keys - 1) / keys, ns = (max_len + keys - 1) / keys;
+      if (np + ns > 8) continue;
+      p.pref_keys = p.suf_keys = keys;
+      p.n_pref = np;
+      p.n_suf = ns;
+      break;
+    }
   const int splits = p.n_pref + p.n_suf;
   p.fused = !p.own && splits >= 1 && splits <= 8 &&
-            ((splits == 1 && prefix_len == 0) || pairs * splits <= (kv_f16 ? 2 * kSms : kSms * 3 / 4));
+            ((splits == 1 && prefix_len == 0) || pairs * splits <= limit);
   return p;
 }
 
