@@ -300,6 +300,17 @@ def test_shared_prefix_of_few_splits(cuda, kv, nh, nkv, n, prefix, longest):
     assert s.d["err"].item() == 0
 
 
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("nh,nkv,lens,prefix", [(16, 2, [700], 9000), (4, 4, [0, 5000, -1], 4100), (28, 4, [130, 4000], 0),
+                                                (16, 2, [1, 300, 2600], 2300), (8, 1, [0], 20000)])
+def test_shared_prefix_of_many_splits(cuda, kv, nh, nkv, lens, prefix):
+    """17 to 70 splits of few rows: the combine's lanes, of which some have no split."""
+    s = Shared(cuda, prefix, lens, nh, nkv, kv, seed=prefix, extra=4)
+    K.attn_shared_prefix(**s.d)
+    s.check()
+    assert s.d["err"].item() == 0
+
+
 def test_shared_prefix_few_splits_of_both_streams_and_no_keys(cuda):
     """Sequences that hold nothing get zeros; replays beside an eager call agree."""
     s = Shared(cuda, 0, [0, 0, 40], 16, 2, "f16", max_len=300)

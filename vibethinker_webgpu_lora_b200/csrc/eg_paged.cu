@@ -149,6 +149,7 @@ struct SharedPlan {
   int tc, row_tiles;   // prefix on the tcgen05 tensor cores, in tiles of 128 rows
   int fused;           // everything in one launch, a cluster of all splits for each 8 rows of a sequence
   int own;             // prefix in a kernel of its own (tc, or f32 in CTAs of 16 rows)
+  int lanes;           // of the combine, which take the splits in turns of 8 (one: of 32)
   int suf_keys, n_suf;                // keys per suffix split, most splits of a sequence
 };
 
@@ -246,6 +247,7 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
       break;
     }
   const int splits = p.n_pref + p.n_suf;
+  p.lanes = splits > 16 && nkv * p.groups <= kSms ? 4 : 1;
   p.fused = !p.own && splits >= 1 && splits <= 8 &&
             ((splits == 1 && prefix_len == 0) || pairs * splits <= limit);
   return p;
@@ -1031,10 +1033,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
 // One CTA per 8 rows of a KV head, a thread per (row, 16-byte piece): 32 splits
 // at a time, their weights by thread (row, split) through shared memory, eight
 // of a row's parts in flight.
-__global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant__ SharedArgs a) {
-  __shared__ float sb[32][8], sl[32][8];
+// kLanes groups of 256 threads take the splits in turns and join at the end: few
+// rows with many splits wait for one round of loads after the other (1 sequence,
+// 8192 keys in 64 splits: 4 lanes 10.8 us, one 13.3; 64 x 8192 28.8 and 30.1).
+template <int kLanes>
+__global__ void __launch_bounds__(256 * kLanes) attn_shared_combine(const __grid_constant__ SharedArgs a) {
+  constexpr int kC = 32 / kLanes;  // splits of a lane's turn
+  __shared__ float sb[kLanes][kC][8], sl[kLanes][kC][8];
   const int kvh = blockIdx.x / a.p.groups, row0 = blockIdx.x % a.p.groups * 8;
-  const int rr = threadIdx.x & 7, c = threadIdx.x >> 3, r = row0 + rr, G = a.p.G;
+  const int q = threadIdx.x >> 8, t = threadIdx.x & 255, rr = t & 7, c = t >> 3, r = row0 + rr, G = a.p.G;
   const int b = r / G, len = r < a.p.rows ? __ldg(a.lens + b) : -1;
   const bool on = len >= 0;  // a padding sequence's row stays as it is
   const int ns = on ? a.p.n_pref + (min(len, a.max_len) + a.p.suf_keys - 1) / a.p.suf_keys : 0;
@@ -1043,10 +1050,12 @@ __global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant
   pdl_wait();
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; __syncthreads_or(s0 < ns); s0 += 32) {
+  for (int s0 = kC * q; __syncthreads_or(s0 < ns); s0 += 32) {
     const int s = s0 + c;
-    sb[c][rr] = s < ns ? __ldcg(a.pm + row + s * step) : -INFINITY;
-    sl[c][rr] = s < ns ? __ldcg(a.pl + row + s * step) : 0.f;
+    if (c < kC) {
+      sb[q][c][rr] = s < ns ? __ldcg(a.pm + row + s * step) : -INFINITY;
+      sl[q][c][rr] = s < ns ? __ldcg(a.pl + row + s * step) : 0.f;
+    }
     float4 x[8];
 #pragma unroll
     for (int j = 0; j < 8; j++)
@@ -1054,10 +1063,12 @@ __global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant
     __syncthreads();
     float nm = m;
 #pragma unroll 8
-    for (int j = 0; j < 32; j++) nm = fmaxf(nm, sb[j][rr]);
+    for (int j = 0; j < kC; j++) nm = fmaxf(nm, sb[q][j][rr]);
     __syncthreads();
-    const float mine = sb[c][rr];
-    sb[c][rr] = mine == -INFINITY ? 0.f : exp2f(mine - nm);
+    if (c < kC) {
+      const float mine = sb[q][c][rr];
+      sb[q][c][rr] = mine == -INFINITY ? 0.f : exp2f(mine - nm);
+    }
     const float f = m == -INFINITY ? 0.f : exp2f(m - nm);
     m = nm;
     l *= f;
@@ -1066,7 +1077,7 @@ __global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant
     o.z *= f;
     o.w *= f;
     __syncthreads();
-    for (int j0 = 0; j0 < 32 && s0 + j0 < ns; j0 += 8) {
+    for (int j0 = 0; j0 < kC && s0 + j0 < ns; j0 += 8) {
       if (j0) {
 #pragma unroll
         for (int j = 0; j < 8; j++)
@@ -1075,13 +1086,36 @@ __global__ void __launch_bounds__(256) attn_shared_combine(const __grid_constant
 #pragma unroll
       for (int j = 0; j < 8; j++)
         if (s0 + j0 + j < ns) {
-          const float w = sb[j0 + j][rr];
-          l += w * sl[j0 + j][rr];
+          const float w = sb[q][j0 + j][rr];
+          l += w * sl[q][j0 + j][rr];
           o.x += w * x[j].x;
           o.y += w * x[j].y;
           o.z += w * x[j].z;
           o.w += w * x[j].w;
         }
+    }
+  }
+  if (kLanes > 1) {
+    __shared__ float4 so[kLanes][256];
+    __shared__ float sm[kLanes][256], ss[kLanes][256];
+    so[q][t] = o;
+    sm[q][t] = m;
+    ss[q][t] = l;
+    __syncthreads();
+    if (q) return;
+#pragma unroll
+    for (int i = 1; i < kLanes; i++) m = fmaxf(m, sm[i][t]);
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kLanes; i++) {
+      const float f = sm[i][t] == -INFINITY ? 0.f : exp2f(sm[i][t] - m);
+      const float4 x = so[i][t];
+      l += f * ss[i][t];
+      o.x += f * x.x;
+      o.y += f * x.y;
+      o.z += f * x.z;
+      o.w += f * x.w;
     }
   }
   if (!on) return;
@@ -1175,7 +1209,8 @@ cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
   if (e == cudaSuccess && blocks > 0) e = launch_warps<KVT, 1>(a, blocks, a.p.own ? 0 : pref, a.p.own, st);
   void* args[1] = {const_cast<SharedArgs*>(&a)};
   if (e == cudaSuccess)
-    e = launch_pdl((const void*)attn_shared_combine, no_smem, (unsigned)(a.nkv * a.p.groups), 256, 0, blocks > 0 || a.p.own, args, st);
+    e = launch_pdl(a.p.lanes > 1 ? (const void*)attn_shared_combine<4> : (const void*)attn_shared_combine<1>, no_smem,
+                   (unsigned)(a.nkv * a.p.groups), 256 * a.p.lanes, 0, blocks > 0 || a.p.own, args, st);
   return e;
 }
 
