@@ -150,6 +150,7 @@ struct SharedPlan {
   int fused;           // everything in one launch, a cluster of all splits for each 8 rows of a sequence
   int own;             // prefix in a kernel of its own (tc, or f32 in CTAs of 16 rows)
   int lanes;           // of the combine, which take the splits in turns of 8 (one: of 32)
+  int many;            // f32: 4 warps a CTA, two CTAs an SM
   int suf_keys, n_suf;                // keys per suffix split, most splits of a sequence
 };
 
@@ -192,11 +193,14 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   // What the prefix's scores number decides its kernel (16 heads, 2 KV heads):
   // f16 on the tensor cores from 900,000 on (16 sequences x 2048 14.6 us there,
   // 11.2 by warps; 16 x 4096 15.4 and 18.1; 64 x 1024 14.4 and 17.3); f32 in
-  // CTAs of 16 rows from 250,000 on (16 x 512 11.4 us there, 10.6 in CTAs of 8;
-  // 16 x 2048 19.3 and 24.0); below, the prefix and the suffixes share a launch.
+  // CTAs of 16 rows from 1,000,000 on; below, the prefix and the suffixes share a
+  // launch.  f32 takes 4 warps a CTA where there is work for them (16 x 512 9.4 us,
+  // 11.1 with 8; 64 x 8192 95 and 110; 4 x 32768 31 and 42; 2 x 8192 13.7 and 12.7).
   const long long scores = (long long)p.rows * nkv * prefix_len;
   p.tc = kv_f16 && prefix_len >= 256 && scores >= 900000;
-  p.own = p.tc || (!kv_f16 && p.groups > 2 && scores >= 250000);
+  p.many = !kv_f16 && ((p.groups * nkv >= 16 && scores + (long long)p.rows * nkv * max_len >= 138000) ||
+                       (p.groups > 2 && scores >= 1500000));
+  p.own = p.tc || (p.many && p.groups > 2 && scores >= 1000000);
   if (p.tc) {
     // one CTA an SM, about 5.5 us and 1.8 us a block of 128 keys: the number of
     // splits with the shortest rounds
@@ -209,13 +213,13 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
       if ((long long)units * n > 4 * kSms) break;
     }
   } else {
-    // two CTAs an SM (f32: one, 128 KB each): what is resident at once beside the
+    // two CTAs an SM (f32 of 8 warps: one): what is resident at once beside the
     // suffixes (16 x 2048 f16 11.2 us so, 13.9 with four an SM); never under 128
     // keys a split and never above 1024: the tensor core's f32 sums lose about
     // 2^-24.5 a step, all one way, so a warp's 16 tiles stay below 2^-20 (256
     // tiles of a 16384-key split: 1e-5)
     const long long units = (long long)(p.own ? (p.groups + 1) / 2 : p.groups) * nkv;
-    const long long want = std::max(1LL, (kv_f16 ? 2LL : 1LL) * kSms / units);
+    const long long want = std::max(1LL, (kv_f16 || p.many ? 2LL : 1LL) * kSms / units);
     p.pref_keys = std::min(1024, std::max(128, round_up((int)((prefix_len + want - 1) / want), 64)));
   }
   p.n_pref = (prefix_len + p.pref_keys - 1) / p.pref_keys;
@@ -248,7 +252,7 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
     }
   const int splits = p.n_pref + p.n_suf;
   p.lanes = splits > 16 && nkv * p.groups <= kSms ? 4 : 1;
-  p.fused = !p.own && splits >= 1 && splits <= 8 &&
+  p.fused = !p.own && !p.many && splits >= 1 && splits <= 8 &&
             ((splits == 1 && prefix_len == 0) || pairs * splits <= limit);
   return p;
 }
@@ -272,10 +276,11 @@ struct WarpTile {
   static constexpr int kRow = kHeadDim * (int)sizeof(KVT);  // bytes of a staged row
   static constexpr int kBytes = 2 * kPage * kRow;           // K and V of one tile
   // warps of a CTA, each with its own tiles, and how many a warp stages: 64 KB for
-  // f16 (three CTAs an SM); 128 KB for f32, whose warps compute longer, so twice
-  // the warps hide more than a second stage (17 x 1001: 19.2 us, 4 warps of 2 stages 1.8 more)
+  // f16 (three CTAs an SM).  f32, whose warps compute longer, gains more by warps
+  // than by a second stage: 64 KB in 4 warps, or 128 KB in 8 where there are few
+  // CTAs (the plan's choice)
   static constexpr bool kF32 = std::is_same<KVT, float>::value;
-  static constexpr int kWarps = kF32 ? 8 : 4, kStages = kF32 ? 1 : 2;
+  static constexpr int kStages = kF32 ? 1 : 2;
   static constexpr int kChunks = kRow / 16;
 };
 
@@ -349,11 +354,10 @@ __device__ __forceinline__ void v_frag(const unsigned char* st, int dt, uint32_t
 // rows of one sequence, the prefix's first, and join their parts through each
 // other's shared memory: one launch, for few splits.  Every CTA of a cluster
 // reaches both of its barriers; none leaves before the others have read its parts.
-template <typename KVT, int NG, bool FUSED>
-__global__ void __launch_bounds__(32 * WarpTile<KVT>::kWarps) attn_shared_kernel(const __grid_constant__ SharedArgs a, int pref) {
+template <typename KVT, int NG, int kWarps, bool FUSED>
+__global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_constant__ SharedArgs a, int pref) {
   using W = WarpTile<KVT>;
   constexpr bool F32 = W::kF32;
-  constexpr int kWarps = W::kWarps;
   extern __shared__ __align__(128) unsigned char sm[];
   __shared__ float sm_m[kWarps][8 * NG], sm_l[kWarps][8 * NG];
   __shared__ float part_m[FUSED ? 8 : 1], part_l[FUSED ? 8 : 1];
@@ -1178,21 +1182,22 @@ cudaError_t page_map(CUtensorMap* map, const void* pool, const SharedArgs& a) {
              : cudaErrorInvalidValue;
 }
 
-template <typename KVT, int NG, bool FUSED = false>
+template <typename KVT, int NG, int kWarps, bool FUSED = false>
 cudaError_t launch_warps(const SharedArgs& a, long long blocks, int pref, bool early, cudaStream_t st) {
   static OncePerDevice once;
   void* args[2] = {const_cast<SharedArgs*>(&a), &pref};
   using W = WarpTile<KVT>;
-  return launch_pdl((const void*)attn_shared_kernel<KVT, NG, FUSED>, once, (unsigned)blocks, 32 * W::kWarps,
-                    W::kWarps * W::kStages * W::kBytes, early, args, st, FUSED ? a.p.n_pref + a.p.n_suf : 1);
+  return launch_pdl((const void*)attn_shared_kernel<KVT, NG, kWarps, FUSED>, once, (unsigned)blocks, 32 * kWarps,
+                    kWarps * W::kStages * W::kBytes, early, args, st, FUSED ? a.p.n_pref + a.p.n_suf : 1);
 }
 
 template <typename KVT>
 cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
   static OncePerDevice tc_once, no_smem;
+  constexpr bool kF32 = WarpTile<KVT>::kF32;
   cudaError_t e = cudaSuccess;
   if (a.p.fused)
-    return launch_warps<KVT, 1, true>(a, (long long)a.nseq * a.nkv * a.p.gch * (a.p.n_pref + a.p.n_suf), 0, false, st);
+    return launch_warps<KVT, 1, kF32 ? 8 : 4, true>(a, (long long)a.nseq * a.nkv * a.p.gch * (a.p.n_pref + a.p.n_suf), 0, false, st);
   const int pref = a.p.n_pref * a.nkv * (a.p.own ? (a.p.groups + 1) / 2 : a.p.groups);
   if (a.p.tc) {
     CUtensorMap km, vm;
@@ -1203,10 +1208,12 @@ cudaError_t launch_shared(const SharedArgs& a, cudaStream_t st) {
       e = launch_pdl((const void*)attn_prefix_tc_kernel, tc_once, (unsigned)(a.p.n_pref * a.nkv * a.p.row_tiles), kTcThreads,
                      kTcSmem, false, args, st);
   } else if constexpr (std::is_same<KVT, float>::value) {
-    if (a.p.own) e = launch_warps<KVT, 2>(a, pref, pref, false, st);
+    if (a.p.own) e = launch_warps<KVT, 2, 4>(a, pref, pref, false, st);
   }
   const long long blocks = (a.p.own ? 0 : pref) + (long long)a.p.n_suf * a.nseq * a.nkv * a.p.gch;
-  if (e == cudaSuccess && blocks > 0) e = launch_warps<KVT, 1>(a, blocks, a.p.own ? 0 : pref, a.p.own, st);
+  if (e == cudaSuccess && blocks > 0)
+    e = kF32 && !a.p.many ? launch_warps<KVT, 1, kF32 ? 8 : 4>(a, blocks, a.p.own ? 0 : pref, a.p.own, st)
+                          : launch_warps<KVT, 1, 4>(a, blocks, a.p.own ? 0 : pref, a.p.own, st);
   void* args[1] = {const_cast<SharedArgs*>(&a)};
   if (e == cudaSuccess)
     e = launch_pdl(a.p.lanes > 1 ? (const void*)attn_shared_combine<4> : (const void*)attn_shared_combine<1>, no_smem,
