@@ -1225,6 +1225,10 @@ bool misaligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) &
 
 size_t shared_rows(const SharedPlan& p, int nkv) { return (size_t)(p.n_pref + p.n_suf) * nkv * p.groups * 8; }
 size_t shared_bytes(const SharedPlan& p, int nkv) { return shared_rows(p, nkv) * (kHeadDim + 2) * sizeof(float); }
+// what a call is asked for: enough for either cache type
+size_t shared_need(const SharedPlan& p, const SharedPlan& other, int nkv) {
+  return std::max<size_t>(16, std::max(shared_bytes(p, nkv), shared_bytes(other, nkv)));
+}
 
 const char* shared_dims(int nseq, int nh, int nkv, int prefix_len, int max_len) {
   if (nseq < 1 || nseq > 65536) return "need 1 <= nseq <= 65536";
@@ -1276,10 +1280,7 @@ EG_API eg_status eg_op_attn_shared_prefix_bytes(int nseq, int nh, int nkv, int p
                                                 uint64_t* bytes) {
   if (!bytes) return fail(EG_ERR_ARG, "attn_shared_prefix: null argument");
   if (const char* why = shared_dims(nseq, nh, nkv, prefix_len, max_len)) return fail(EG_ERR_ARG, "attn_shared_prefix: %s", why);
-  size_t n = 16;  // enough for either cache type
-  for (int f16 = 0; f16 < 2; f16++)
-    n = std::max(n, shared_bytes(shared_plan(nseq, nh, nkv, prefix_len, max_len, f16), nkv));
-  *bytes = n;
+  *bytes = shared_need(shared_plan(nseq, nh, nkv, prefix_len, max_len, 0), shared_plan(nseq, nh, nkv, prefix_len, max_len, 1), nkv);
   return EG_OK;
 }
 
@@ -1300,7 +1301,7 @@ EG_API eg_status eg_op_attn_shared_prefix(const float* q, int64_t ldq, int nseq,
     return fail(EG_ERR_ARG, "attn_shared_prefix: 16-byte aligned buffers required");
   SharedArgs a = {};
   a.p = shared_plan(nseq, nh, nkv, prefix_len, max_len, kv_f16);
-  const size_t need = shared_bytes(a.p, nkv);
+  const size_t need = shared_need(a.p, shared_plan(nseq, nh, nkv, prefix_len, max_len, !kv_f16), nkv);
   if (ws_bytes < need)
     return fail(EG_ERR_ARG, "attn_shared_prefix: workspace of %llu bytes, %llu needed", (unsigned long long)ws_bytes, (unsigned long long)need);
   a.q = q;
