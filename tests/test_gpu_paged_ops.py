@@ -290,7 +290,7 @@ def test_shared_prefix_bounds_read_on_the_device(cuda):
 
 @pytest.mark.parametrize("kv", ["f16", "f32"])
 @pytest.mark.parametrize("nh,nkv,n", [(8, 1, 3), (12, 1, 2), (2, 2, 5), (40, 8, 6)])
-@pytest.mark.parametrize("prefix,longest", [(0, 1), (0, 128), (129, 0), (0, 1000), (512, 512), (515, 513), (640, 130), (1024, 100), (2048, 640), (30, 2048), (2000, 1900)])
+@pytest.mark.parametrize("prefix,longest", [(0, 1), (0, 128), (129, 0), (0, 1000), (512, 512), (515, 513), (640, 130), (1024, 100), (2048, 640), (30, 2048), (2000, 1900), (896, 0), (600, 100), (700, 128)])
 def test_shared_prefix_of_few_splits(cuda, kv, nh, nkv, n, prefix, longest):
     """1 to 9 splits: joined within a cluster up to 8, by a launch of their own from 9 on."""
     lens = [longest, -1, 0, longest // 2, longest, min(3, longest)][:n]
@@ -563,7 +563,7 @@ def test_sample(cuda, kind, n):
         check_sample(x, got, probs, t, k, p, m, r)
 
 
-@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("rows", [1, 3, 12, 13, 40, 70])
 def test_sample_full_vocabulary(cuda, rows):
     n = 151936
     x = np.concatenate([rows_for(n, -(-rows // 2), 1, "flat"), rows_for(n, rows // 2, 2, "peaked")])
