@@ -1,0 +1,37 @@
+"""The paged serving operators at the ends of what they take: sizes of q and of
+the cache's values, lengths and counts (definitions: paged_ref.py)."""
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as R
+from test_gpu_paged_ops import check_sample
+from vibethinker_webgpu_lora_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- sampling
+@pytest.mark.parametrize("rows,n", [(65, 1 << 18), (65, 300000), (33, 1 << 19), (40, (1 << 19) - 1), (13, 1 << 20),
+                                    (20, (1 << 20) - 3), (70, 1 << 20)])
+@pytest.mark.parametrize("kind", ["equal", "half", "two thirds"])
+def test_sample_of_long_rows_of_equal_logits(cuda, rows, n, kind):
+    """Vocabularies up to the longest taken, with 2^18 equal logits and more in what
+    one CTA holds, alone or above lower ones: every row gets its id."""
+    rng = np.random.default_rng(n)
+    x = torch.zeros(rows, n, device=cuda)
+    if kind != "equal":
+        x -= torch.from_numpy((rng.random(n) < (0.5 if kind == "half" else 1 / 3)).astype(np.float32)).to(cuda)
+    r = rng.random(rows).astype(np.float32)
+    r[0], r[-1] = 0.0, 1.0
+    f = lambda v: torch.full((rows,), v, device=cuda)  # noqa: E731
+    some = sorted({0, 1, rows // 2, rows - 1})
+    host = x[some].cpu().numpy()
+    for k, p in ((0, 1.0), (n // 5, 1.0), (n - n // 7, 1.0), (0, 0.75)):
+        ids, probs = torch.full((rows,), -7, dtype=torch.int32, device=cuda), f(9.0)
+        K.sample_filtered(x, torch.from_numpy(r).to(cuda), ids, top_k=torch.full((rows,), k, dtype=torch.int32, device=cuda),
+                          top_p=f(p), probs=probs)
+        torch.cuda.synchronize()
+        assert ((ids >= 0) & (ids < (k if k and kind == "equal" else n))).all() and (probs < 1e-4).all()
+        got, share = ids.cpu().numpy().view(np.uint32), probs.cpu().numpy().astype(np.float64)
+        check_sample(host, got[some], share[some], 1.0, k, p, 0.0, r[some])

@@ -297,6 +297,9 @@ constexpr int kQBits = 26;
 constexpr uint32_t kQBase = (1u << kQBits) - (1u << 22);
 constexpr uint32_t kDense = 512;   // tokens of a CTA in one bin, at most, in the usual form
 constexpr unsigned long long kCountOne = 1ull << 46;
+constexpr int kSliceMost = (1 << 18) - 1;  // tokens of a CTA, at most: what a count above bit 46 holds
+// Tokens of each of a row's c CTAs, in whole 16-byte pieces.
+__host__ __device__ __forceinline__ int slice_of(int n, int c) { return ((n + c - 1) / c + 3) & ~3; }
 constexpr float kRound = 12582912.f;  // 1.5 2^23: x + kRound rounds |x| < 2^22 to an integer in the low bits
 constexpr uint32_t kRoundBits = 0x4B400000u;
 constexpr uint32_t kPartBase = kRoundBits - (1u << 22);  // of a token's part of a sum, what q - kQBase does not hold
@@ -312,7 +315,7 @@ struct __align__(16) FastSmem {
     struct {
       uint32_t cnt[kBins], sum[kBins];
     };
-    unsigned long long hist[kBins];  // 64-bit form: count << 46 | sum of q
+    unsigned long long hist[kBins];  // 64-bit form: count << 46 | sum of q, of kSliceMost tokens at most
     double above[kBins];             // then, in the leader, the mass above each bin
   };
   uint32_t count_above[kBins];
@@ -746,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float* x = a.logits + row * a.ld;
-  const int per = ((a.n + C - 1) / C + 3) & ~3, e0 = min(a.n, rank * per), e1 = min(a.n, e0 + per);
+  const int per = slice_of(a.n, C), e0 = min(a.n, rank * per), e1 = min(a.n, e0 + per);
   const RowParams P = row_params(a, row);
 
   if (staged) {  // 16 bytes a copy where the row allows it
@@ -1055,12 +1058,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 int cluster_size(int rows, int n) {
   int c = 1;
   while (c < 8 && 2LL * rows * c <= (c == 4 ? 96 : 128) && n / (2 * c) >= 4096) c *= 2;
+  while (slice_of(n, c) > kSliceMost) c *= 2;  // 8 hold the longest row, 2^20
   return c;
 }
 
 template <int kThreads>
 cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
-  const int per = ((a.n + c - 1) / c + 3) & ~3;
+  const int per = slice_of(a.n, c);
   const int staged = per <= ((long long)a.rows * c <= 148 ? kSliceAlone : kSlice);
   const size_t smem = sizeof(FastSmem) + std::max<size_t>(staged ? (size_t)per * 4 + kStagedHits * 2 : kHits * 4, kList * 12 + kCountMost * 8);
   static_assert(sizeof(FastSmem) + kSlice * 4 + kStagedHits * 2 <= 113 << 10, "two CTAs an SM");
