@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import paged_ref as R
-from test_gpu_paged_ops import check_sample
+from test_gpu_paged_ops import check_sample, run_sample
 from vibethinker_webgpu_lora_b200 import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +35,19 @@ def test_sample_of_long_rows_of_equal_logits(cuda, rows, n, kind):
         assert ((ids >= 0) & (ids < (k if k and kind == "equal" else n))).all() and (probs < 1e-4).all()
         got, share = ids.cpu().numpy().view(np.uint32), probs.cpu().numpy().astype(np.float64)
         check_sample(host, got[some], share[some], 1.0, k, p, 0.0, r[some])
+
+
+@pytest.mark.parametrize("t,share", [(1.13e-7, 0.9874), (1e-7, 0.9976), (2.2e-7, 0.1426), (5e-7, 0.0043)])
+def test_sample_steps_far_above_the_temperature(cuda, t, share):
+    """Temperatures below a step of f32: one best logit of 8 and 3,999 that
+    share the value 3 2^-21 below it, whose masses are far from 0 together.
+    Each row takes the best token up to its share of the mass, then the others."""
+    x = np.full((6, 4000), 8 - 3 * 2.0 ** -21, np.float32)
+    for i in range(6):
+        x[i, 667 * i] = 8.0
+    r = np.array([0.5, 0.9, share - 1e-3, share + 1e-3, 0.9999, 1.0], np.float32)
+    for k, p in ((0, 1.0), (2001, 1.0), (0, 0.98)):
+        got, probs = run_sample(cuda, x, t, k, p, 0.0, r)
+        if not k and p == 1 and share > 0.9:
+            assert abs(probs[0] - share) < 1e-4
+        check_sample(x, got, probs, t, k, p, 0.0, r)

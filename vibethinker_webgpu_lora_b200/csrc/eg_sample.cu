@@ -297,7 +297,7 @@ constexpr int kQBits = 26;
 constexpr uint32_t kQBase = (1u << kQBits) - (1u << 22);
 constexpr uint32_t kDense = 512;   // tokens of a CTA in one bin, at most, in the usual form
 constexpr unsigned long long kCountOne = 1ull << 46;
-constexpr int kSliceMost = (1 << 18) - 1;  // tokens of a CTA, at most: what a count above bit 46 holds
+constexpr int kSliceMost = (1 << 18) - 1;  // tokens of a CTA, at most: what a count above bit 46 holds, and q < 2^28 below it
 // Tokens of each of a row's c CTAs, in whole 16-byte pieces.
 __host__ __device__ __forceinline__ int slice_of(int n, int c) { return ((n + c - 1) / c + 3) & ~3; }
 constexpr float kRound = 12582912.f;  // 1.5 2^23: x + kRound rounds |x| < 2^22 to an integer in the low bits
@@ -369,7 +369,7 @@ __device__ __forceinline__ int bin_of(const Bins& B, float x, uint32_t& q) {
   }
   if (B.poly) {
     q = (1u << kQBits) + __float_as_int(bin_part(B, x, p)) - (int)kRoundBits;
-  } else {  // u up to 1: in 64 bits, f32 would leave 2^-23 of the weight
+  } else {  // |u| up to 1.26: in 64 bits, f32 would leave 2^-23 of the weight; q < 2^27.9
     const double u = ((double)B.top - (double)x - (double)(p - kRound) * B.width) * (B.step / B.width);
     q = (uint32_t)__double2ll_rn(exp64(-u) * (double)(1 << kQBits));
   }
@@ -863,10 +863,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     const float grid = __uint_as_float((__float_as_uint(all) & 0x7f800000u) - (23u << 23));
     B.xmax = mx;
     B.width = ceilf(w / grid) * grid;
+    // a grid far above t (t below a step of f32 at the maximum): steps of w, 2.01 t at
+    // most, off the grid, which the 64-bit form takes, but no step that lets q pass 2^28
+    const bool on_grid = B.width <= 2.5 * P.t;
+    if (!on_grid) B.width = w;
     B.inv_width = 1.f / B.width;
     B.inv_t = (float)(1.0 / P.t);
     B.step = (double)B.width / P.t;
-    B.poly = B.step <= 0.0625;
+    B.poly = on_grid && B.step <= 0.0625;
     B.top = B.poly ? ceilf(mx / grid) * grid : mx;  // at most grid <= width above: t / 16
     B.lead = ((double)B.top - (double)mx) / P.t;
   }
