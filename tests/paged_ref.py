@@ -58,6 +58,17 @@ def attention(q, k, v):
     return o, bound + 1e-30
 
 
+# The relative error (of all outputs together, in the 2-norm) that attention on
+# ordinary inputs (q 1.5 and keys 1 in size) may have.  The tensor core's f32 sums
+# are cut, not rounded: 2^-24 of the running sum a step on the average, all one
+# way.  Scores: 16 steps (24 for an f32 cache) of a sum whose size is 2.2 on the
+# average (in powers of 2): 24 2^-24 ln 2 2.2 = 2.2e-6 of a weight.  Outputs: at
+# most 48 steps of a part (16 tiles of three products), half of them on the
+# average: 1.4e-6.  The hi + lo pairs (2^-22 of a part, its sign random) and the
+# roundings of the sums in f32 add a few 2^-24.
+LIMIT = 4e-6
+
+
 def sample(x, t=1.0, k=0, p=1.0, minp=0.0, r=0.5):
     """(id, share of the mass kept) of one row of f32 logits; the parameters in 64 bits."""
     x = np.asarray(x, np.float32)

@@ -5,10 +5,11 @@ import pytest
 import torch
 
 import paged_ref as R
-from test_gpu_paged_ops import check_sample, run_sample
+from test_gpu_paged_ops import Shared, check_sample, relative, run_sample
 from vibethinker_webgpu_lora_b200 import kernels as K
 
 pytestmark = pytest.mark.gpu
+HD = R.HD
 
 
 # ---------------------------------------------------------------- sampling
@@ -51,3 +52,41 @@ def test_sample_steps_far_above_the_temperature(cuda, t, share):
         if not k and p == 1 and share > 0.9:
             assert abs(probs[0] - share) < 1e-4
         check_sample(x, got, probs, t, k, p, 0.0, r)
+
+
+# ---------------------------------------------------------------- attention
+def put(s, **kw):
+    """Host arrays of a case, changed, to the device."""
+    for name in kw:
+        setattr(s, name, kw[name])
+    shape = s.d["k_cache"].shape
+    s.d["k_cache"].copy_(torch.from_numpy(s.kc.reshape(shape)))
+    s.d["v_cache"].copy_(torch.from_numpy(s.vc.reshape(shape)))
+    s.d["q"].copy_(torch.from_numpy(s.q[:, :s.nh * HD]))
+
+
+@pytest.mark.parametrize("size", [0.01, 30.0, 100.0, 300.0, 8000.0])
+@pytest.mark.parametrize("n,prefix", [(2, 800), (40, 4000), (130, 1000)])
+def test_shared_prefix_f16_keys_of_any_size(cuda, n, prefix, size):
+    """Keys of an f16 cache far above 1 under queries as far below it, and the
+    other way round: the error is that of ordinary sizes (R.LIMIT)."""
+    s = Shared(cuda, prefix, [60] * n, 16, 2, "f16", seed=18)
+    put(s, kc=(s.kc.astype(np.float32) * np.float32(size)).astype(np.float16), q=s.q / np.float32(size))
+    K.attn_shared_prefix(**s.d)
+    err = relative(s, range(0, n, max(1, n // 5)))
+    print("relative error", err)
+    assert err < R.LIMIT
+
+
+@pytest.mark.parametrize("kv,n,prefix", [("f16", 2, 800), ("f16", 40, 4000), ("f32", 3, 500), ("f32", 40, 4000)])
+def test_shared_prefix_one_large_dimension(cuda, kv, n, prefix):
+    """One dimension of the keys 20,000 times the others, one of the queries as far below them."""
+    s = Shared(cuda, prefix, [60] * n, 16, 2, kv, seed=19)
+    s.kc[..., 7] = (np.sign(s.kc[..., 7]) * 20000).astype(s.kc.dtype)
+    q = s.q.reshape(n, 16, HD)
+    q[..., 7] *= 1e-4
+    put(s, q=q.reshape(n, -1))
+    K.attn_shared_prefix(**s.d)
+    err = relative(s, range(0, n, max(1, n // 5)))
+    print("relative error", err)
+    assert err < R.LIMIT

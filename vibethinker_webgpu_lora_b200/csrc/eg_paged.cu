@@ -688,6 +688,7 @@ struct TcSmem {
   int err;
   int nv[2][8];  // valid keys of each page of a stage's block
   float m0[256], m1[256];  // each warpgroup's bases and sums at the end
+  float unscale[128];      // of a row's scores
 };
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
@@ -889,7 +890,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
     // ------------------------------------------------ softmax, one thread a row
     const int w = warp >> 2, r = tid & 127;
     {
-      // q times log2(e) / sqrt(128) as f16 hi and lo: 8 rows x 4 float4 a load (full sectors)
+      // q times log2(e) / sqrt(128) as f16 hi and lo: 8 rows x 4 float4 a load (full sectors).
+      // A row is scaled by the power of two that brings its largest element to [2^14, 2^15),
+      // taken out of its scores again, so that its lo parts, of f16's 2^-24 steps, hold it to
+      // 2^-39 of that element: large keys under small queries cost no precision, and q has the
+      // range of f32.  (Unscaled: keys of 300 and queries of 0.005 gave an error of 4e-5.)
       const float c = 1.4426950408889634f * 0.08838834764831845f;
       float4 qx[16];
 #pragma unroll
@@ -900,10 +905,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
         for (int i = 0; i < 8; i++)
           qx[8 * g + i] = gr < p.rows ? __ldg(reinterpret_cast<const float4*>(q) + 4 * i + (lane >> 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+      float up[2];  // c and the row's scale
+#pragma unroll
+      for (int g = 0; g < 2; g++) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float4 v = qx[8 * g + i];
+          top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));  // the row's other pieces: lanes 8 apart
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        // 2^e, e at most 100: below 2^-86 nothing of q is felt
+        const int e = min(100, 14 + 127 - (int)(__float_as_uint(top * c) >> 23));
+        up[g] = c * __uint_as_float((uint32_t)(127 + e) << 23);
+        if (lane < 8) S.unscale[16 * warp + 8 * g + lane] = __uint_as_float((uint32_t)(127 - e) << 23);
+      }
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int rr = 16 * warp + (i & 8) + (lane & 7), f = 4 * (i & 7) + (lane >> 3);  // half a 16-byte chunk
         const float4 v = qx[i];
+        const float c = up[i >> 3];
         uint2 h, l;
         split2(v.x * c, v.y * c, h.x, l.x);
         split2(v.z * c, v.w * c, h.y, l.y);
@@ -919,6 +941,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
 #pragma unroll
     for (int i = 0; i < kHeadDim; i++) O[i] = 0.f;
     float m = -INFINITY, l = 0.f;  // the base b is m - kPBits
+    if (!tc_wait(&S.q_full, 0, &S.err)) dead = true;  // the other warps' S.unscale
+    const float us = S.unscale[r];
     for (int j = w; j < nblk; j += 2) {
       if (!dead && !tc_wait(&S.s_full[w], (j >> 1) & 1, &S.err)) dead = true;
       // the block's valid keys: every page whole, but at the end of the prefix (or beside a bad page)
@@ -949,7 +973,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
           mx[0] = fmaxf(mx[0], __uint_as_float(v[0][d]));
           mx[1] = fmaxf(mx[1], __uint_as_float(v[1][d]));
         }
-        top = fmaxf(top, fmaxf(mx[0], mx[1]));
+        top = fmaxf(top, us * fmaxf(mx[0], mx[1]));
       }
       const float corr = m == -INFINITY ? 0.f : ex2(m - top), b = top == -INFINITY ? 0.f : top - kPBits;
       m = top;
@@ -963,7 +987,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_prefix_tc_kernel(const __g
           uint32_t o[32];
 #pragma unroll
           for (int d = 0; d < 16; d++) {
-            const float x = ex2(__uint_as_float(v[i][2 * d]) - b), y = ex2(__uint_as_float(v[i][2 * d + 1]) - b);
+            const float x = ex2(fmaf(__uint_as_float(v[i][2 * d]), us, -b)), y = ex2(fmaf(__uint_as_float(v[i][2 * d + 1]), us, -b));
             s0 += x;
             s1 += y;
             split2(x, y, o[d], o[16 + d]);
