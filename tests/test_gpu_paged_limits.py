@@ -90,3 +90,20 @@ def test_shared_prefix_one_large_dimension(cuda, kv, n, prefix):
     err = relative(s, range(0, n, max(1, n // 5)))
     print("relative error", err)
     assert err < R.LIMIT
+
+
+@pytest.mark.parametrize("kv,n,prefix", [("f16", 2, 800), ("f16", 40, 4000), ("f32", 3, 500), ("f32", 40, 4000)])
+def test_shared_prefix_largest_queries(cuda, kv, n, prefix):
+    """|q| / 8 up to the f16 range's end, 2^19.  What is added to ordinary errors, over
+    sqrt(128): an f32 key of 1e-5 is held to 2^-36, evenly spread, which such a query makes
+    3.9e-7 of a score; the other queries' lo parts may be held to 2^-39 of the largest
+    (2^-23 each, 5.4e-7 of a score)."""
+    s = Shared(cuda, prefix, [60] * n, 16, 2, kv, seed=20)
+    s.kc[..., 5] = (s.kc[..., 5].astype(np.float32) * np.float32(1e-5)).astype(s.kc.dtype)
+    q = s.q.reshape(n, 16, HD)
+    q[..., 5] = np.sign(q[..., 5]) * 8 * 65504.0
+    put(s, q=q.reshape(n, -1))
+    K.attn_shared_prefix(**s.d)
+    err = relative(s, range(0, n, max(1, n // 5)))
+    print("relative error", err)
+    assert err < R.LIMIT + 7e-7

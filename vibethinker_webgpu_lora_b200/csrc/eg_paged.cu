@@ -454,7 +454,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
     const int r = row0 + 8 * n + g;
     const bool on = 8 * n + g < nrow;
     const float* q = a.q + (on ? (long long)(r / G) * a.ldq + (kvh * G + r % G) * kHeadDim : 0) + 2 * tq;
-    const float c = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
+    // log2(e) / sqrt(128) / 2: with the half |q| / 8 may fill the f16 range; the scores are doubled again
+    const float c = 0.5f * 1.4426950408889634f * 0.08838834764831845f;
 #pragma unroll
     for (int ks = 0; ks < 8; ks++)
 #pragma unroll
@@ -506,8 +507,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
 #pragma unroll
     for (int n = 0; n < NG; n++) {
       // keys g (S[0], S[1]) and g + 8 (S[2], S[3]) for rows 2 tq, 2 tq + 1
-      const float s0 = v0 ? fmaf(S2[n][0], 1.f / kLift, S[n][0]) : -INFINITY, s1 = v0 ? fmaf(S2[n][1], 1.f / kLift, S[n][1]) : -INFINITY;
-      const float s2 = v1 ? fmaf(S2[n][2], 1.f / kLift, S[n][2]) : -INFINITY, s3 = v1 ? fmaf(S2[n][3], 1.f / kLift, S[n][3]) : -INFINITY;
+      auto score = [&](int j, bool on) { return on ? fmaf(S2[n][j], 2.f / kLift, S[n][j] + S[n][j]) : -INFINITY; };
+      const float s0 = score(0, v0), s1 = score(1, v0), s2 = score(2, v1), s3 = score(3, v1);
       float n0 = fmaxf(s0, s2), n1 = fmaxf(s1, s3);
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1) {
