@@ -107,3 +107,18 @@ def test_shared_prefix_largest_queries(cuda, kv, n, prefix):
     err = relative(s, range(0, n, max(1, n // 5)))
     print("relative error", err)
     assert err < R.LIMIT + 7e-7
+
+
+@pytest.mark.parametrize("kv,n,prefix", [("f16", 2, 512), ("f16", 1, 9000), ("f16", 40, 4000), ("f32", 3, 100), ("f32", 9, 4000),
+                                         ("f32", 40, 4000), ("f16", 3, 0), ("f32", 70, 0)])
+def test_shared_prefix_lengths_where_none_are_allowed(cuda, kv, n, prefix):
+    """max_len = 0: a length above it is flagged in every form, and the prefix alone is used."""
+    s = Shared(cuda, prefix, [0] * n, 16, 2, kv, seed=21, max_len=0)
+    K.attn_shared_prefix(**s.d)
+    s.check(range(0, n, max(1, n // 5)))
+    assert s.d["err"].item() == 0
+    s.d["lens"][n - 1] = 1
+    s.d["out"].fill_(5.0)
+    K.attn_shared_prefix(**s.d)
+    s.check(range(0, n, max(1, n // 5)))
+    assert s.d["err"].item() == 1

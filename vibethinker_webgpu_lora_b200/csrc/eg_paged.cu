@@ -422,8 +422,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
   if (FUSED) {
     if (k1 > a.max_len && a.err && threadIdx.x == 0) *a.err = 1;
     k1 = split < p.n_pref ? kmax : max(k0, min(k1, kmax));
-  } else if ((int)blockIdx.x >= pref) {
-    if (k1 > a.max_len && a.err && threadIdx.x == 0) *a.err = 1;
+  } else if ((int)blockIdx.x >= pref) {  // a length above max_len is flagged by the combine, which sees every one
     k1 = min(k1, kmax);
     if (k0 >= k1) {
       if (p.own) pdl_wait();
@@ -1076,6 +1075,7 @@ __global__ void __launch_bounds__(256 * kLanes) attn_shared_combine(const __grid
   const int ns = on ? a.p.n_pref + (min(len, a.max_len) + a.p.suf_keys - 1) / a.p.suf_keys : 0;
   const size_t row = part_row(a, 0, kvh, r), step = (size_t)a.nkv * a.p.groups * 8;  // rows of a split
   const float4* po = a.po + part_at(row, c);
+  if (len > a.max_len && a.err) *a.err = 1;
   pdl_wait();
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
