@@ -440,6 +440,9 @@ EG_API eg_status eg_op_kv_append_paged(const float* qkv, int64_t ld, int T, cons
  * the first lens[b] rows of the sequence's own pages (pages [nseq][max_pages]),
  * scores scaled by 1/sqrt(128); out rows ldo floats apart.  f32 results for
  * either cache type; |q|/8 and an f32 cache's values must lie in the f16 range.
+ * An infinity or NaN in q or in a row of the cache that counts, or a value past
+ * that range: the rows that meet it are not finite (or a key that scores
+ * -infinity has no weight); a result that is not finite sets err.
  * lens[b] = 0: the prefix alone; no key at all: zeros; lens[b] < 0: a padding
  * sequence, its out row is left as it was.  lens[b] > max_len: err, max_len
  * rows are used; a page outside the pool: err, its rows are left out.

@@ -122,3 +122,25 @@ def test_shared_prefix_lengths_where_none_are_allowed(cuda, kv, n, prefix):
     K.attn_shared_prefix(**s.d)
     s.check(range(0, n, max(1, n // 5)))
     assert s.d["err"].item() == 1
+
+
+@pytest.mark.parametrize("kv,n,prefix", [("f16", 2, 300), ("f16", 1, 9000), ("f16", 40, 4000), ("f32", 3, 100), ("f32", 40, 4000)])
+@pytest.mark.parametrize("where", ["prefix", "suffix"])
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_shared_prefix_values_that_are_not_finite(cuda, kv, n, prefix, where, what):
+    """An infinity of the cache (an f32 cache: any value past the f16 range): the
+    rows that meet it are flagged, all others are right."""
+    s = Shared(cuda, prefix, [60] * n, 16, 2, kv, seed=22)
+    row = R.rows_of(s.ppages, prefix)[prefix // 3] if where == "prefix" else R.rows_of(s.pages[n - 1], 60)[33]
+    c = s.d["k_cache" if what == "k" else "v_cache"].view(-1, 2, HD)
+    c[int(row), 1, 3] = float("inf") if kv == "f16" else 1e5
+    K.attn_shared_prefix(**s.d)
+    torch.cuda.synchronize()
+    assert s.d["err"].item() == 1
+    met = s.d["out"].view(n, 2, 8 * HD)[:, 1]  # the second KV head's
+    assert not torch.isfinite(met[n - 1]).all()
+    got = s.d["out"].cpu().numpy().astype(np.float64).reshape(n, 16, HD)
+    for b in range(0, n, max(1, n // 5)):
+        o, bound = s.want(b)
+        heads = slice(0, 16 if where == "suffix" and b < n - 1 else 8)
+        assert (abs(got[b] - o) <= bound)[heads].all()

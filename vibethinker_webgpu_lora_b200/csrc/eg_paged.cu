@@ -263,6 +263,15 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   return d;
 }
 
+// An output: o / l (no key at all: zeros).  What is not finite is flagged: q or a
+// key or value that is not, or an f32 cache's value past the f16 range.
+__device__ __forceinline__ void store_out(const SharedArgs& a, float* dst, float4 o, float l) {
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const float4 y = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  *reinterpret_cast<float4*>(dst) = y;
+  if (!(0.f * y.x + 0.f * y.y + 0.f * y.z + 0.f * y.w == 0.f) && a.err) *a.err = 1;
+}
+
 // One warp's walk over the 16-key tiles of a key range, 8 rows at a time.
 // S^T = K q^T and O^T = V^T p^T as mma.sync m16n8k16 (16 keys or dims x 8
 // rows), so the 8 query heads of a group fill the n side exactly.  q and p are
@@ -647,10 +656,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_shared_kernel(const __grid_c
           o.z += f * x[s].z;
           o.w += f * x[s].w;
         }
-      const float inv = l != 0.f ? 1.f / l : 0.f;  // no key at all: zeros
       const int rr = row0 + r;
-      reinterpret_cast<float4*>(a.out + (long long)(rr / G) * a.ldo + (kvh * G + rr % G) * kHeadDim)[c] =
-          make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      store_out(a, a.out + (long long)(rr / G) * a.ldo + (kvh * G + rr % G) * kHeadDim + 4 * c, o, l);
     }
     cl.sync();  // the parts are read
     return;
@@ -1148,9 +1155,7 @@ __global__ void __launch_bounds__(256 * kLanes) attn_shared_combine(const __grid
     }
   }
   if (!on) return;
-  const float inv = l != 0.f ? 1.f / l : 0.f;  // no key at all: zeros
-  reinterpret_cast<float4*>(a.out + b * a.ldo + (kvh * G + r % G) * kHeadDim)[c] =
-      make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  store_out(a, a.out + b * a.ldo + (kvh * G + r % G) * kHeadDim + 4 * c, o, l);
 }
 
 // The launches of one call: the prefix kernel (tcgen05), the suffix kernel
