@@ -144,3 +144,17 @@ def test_shared_prefix_values_that_are_not_finite(cuda, kv, n, prefix, where, wh
         o, bound = s.want(b)
         heads = slice(0, 16 if where == "suffix" and b < n - 1 else 8)
         assert (abs(got[b] - o) <= bound)[heads].all()
+
+
+@pytest.mark.parametrize("kv,n,prefix,longest", [
+    ("f16", 2, 256, 32), ("f16", 16, 2048, 640), ("f16", 3, 9001, 100), ("f16", 64, 2051, 200), ("f16", 130, 1000, 90),
+    ("f16", 300, 257, 30), ("f16", 40, 8192, 1024), ("f32", 2, 300, 60), ("f32", 17, 1001, 333), ("f32", 40, 4000, 200)])
+def test_shared_prefix_error_is_that_of_f32(cuda, kv, n, prefix, longest):
+    """Ordinary inputs in each form (one launch, warps, tensor cores, f32 in 4
+    and 8 warps): the relative error is R.LIMIT at most.  Without one of the lo
+    parts it is above 5e-5 (test_paged_limits.py)."""
+    s = Shared(cuda, prefix, [(i * 53) % (longest + 1) for i in range(n)], 16, 2, kv, seed=23, max_len=longest)
+    K.attn_shared_prefix(**s.d)
+    err = relative(s, range(0, n, max(1, n // 6)))
+    print("relative error", err)
+    assert err < R.LIMIT
