@@ -5,20 +5,25 @@ nvcc compiles the CUDA sources for `-gencode arch=compute_100a,code=sm_100a`
 with -ffp-contract=off so its arithmetic matches the reference's JS doubles
 operation by operation.  Objects go to _build/ beside this file, the shared
 library next to the package so it ships with the source tree, and beside it the
-Python binding of the ops on torch tensors (_ops, against the installed torch).
+Python binding of the ops on torch tensors (_ops, against the installed torch;
+left out where there is none: the library itself does not need it).
 """
 from __future__ import annotations
 
+import importlib.metadata
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libemberglass_cuda.so")
-OPS = os.path.join(HERE, "_ops.so")
+OPS = os.path.join(HERE, "_ops" + sysconfig.get_config_var("EXT_SUFFIX"))  # one for each Python
+OPS_TORCH = os.path.join(BUILD, "_ops.torch")  # the torch that it was built against
 INCLUDE = os.path.join(ROOT, "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -72,13 +77,23 @@ def build(verbose: bool = False, extra_nvflags: list[str] | None = None) -> str:
     return LIB
 
 
-def build_ops(verbose: bool = False) -> str:
-    """_ops.so: csrc/eg_torch.cpp against torch's headers and libraries and the
-    library above (found beside it at run time)."""
-    src = os.path.join(CSRC, "eg_torch.cpp")
-    if _stale(OPS, [src, __file__, os.path.join(INCLUDE, "emberglass.h")]):
-        import sysconfig
+def _torch() -> str | None:
+    """The installed torch, by version and place (not imported); None without one."""
+    spec = importlib.util.find_spec("torch")
+    return f"{importlib.metadata.version('torch')} {spec.origin}" if spec else None
 
+
+def build_ops(verbose: bool = False) -> str | None:
+    """The binding: csrc/eg_torch.cpp against torch's headers and libraries and the
+    library above (found beside it at run time).  Built again for another torch."""
+    src = os.path.join(CSRC, "eg_torch.cpp")
+    have = _torch()
+    if have is None:
+        print("torch is not installed: the library is built without the Python binding of its paged serving ops",
+              file=sys.stderr)
+        return None
+    built = open(OPS_TORCH).read() if os.path.exists(OPS_TORCH) else ""
+    if built != have or _stale(OPS, [src, __file__, os.path.join(INCLUDE, "emberglass.h")]):
         import torch
         from torch.utils.cpp_extension import include_paths, library_paths
         inc = [f for p in include_paths() + ["/usr/local/cuda/include"] for f in ("-isystem", p)]
@@ -87,6 +102,8 @@ def build_ops(verbose: bool = False) -> str:
               "-I", INCLUDE, *inc, "-isystem", sysconfig.get_paths()["include"], src, "-o", OPS, "-L", HERE,
               "-l:" + os.path.basename(LIB), *libs, "-lc10",
               "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], verbose)
+        with open(OPS_TORCH, "w") as f:
+            f.write(have)
     return OPS
 
 

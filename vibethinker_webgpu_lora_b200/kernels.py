@@ -124,7 +124,11 @@ def _ops():
     if _native is None:
         import torch  # noqa: F401  (its libraries, before the binding that links them)
         L.lib()
-        from . import _ops as native
+        try:
+            from . import _ops as native
+        except ImportError as e:
+            raise ImportError("the binding of the paged serving ops is missing, or not of this Python and torch: run "
+                              f"__graft_entry__.build() (python vibethinker_webgpu_lora_b200/build.py): {e}") from e
         _native = native
     return _native
 
