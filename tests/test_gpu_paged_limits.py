@@ -54,6 +54,21 @@ def test_sample_steps_far_above_the_temperature(cuda, t, share):
         check_sample(x, got, probs, t, k, p, 0.0, r)
 
 
+@pytest.mark.parametrize("value", [-9.5e29, -8.9e29, -1e28, -1e24, -1e22, -3e15, -1.0, -1e-20, 1e-42, 1e15, 6e21, 1e24, 1e30, 3e38])
+@pytest.mark.parametrize("n", [1, 41, 9001])
+def test_sample_equal_logits_of_any_size(cuda, n, value):
+    """A row of one value, and one of it and lower ones, at every size of the value."""
+    x = np.full((5, n), value, np.float32)
+    x[1, : n // 2] = -np.inf
+    x[2, n // 3:] = np.float32(value) - abs(np.float32(value)) / 16  # far below, or the same for the smallest
+    x[3, ::2] = np.nan
+    x[3, n - 1] = value
+    r = np.array([0.3, 0.5, 0.7, 0.9, 1.0], np.float32)
+    for t, k, p, m in [(1.0, 0, 1.0, 0.0), (0.05, 7, 1.0, 0.02), (1e-7, 0, 0.9, 0.0), (1e5, 0, 0.5, 0.3)]:
+        got, probs = run_sample(cuda, x, t, k, p, m, r)
+        check_sample(x, got, probs, t, k, p, m, r)
+
+
 # ---------------------------------------------------------------- attention
 def put(s, **kw):
     """Host arrays of a case, changed, to the device."""

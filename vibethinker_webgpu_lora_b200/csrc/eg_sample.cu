@@ -536,7 +536,7 @@ __device__ __forceinline__ void leader_ranges(FastSmem& S, cg::cluster_group& cl
   uint32_t cb, ncand, ca[kPer];
   warp_sums<kThreads>(S.wsum, mb, total);
   warp_sums<kThreads>(S.wcnt, cb, ncand);
-  last = (int)warp_max(lane < kThreads / 32 ? S.red[0][lane] : -1.f);
+  last = (int)warp_max(lane < kThreads / 32 ? fmaxf(S.red[0][lane], 0.f) : 0.f);
   double am = mb + (mi - ms);
   uint32_t ac = cb + (ci - cs);
   const bool k_on = P.k > 0 && (uint32_t)P.k < ncand;
@@ -862,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     const float all = (float)((fabs((double)mx) + (kBins - 4.0) * w) * 1.002);
     const float grid = __uint_as_float((__float_as_uint(all) & 0x7f800000u) - (23u << 23));
     B.xmax = mx;
-    B.width = ceilf(w / grid) * grid;
+    B.width = fmaxf(ceilf(w / grid), 1.f) * grid;  // w / grid may underflow
     // a grid far above t (t below a step of f32 at the maximum): steps of w, 2.01 t at
     // most, off the grid, which the 64-bit form takes, but no step that lets q pass 2^28
     const bool on_grid = B.width <= 2.5 * P.t;
@@ -1012,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   if (rank != 0) return;
 
   const int nl = (int)S.n_list;
-  if (nl > kList) {
+  if (nl > kList || nl == 0) {  // too many; or, should the bins ever miss a row's tokens, none: every row is written
     __syncthreads();
     sample_generic<kThreads>(a, row, *reinterpret_cast<GenericSmem*>(dsm));
     return;
