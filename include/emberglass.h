@@ -406,7 +406,8 @@ EG_API eg_status eg_op_sample_topk(const uint32_t* ids, const float* vals, int k
                                    float r, uint32_t* out, void* stream);
 
 /* ---------------- paged serving ops ----------------------------------------
- * Operators over the paged cache of eg_seq_init_paged's kind: pools
+ * Operators over a paged cache of the caller's, laid out as eg_seq_init_paged's
+ * slots are (whose own pool stays inside the runtime): pools
  * [n_pages][16][nkv][128] (f16 when kv_f16 else f32), row t of a sequence at
  * row t % 16 of page pages[t / 16].  Positions, slots, page ids and lengths
  * are read on the device, so a captured graph serves every step.  err: one
@@ -426,7 +427,7 @@ EG_API eg_status eg_op_sample_topk(const uint32_t* ids, const float* vals, int k
  * pos[t] < 0: a padding row, nothing of it is read on or written.  A position
  * outside the table or the slot's pages, a slot outside n_slots or a page
  * outside the pool: err, and nothing is written for that row.  Two rows with
- * the same slot and position in one call: either's values may stay.  qkv,
+ * the same slot and position in one call: each element is one of the two's.  qkv,
  * q_out, caches and tables 16-byte aligned, ld and ldq multiples of 4. */
 EG_API eg_status eg_op_kv_append_paged(const float* qkv, int64_t ld, int T, const int* pos, const int* slot,
                                        const uint32_t* pages, int n_slots, int max_pages, int n_pages,
@@ -434,12 +435,13 @@ EG_API eg_status eg_op_kv_append_paged(const float* qkv, int64_t ld, int T, cons
                                        const float* sin_t, int table_len, int nh, int nkv, int kv_f16,
                                        float* q_out, int64_t ldq, int* err, void* stream);
 /* One decode token of each of nseq sequences that share a prefix
- * (ATTN_PARTIAL_PAGED + ATTN_COMBINE, kernels.js:1657-1911, with the prefix
- * computed once for all): q row b (turned, nh heads of 128, ldq floats from
- * row to row) attends over the prefix_len rows of prefix_pages and then over
- * the first lens[b] rows of the sequence's own pages (pages [nseq][max_pages]),
- * scores scaled by 1/sqrt(128); out rows ldo floats apart.  f32 results for
- * either cache type; |q|/8 and an f32 cache's values must lie in the f16 range.
+ * (ATTN_PARTIAL_PAGED + ATTN_COMBINE, kernels.js:1657-1911; a long prefix is
+ * computed once for all of them, a short one for each where that is quicker):
+ * q row b (turned, nh heads of 128, ldq floats from row to row) attends over
+ * the prefix_len rows of prefix_pages and then over the first lens[b] rows of
+ * the sequence's own pages (pages [nseq][max_pages]), scores scaled by
+ * 1/sqrt(128); out rows ldo floats apart.  f32 results for either cache type;
+ * |q|/8 and an f32 cache's values must lie in the f16 range.
  * An infinity or NaN in q or in a row of the cache that counts, or a value past
  * that range: the rows that meet it are not finite (or a key that scores
  * -infinity has no weight); a result that is not finite sets err.

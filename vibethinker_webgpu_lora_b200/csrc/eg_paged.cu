@@ -60,8 +60,10 @@ __device__ __forceinline__ void store4<__half>(__half* d, float4 v) {
 
 // The bound is bytes, 512 read and 256 or 512 written a head.  U heads a half-
 // warp, their loads issued first: at 16384 tokens of 48 heads (743 MB) U = 2
-// runs at the copy rate (113 us, U = 1 120), at 512 tokens of 20 the launch and
-// three dependent loads are the time (U = 1 3.1 us, U = 2 3.5).
+// runs at the copy rate (112 us, U = 1 120), at 512 tokens of 20 the launch and
+// three dependent loads are the time (U = 1 3.2 us, U = 2 3.5).  The call takes
+// U = 2 from 131,072 heads on (0.94 of U = 1 there); below 36,000 heads it is
+// 0.95 to 1.28 of U = 1, from 40,000 to 131,072 0.93 to 0.99.
 template <typename KVT, int U>
 __global__ void __launch_bounds__(256) kv_append_paged_kernel(AppendArgs a) {
   const int H = a.nh + 2 * a.nkv, l = threadIdx.x & 15;
@@ -190,12 +192,20 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   p.rows = nseq * p.G;
   p.groups = (p.rows + 7) / 8;
   p.row_tiles = (p.rows + 127) / 128;
-  // What the prefix's scores number decides its kernel (16 heads, 2 KV heads):
-  // f16 on the tensor cores from 900,000 on (16 sequences x 2048 14.6 us there,
-  // 11.2 by warps; 16 x 4096 15.4 and 18.1; 64 x 1024 14.4 and 17.3); f32 in
-  // CTAs of 16 rows from 1,000,000 on; below, the prefix and the suffixes share a
-  // launch.  f32 takes 4 warps a CTA where there is work for them (16 x 512 9.4 us,
-  // 11.1 with 8; 64 x 8192 95 and 110; 4 x 32768 31 and 42; 2 x 8192 13.7 and 12.7).
+  // What the prefix's scores number decides its kernel: f16 on the tensor cores
+  // from 900,000 on (128 shapes of 16/2, 28/4 and 32/8 heads: 1.08 to 1.73 of the
+  // warps' time up to 530,000, 0.44 to 0.93 from 1,800,000 on, 0.86 to 1.33 about
+  // 900,000 to 1,050,000; 16 heads, 16 sequences x 2048: 15.0 and 10.1 us, x 4096
+  // 15.4 and 15.4, x 8192 17.0 and 25.1); f32 in CTAs of 16 rows from 1,000,000 on;
+  // below, the prefix and the suffixes share a launch.
+  // f32 takes 4 warps a CTA, two CTAs an SM, where there is work for them, else 8
+  // warps.  Over 582 shapes (those heads and 8/1, 1 to 64 sequences, prefixes of 128
+  // to 32768, own keys of 16 to 1024), 4 warps take of the time of 8, with 16 groups
+  // and KV heads or more: 0.84 to 1.13 (median 1.09) below 100,000 scores in all,
+  // 0.78 to 1.07 (0.95) to 138,000, 0.59 to 1.08 (0.83) above; with fewer: 0.77 to
+  // 1.35 (1.06) up to 1,500,000 of the prefix, 0.74 to 0.95 above (groups > 2: 0.74 to 0.85).
+  // The rule is within 0.8 % of the better one on the average, at worst 1.30 of it (1
+  // sequence of 32/8 heads, 2048 + 1024 keys).
   const long long scores = (long long)p.rows * nkv * prefix_len;
   p.tc = kv_f16 && prefix_len >= 256 && scores >= 900000;
   p.many = !kv_f16 && ((p.groups * nkv >= 16 && scores + (long long)p.rows * nkv * max_len >= 138000) ||
@@ -237,10 +247,12 @@ SharedPlan shared_plan(int nseq, int nh, int nkv, int prefix_len, int max_len, i
   // without a prefix has nothing to join and reads nothing twice: any number (32
   // sequences x 16 heads of their own x 128 keys 9.4 and 11.3).
   const int limit = kv_f16 ? 2 * kSms : kSms * 3 / 4;
-  // f16: longer splits where that makes 8 of them (16 x 2048 + 640 in 384 keys 10.3
-  // us, 12.0 in 8 of 256 and 5 of 128 with the combine; few pairs, which leave SMs
-  // to more splits, gain up to 384: 2 x 2048 + 2048 in 512 9.9 and 9.3; f32 loses:
-  // 2 x 1024 + 1024 in 256 9.8 and 9.0)
+  // f16: longer splits where that makes 8 of them, up to 512 keys, 384 with few
+  // pairs, which leave SMs to more splits (16 x 2048 + 640 in 384 keys 10.3 us, 12.0
+  // in 8 of 256 and 5 of 128 with the combine; 2 x 2048 + 2048 in 512 9.9 and 8.2; f32
+  // loses: 2 x 1024 + 1024 in 256 9.8 and 9.0).  Over 350 shapes that it changes, of
+  // the time without: 8 query heads a KV head 0.78 to 1.13, 1 to 7 of them, whose
+  // CTAs hold empty rows, 0.83 to 1.38 (8 x 3000 + 64 of 4/4 heads 11.0 and 8.0)
   if (kv_f16 && !p.own && p.n_pref + p.n_suf > 8 && pairs * 8 <= limit)
     for (int keys = 64; keys <= (pairs >= 8 ? 512 : 384); keys += 64) {
       const int np = (prefix_len + keys - 1) / keys, ns = (max_len + keys - 1) / keys;

@@ -276,15 +276,15 @@ __device__ __noinline__ void sample_generic(const SampleArgs& a, int row, Generi
 // usual form q stays within 2^26 +- 2^22 and two 32-bit shared-memory atomics
 // take the count and, modulo 2^32, the bits of kRound + q - 2^26: with the count
 // they give the sum of q above 2^26 - 2^22 (below 2^23 each: 512 tokens of a CTA
-// in one bin cannot overflow it; rows with more, or with steps of x / t above
-// 1/16, are counted again with 64-bit atomics, which cost three times as much).
+// in one bin cannot overflow it; rows with more are counted again, and rows with
+// steps of x / t above 1/16 at once, with 64-bit atomics: 256 rows of 151,936 118 us
+// in the usual form, 210 as bf16 values, 302 with a tenth of the tokens at -1e9).
 // The two atomics, 4 cycles of an SM each for a warp, bound the pass (38,000
 // tokens a CTA: 5.2 us).  The leader CTA turns the merged bins into running
-// counts and masses,
-// which fix each filter's and the sample's bin; only the tokens of those few
-// bins are gathered and put in order, in the same integers.
+// counts and masses, which fix each filter's and the sample's bin; only the tokens
+// of those few bins are gathered and put in order, in the same integers.
 // Tokens past the last bin (64 below the maximum in x / t or more) weigh
-// nothing: 150,000 of them are 2^-74 of the best token.
+// nothing: 2^20 of them are 2^-72 of the best token.
 namespace cg = cooperative_groups;
 
 constexpr int kBins = 2048;        // the last one: past the range
@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       }
     } else if (vec) {
       // eight tokens a thread, the next eight already on their way; they pass L1 by
-      // (256 rows: 132 us, 137 through it)
+      // (256 rows: 119 us, 123 through it)
       const int last = (e1 - e0) & ~3;  // up to here four at a time lie in the row
       const float4* x4 = reinterpret_cast<const float4*>(x + e0);
       auto load = [&](int i) {
@@ -1055,10 +1055,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 }
 
 // CTAs of a row's cluster: as many as leave every CTA an SM of its own, with
-// slices of 4096 tokens or longer (32 rows of 151936, top-p: 4 CTAs a row 38 us, 2
-// 45, 8 62; 64 rows: 2 45, 4 49; 256 rows: 1 114, 2 134); clusters of 8, which do
-// not fill the GPCs' SMs, for up to 12 rows (12 rows: 8 CTAs a row 28 us, 4 33; 16
-// rows: 44 and 37).
+// slices of 4096 tokens or longer, and clusters of 8, which do not fill the GPCs'
+// SMs, for up to 12 rows.  us a call for rows of 151,936 (top-p and min-p) by 1 / 2 /
+// 4 / 8 CTAs a row: 12 rows 57 / 39 / 31 / 26, 16 rows 57 / 39 / 31 / 42, 32 rows 58 /
+// 41 / 33 / 63, 64 rows 65 / 44 / 44 / 106, 256 rows 117 / 127 / 151 / 365; rows of
+// 32,000: 12 rows 22 / 21 / 18 / 19, 64 rows 22 / 21 / 24 / 77.  (13 rows would take 27
+// by 8 and take 32 by 4, 65 rows 45 by 2 and 65 by 1: clusters find room by GPCs.)
 int cluster_size(int rows, int n) {
   int c = 1;
   while (c < 8 && 2LL * rows * c <= (c == 4 ? 96 : 128) && n / (2 * c) >= 4096) c *= 2;
@@ -1095,8 +1097,8 @@ cudaError_t launch_sample(const SampleArgs& a, int c, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, sample_kernel<kThreads>, a, staged);
 }
 
-// 1024 threads for the few rows that take clusters of 8 (27 us against 29), else
-// 512, two CTAs an SM.
+// 1024 threads for the few rows that take clusters of 8 (1 row 25.3 us, 25.9 with
+// 512), else 512, two CTAs an SM (256 rows 117 us, 121 with 1024).
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
   const int c = cluster_size(a.rows, a.n);
   return c == 8 ? launch_sample<1024>(a, c, st) : launch_sample<512>(a, c, st);

@@ -156,9 +156,10 @@ def attn_shared_prefix(q, k_cache, v_cache, prefix_pages, prefix_len, pages, len
                        stream=None):
     """One decode token of each of nseq sequences over a shared prefix: q
     [nseq][nh * 128] attends over prefix_len rows of prefix_pages, then lens[b]
-    (<= max_len) rows of pages[b]; the prefix is computed once for all.  lens[b]
+    (<= max_len) rows of pages[b]; a long prefix is computed once for all.  lens[b]
     < 0 pads (out row left as it was).  ws: attn_shared_prefix_bytes(...) bytes
-    (uint8), one for each call that may overlap."""
+    (uint8), one for each call that may overlap.  err is set too when a result is
+    not finite."""
     L.check((_native or _ops()).attn_shared_prefix(q, k_cache, v_cache, prefix_pages, prefix_len, pages, lens, max_len,
                                                    out, ws, err, L.stream_ptr(stream)))
 
